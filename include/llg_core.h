@@ -53,6 +53,7 @@ enum {
 
 /* Element types of 16/32-bit tensors; values equal the reference's enum DType (csrc/tc_params.h:23). */
 enum { LLG_DT_NONE = 0, LLG_DT_BF16 = 1, LLG_DT_F16 = 2, LLG_DT_F32 = 3 };
+#define LLG_DT_E4M3 4  /* elements of a quantised key/value cache (llg_paged_kv); not a type of the entry points before it */
 
 /* Quantizer modes; values equal the reference's enum QuantMode (csrc/quant.h:9-14). */
 enum { LLG_QUANT_FP8_STATIC = 0, LLG_QUANT_FP8_PER_TOKEN = 1, LLG_QUANT_INT8_PER_TOKEN = 2, LLG_QUANT_NVFP4 = 3 };
@@ -267,6 +268,82 @@ LLG_API void llg_set_wait_limit(int64_t cycles);
 #define LLG_STATIC_WS_ELEMS (1 << 20)
 #define LLG_STATIC_COUNTERS 4096
 LLG_API int llg_tc_gemm_static_ws(const llg_tc_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Paged key/value cache of a decoder layer. k and v are [pages, kv_heads, page_size, head_dim] with any page, head and slot
+ * strides (elements; a multiple of 16 bytes each, pointers 16-byte aligned, unit stride inside a row), so both orders of heads
+ * and slots and interleaved k / v allocations are views of it. Token j of sequence i is row
+ * (page_table[i][j / page_size], head, j % page_size).
+ * Element types: BF16 or F16, or E4M3 with one e8m0 byte b per row in k_scale / v_scale [pages, kv_heads, page_size] (any
+ * strides, in bytes): a stored value x stands for x * 2^(b - 127).
+ * kv_lens[i] counts the tokens of sequence i in the cache, its new tokens included: they are the last ones. q_starts
+ * [batch + 1] gives the rows of the new tokens in the per-token tensors; NULL: every sequence has tokens / batch of them
+ * (tokens must be a multiple of batch). Rows at and behind q_starts[batch] belong to no sequence: they are neither read into
+ * the cache nor written. Lengths and offsets are read on the device only, so a captured call follows them from replay to replay.
+ * A length beyond table_width * page_size is cut to it. A page table entry in use that names no page (negative, or >= pages)
+ * is not followed: its rows are not written and read as zeros, and llg_device_status() returns 32. Sequences may share pages
+ * that a call only reads; the slots that one call writes must be distinct.
+ * No counterpart in the reference, which leaves the cache to the serving framework. */
+typedef struct llg_paged_kv {
+  void* k; void* v;
+  int64_t k_stride[3], v_stride[3];              /* page, head, slot */
+  void* k_scale; void* v_scale;                  /* E4M3 only, else NULL */
+  int64_t k_scale_stride[3], v_scale_stride[3];
+  const int32_t* page_table; int64_t table_stride;  /* [batch, table_width], row stride in elements */
+  const int32_t* kv_lens;                        /* [batch] */
+  const int32_t* q_starts;                       /* [batch + 1] or NULL */
+  int32_t dtype;                                 /* LLG_DT_BF16, LLG_DT_F16 or LLG_DT_E4M3 */
+  int32_t pages, kv_heads, page_size, head_dim;  /* head_dim a multiple of 16, at most 256 */
+  int32_t table_width, batch, tokens;
+} llg_paged_kv;
+
+/* Writes the new tokens' keys and values, k_in and v_in [tokens, kv_heads, head_dim], into the cache. E4M3: per row
+ * e = the smallest integer with max|x| * 2^-e <= 448, within [-100, 119] (-100 for a zero row); the value stored is
+ * e4m3(x * 2^-e), to nearest even, saturating, and the byte e + 127. BF16 / F16: a copy, in_dtype must be the cache's. */
+typedef struct llg_kv_append_args {
+  llg_paged_kv kv;
+  const void* k_in; const void* v_in;
+  int64_t k_in_stride[2], v_in_stride[2];        /* token, head; elements, multiples of 16 bytes */
+  int32_t in_dtype;                              /* LLG_DT_BF16, LLG_DT_F16, LLG_DT_F32 */
+} llg_kv_append_args;
+
+LLG_API int llg_kv_append(const llg_kv_append_args* args, void* stream);
+
+/* Reads the first max_len tokens of every sequence back: k_out and v_out [batch, max_len, kv_heads, head_dim], contiguous,
+ * zero behind kv_lens[i]. kv.q_starts and kv.tokens are not used. out_dtype: the cache's for BF16 / F16; BF16, F16 or F32 for E4M3. */
+typedef struct llg_kv_read_args {
+  llg_paged_kv kv;
+  void* k_out; void* v_out;
+  int32_t max_len, out_dtype;
+} llg_kv_read_args;
+
+LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
+
+/* Attention of every sequence's new tokens over its cached ones, the new ones included (append first). Query head h of
+ * `heads` reads kv head h / (heads / kv_heads). Query t of a sequence's n new tokens stands at position kv_len - n + t and
+ * sees key j when j <= position (causal) and j > position - window (window > 0); scores are scale * q . k, o = softmax v,
+ * lse = log of the sum of exp(scores) (natural, fp32). A query that sees no key gives o = 0 and lse = -inf.
+ * head_dim 64 or 128; q and out in the cache's 16-bit type, or either 16-bit type over E4M3; heads / kv_heads <= 32.
+ * With F16 queries an E4M3 value is used as F16 (its row's power of two applied). ws: llg_paged_attention_ws() bytes of
+ * scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
+typedef struct llg_attn_args {
+  llg_paged_kv kv;
+  const void* q; int64_t q_stride[2];            /* token, head; elements, multiples of 16 bytes */
+  void* out; int64_t out_stride[2];
+  float* lse; int64_t lse_stride;                /* NULL or [tokens, heads], unit stride over heads */
+  int32_t q_dtype, heads;
+  float scale;
+  int32_t causal, window;
+  void* ws; int64_t ws_bytes;
+} llg_attn_args;
+
+LLG_API int llg_paged_attention(const llg_attn_args* args, void* stream);
+/* Bytes of scratch llg_paged_attention needs for these arguments on the current device (ws itself is not looked at); at most
+ * a few megabytes per device, whatever the lengths are. Negative: LLG_E_*. */
+LLG_API int64_t llg_paged_attention_ws(const llg_attn_args* args);
+
+/* sizeof of llg_paged_kv, llg_kv_append_args, llg_kv_read_args, llg_attn_args as this library was compiled. */
+LLG_API void llg_attn_struct_sizes(int32_t out[4]);
 
 /* sizeof of llg_skinny_args, llg_tc_args, llg_quant_args, llg_gated_quant_args, llg_push_args as this library was
  * compiled: lets a foreign-function binding verify its struct layout before the first call. No counterpart in the

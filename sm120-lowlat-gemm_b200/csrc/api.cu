@@ -725,4 +725,125 @@ int llg_gated_quant(const llg_gated_quant_args* g, void* stream) {
   return LLG_OK;
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// paged key/value cache
+
+}  // extern "C"
+
+namespace {
+
+int kv_elem_bytes(int dt) { return dt == LLG_DT_F32 ? 4 : dt == LLG_DT_E4M3 ? 1 : 2; }
+
+// Strides of a tensor whose rows are read and written 16 bytes at a time.
+bool strides16(const int64_t* st, int n, int es) {
+  for (int i = 0; i < n; ++i)
+    if ((st[i] * es) % 16) return false;
+  return true;
+}
+
+int check_paged(const llg_paged_kv& c, bool new_tokens, const char* who) {
+  if (c.dtype != LLG_DT_BF16 && c.dtype != LLG_DT_F16 && c.dtype != LLG_DT_E4M3)
+    return fail(LLG_E_INVALID, "%s: the cache must be bf16, f16 or e4m3", who);
+  if (c.head_dim < 16 || c.head_dim > 256 || c.head_dim % 16)
+    return fail(LLG_E_INVALID, "%s: head_dim must be a multiple of 16 up to 256, got %d", who, c.head_dim);
+  if (c.pages < 0 || c.page_size < 1 || c.kv_heads < 1 || c.table_width < 0 || c.batch < 0 || c.tokens < 0)
+    return fail(LLG_E_INVALID, "%s: pages, page_size, kv_heads, table_width, batch or tokens out of range", who);
+  if ((int64_t)c.table_width * c.page_size > INT32_MAX / 2)
+    return fail(LLG_E_INVALID, "%s: the page table names more than %d tokens per sequence", who, INT32_MAX / 2);
+  if (new_tokens && !c.q_starts && c.batch > 0 && c.tokens % c.batch)
+    return fail(LLG_E_INVALID, "%s: without q_starts the %d tokens must be a multiple of the %d sequences", who, c.tokens, c.batch);
+  if ((c.dtype == LLG_DT_E4M3) != (c.k_scale != nullptr && c.v_scale != nullptr) || (c.k_scale == nullptr) != (c.v_scale == nullptr))
+    if (c.pages > 0) return fail(LLG_E_INVALID, "%s: an e4m3 cache needs k_scale and v_scale, a 16-bit cache takes none", who);
+  const int es = kv_elem_bytes(c.dtype);
+  if (!aligned(c.k, 16) || !aligned(c.v, 16) || !strides16(c.k_stride, 3, es) || !strides16(c.v_stride, 3, es))
+    return fail(LLG_E_INVALID, "%s: cache rows must be 16-byte aligned", who);
+  if (c.batch > 0 && c.tokens > 0 && (!c.kv_lens || (c.table_width > 0 && !c.page_table)))
+    return fail(LLG_E_INVALID, "%s: kv_lens and page_table must be device pointers", who);
+  return LLG_OK;
+}
+
+int launched(const char* who, cudaError_t e) {
+  if (e == cudaSuccess) return LLG_OK;
+  cudaGetLastError();
+  return fail(LLG_E_CUDA, "%s: launch failed (%s)", who, cudaGetErrorString(e));
+}
+
+int check_attn(const llg_attn_args* a) {
+  if (!a) return fail(LLG_E_INVALID, "null arguments");
+  const int rc = check_paged(a->kv, true, "paged_attention");
+  if (rc != LLG_OK) return rc;
+  const llg_paged_kv& c = a->kv;
+  if (c.head_dim != 64 && c.head_dim != 128) return fail(LLG_E_INVALID, "paged_attention: head_dim must be 64 or 128, got %d", c.head_dim);
+  if (a->q_dtype != LLG_DT_BF16 && a->q_dtype != LLG_DT_F16) return fail(LLG_E_INVALID, "paged_attention: q must be bf16 or f16");
+  if (c.dtype != LLG_DT_E4M3 && c.dtype != a->q_dtype) return fail(LLG_E_INVALID, "paged_attention: a 16-bit cache must have q's type");
+  if (a->heads < 1 || a->heads % c.kv_heads || a->heads / c.kv_heads > 32)
+    return fail(LLG_E_INVALID, "paged_attention: %d query heads must be 1 to 32 times the %d kv heads", a->heads, c.kv_heads);
+  if (a->window < 0) return fail(LLG_E_INVALID, "paged_attention: window must be 0 (none) or the number of keys a query sees");
+  if (!aligned(a->q, 16) || !aligned(a->out, 16) || !strides16(a->q_stride, 2, 2) || !strides16(a->out_stride, 2, 2))
+    return fail(LLG_E_INVALID, "paged_attention: rows of q and out must be 16-byte aligned");
+  return LLG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llg_kv_append(const llg_kv_append_args* a, void* stream) {
+  if (!a) return fail(LLG_E_INVALID, "null arguments");
+  const int rc = check_paged(a->kv, true, "kv_append");
+  if (rc != LLG_OK) return rc;
+  if (a->in_dtype < LLG_DT_BF16 || a->in_dtype > LLG_DT_F32) return fail(LLG_E_INVALID, "kv_append: k and v must be bf16, f16 or f32");
+  if (a->kv.dtype != LLG_DT_E4M3 && a->in_dtype != a->kv.dtype) return fail(LLG_E_INVALID, "kv_append: a 16-bit cache takes keys and values of its own type");
+  const int es = kv_elem_bytes(a->in_dtype);
+  if (!aligned(a->k_in, 16) || !aligned(a->v_in, 16) || !strides16(a->k_in_stride, 2, es) || !strides16(a->v_in_stride, 2, es))
+    return fail(LLG_E_INVALID, "kv_append: rows of k and v must be 16-byte aligned");
+  if (a->kv.batch == 0 || a->kv.tokens == 0 || a->kv.pages == 0 || a->kv.table_width == 0) return LLG_OK;
+  if ((int64_t)a->kv.tokens * a->kv.kv_heads > INT32_MAX / 8) return fail(LLG_E_INVALID, "kv_append: too many rows in one call");
+  unsigned* st = status_word_device_ptr();
+  if (!st) return fail(LLG_E_CUDA, "no device status word");
+  return launched("kv_append", kv_append_launch(*a, st, static_cast<cudaStream_t>(stream)));
+}
+
+int llg_kv_read(const llg_kv_read_args* a, void* stream) {
+  if (!a) return fail(LLG_E_INVALID, "null arguments");
+  const int rc = check_paged(a->kv, false, "kv_read");
+  if (rc != LLG_OK) return rc;
+  if (a->max_len < 0) return fail(LLG_E_INVALID, "kv_read: max_len must not be negative");
+  if (a->kv.dtype == LLG_DT_E4M3 ? (a->out_dtype < LLG_DT_BF16 || a->out_dtype > LLG_DT_F32) : a->out_dtype != a->kv.dtype)
+    return fail(LLG_E_INVALID, "kv_read: the output must have a 16-bit cache's type, or be bf16, f16 or f32 for an e4m3 cache");
+  if (a->kv.batch == 0 || a->max_len == 0) return LLG_OK;
+  if (!a->k_out || !a->v_out || !aligned(a->k_out, 16) || !aligned(a->v_out, 16)) return fail(LLG_E_INVALID, "kv_read: outputs must be 16-byte aligned");
+  if (!a->kv.kv_lens || (a->kv.table_width > 0 && !a->kv.page_table)) return fail(LLG_E_INVALID, "kv_read: kv_lens and page_table must be device pointers");
+  if ((int64_t)a->kv.batch * a->max_len > INT32_MAX / 8 || (int64_t)a->kv.batch * a->max_len * a->kv.kv_heads > INT32_MAX)
+    return fail(LLG_E_INVALID, "kv_read: too many rows in one call");
+  unsigned* st = status_word_device_ptr();
+  if (!st) return fail(LLG_E_CUDA, "no device status word");
+  return launched("kv_read", kv_read_launch(*a, st, static_cast<cudaStream_t>(stream)));
+}
+
+int64_t llg_paged_attention_ws(const llg_attn_args* a) {
+  const int rc = check_attn(a);
+  return rc == LLG_OK ? attn_workspace(*a) : rc;
+}
+
+int llg_paged_attention(const llg_attn_args* a, void* stream) {
+  const int rc = check_attn(a);
+  if (rc != LLG_OK) return rc;
+  if (a->kv.batch == 0 || a->kv.tokens == 0) return LLG_OK;
+  if (!a->q || !a->out) return fail(LLG_E_INVALID, "paged_attention: q and out must be device pointers");
+  const int64_t need = attn_workspace(*a);
+  if (a->ws_bytes < need || !a->ws || !aligned(a->ws, 16))
+    return fail(LLG_E_INVALID, "paged_attention: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)need, (long long)a->ws_bytes);
+  unsigned* st = status_word_device_ptr();
+  if (!st) return fail(LLG_E_CUDA, "no device status word");
+  return launched("paged_attention", attn_launch(*a, st, static_cast<cudaStream_t>(stream)));
+}
+
+void llg_attn_struct_sizes(int32_t out[4]) {
+  out[0] = (int32_t)sizeof(llg_paged_kv);
+  out[1] = (int32_t)sizeof(llg_kv_append_args);
+  out[2] = (int32_t)sizeof(llg_kv_read_args);
+  out[3] = (int32_t)sizeof(llg_attn_args);
+}
+
 }  // extern "C"

@@ -1,0 +1,504 @@
+// Attention of few query rows per key/value head over a paged cache (one token, drafted tokens): bound by the bytes of K and V.
+//
+//   s = scale * q . k,  m = max s,  l = sum exp(s - m),  o = sum exp(s - m) v / l       one pass, running m, l and o
+//
+// Key tiles of 64 tokens; each of the CTA's four warps owns 16 of them with its own cp.async ring, softmax state and
+// accumulators, so nothing between the loads and the last merge synchronises more than a warp. The products are taken
+// transposed, S^T[16 keys x rows] = K Q^T and O^T[head_dim x rows] = V^T P^T, so that the rows - 8 for a group of eight heads
+// and one token - are the narrow side (8) of mma.m16n8k16 and no row of the tensor-core tile is padding.
+//   16-bit cache: K by ldmatrix, V by ldmatrix.trans.
+//   e4m3 cache: 16-byte reads of a row give a thread 16 neighbouring values; the order of head_dim inside a product is free, so
+//     they serve four consecutive k steps of K Q^T (Q is read in the same order) and eight row blocks of V^T without any
+//     transposition. bf16: the byte's exponent and mantissa are put into a bf16 as they are, which reads as value * 2^-120
+//     (subnormals included); Q and P carry 2^60 each and the fp32 results the rest, so no multiply is spent per value.
+//     f16: cvt gives the value itself. The row's power of two multiplies the score (K, in fp32) and the probability (V, bf16,
+//     exact there) or the value (V, f16, whose range is too small for the probability to carry it).
+// P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
+// The running maximum moves only when a score exceeds it by more than 2^8: p <= 256 then, and the shuffles and the rescaling of
+// O are skipped for almost every tile.
+#pragma once
+
+#include "paged_kv.cuh"
+
+namespace llg {
+
+constexpr int kRowsKT = 64;       // keys per unit, 16 per warp
+constexpr int kRowsWarps = 4;
+constexpr int kRowsThreads = 32 * kRowsWarps;
+constexpr int kRowsSmem = 96 * 1024;  // two CTAs per SM
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+};
+template <>
+struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+};
+
+// Two e4m3 bytes of `w` (picked by the byte-permutation selectors of w and v) as a pair of 16-bit operands.
+// bf16: value * 2^-120.  f16: the value.
+template <typename T>
+struct Widen;
+template <>
+struct Widen<__nv_bfloat16> {
+  static constexpr bool kScaled = true;
+  // bytes 1 and 3 of `w` -> bf16 pair
+  static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7f007f00u) >> 4) | (w & 0x80008000u); }
+  static __device__ __forceinline__ void four(uint32_t w, uint32_t& lo, uint32_t& hi) {  // bytes 0,1 -> lo; 2,3 -> hi
+    lo = odd(__byte_perm(w, 0u, 0x1404));
+    hi = odd(__byte_perm(w, 0u, 0x3424));
+  }
+  // (a.b0, b.b0) (a.b1, b.b1) (a.b2, b.b2) (a.b3, b.b3)
+  static __device__ __forceinline__ void cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
+    o[0] = odd(__byte_perm(a, b, 0x4404));
+    o[1] = odd(__byte_perm(a, b, 0x5515));
+    o[2] = odd(__byte_perm(a, b, 0x6626));
+    o[3] = odd(__byte_perm(a, b, 0x7737));
+  }
+};
+template <>
+struct Widen<__half> {
+  static constexpr bool kScaled = false;
+  static __device__ __forceinline__ uint32_t pair(uint32_t v) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+    return r;
+  }
+  static __device__ __forceinline__ void four(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = pair(w & 0xffffu);
+    hi = pair(w >> 16);
+  }
+  static __device__ __forceinline__ void cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
+    const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
+    o[0] = pair(x & 0xffffu);
+    o[1] = pair(x >> 16);
+    o[2] = pair(y & 0xffffu);
+    o[3] = pair(y >> 16);
+  }
+};
+
+__device__ __forceinline__ float pow2_of(uint32_t biased) { return __uint_as_float(biased << 23); }
+
+template <typename T, bool FP8, int D, int NB>
+struct RowsCfg {
+  static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
+  static constexpr int kChunks = kRowBytes / 16;      // 16-byte pieces per row
+  static constexpr int kStage = 2 * 16 * kRowBytes + (FP8 ? 32 : 0);  // per warp: K, V, the rows' scale bytes
+  static constexpr int kStages = [] {
+    const int n = kRowsSmem / kRowsWarps / kStage;
+    return n > 8 ? 8 : n;
+  }();
+  static constexpr int kRing = kStages * kStage;      // per warp
+  static constexpr int kRows = NB * 8;
+  static constexpr int kPad = D + 4;                  // floats between rows of the merge buffer
+  static constexpr int kMerge = kRowsWarps * kRows * (kPad + 2) * 4;
+  static constexpr int kSmem = kRowsWarps * kRing > kMerge ? kRowsWarps * kRing : kMerge;
+};
+
+template <typename T, bool FP8, int D, int NB>
+__global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid_constant__ AttnDev p) {
+  using Cfg = RowsCfg<T, FP8, D, NB>;
+  constexpr int S = Cfg::kStages, CH = Cfg::kChunks, KS = D / 16, MB = D / 16;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long scratch[kRowsWarps + 4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int quad = lane & 3, oct = lane >> 2;  // fragment coordinates
+  pdl_trigger();
+  pdl_wait();
+  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  Share share = find_share<kRowsKT, kRowsThreads>(p, scratch);
+  const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
+  const PagedKV& c = p.c;
+  constexpr float kUp = 1.152921504606846976e18f;  // 2^60
+
+  Segment g;
+  while (next_segment<kRowsKT>(p, share, g)) {
+    const int rows = g.toks * p.group;
+    const int nb_used = (rows + 7) >> 3;
+    const int pos0 = g.s.len - g.s.n + g.tok0;  // position of the tile's first token
+
+    // ---- queries: B fragments of K Q^T, row oct of each block
+    uint32_t qf[NB][KS][2];
+    int first_key[NB][2], last_key[NB][2];  // keys that rows 2 * quad, 2 * quad + 1 of a block see: [first, last]
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = nb * 8 + oct;
+      const bool ok = row < rows;
+      const int tok = row / p.group, hh = row - tok * p.group;
+      const unsigned char* src = p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint2 v = make_uint2(0u, 0u);
+        if (ok) {
+          if constexpr (FP8) {  // the order in which a thread holds a row of K: 16 * (quad + 4 i) + 4 j
+            const int i = ks >> 2, j = ks & 3;
+            v = *reinterpret_cast<const uint2*>(src + 2 * (16 * (quad + 4 * i) + 4 * j));
+          } else {
+            v.x = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad));
+            v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
+          }
+        }
+        if constexpr (FP8 && Widen<T>::kScaled) {
+          const __nv_bfloat162 up = __floats2bfloat162_rn(kUp, kUp);
+          *reinterpret_cast<__nv_bfloat162*>(&v.x) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v.x), up);
+          *reinterpret_cast<__nv_bfloat162*>(&v.y) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v.y), up);
+        }
+        qf[nb][ks][0] = v.x;
+        qf[nb][ks][1] = v.y;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nb * 8 + 2 * quad + e;
+        const int pos = pos0 + r / p.group;
+        last_key[nb][e] = r < rows ? (p.causal ? min(pos, g.s.len - 1) : g.s.len - 1) : -1;
+        first_key[nb][e] = p.window > 0 ? pos - p.window + 1 : 0;
+      }
+    }
+
+    float o[NB][MB][4];
+    float m[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[nb][mb][0] = o[nb][mb][1] = o[nb][mb][2] = o[nb][mb][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+    }
+
+    // ---- the warp's ring: tile t holds keys [64 t + 16 warp, + 16)
+    const int nt = g.tile1 - g.tile0;
+    int64_t row_off = -1;   // lanes 0-15: byte offset of K's row for key `lane` of the next tile; 16-31: of V's row; -1: no row
+    uint32_t pend = 0;      // scale byte of the row loaded last
+    uint32_t pend_at = 0;
+    auto locate = [&](int t) {  // fills row_off (and starts the load of the scale byte) for tile t
+      const int key = (g.tile0 + t) * kRowsKT + warp * 16 + (lane & 15);
+      row_off = -1;
+      if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
+        const int block = key / c.page_size, slot = key - block * c.page_size;
+        const int pg = page_of(c, g.seq, block);
+        if (pg >= 0) {
+          row_off = lane < 16 ? pg * c.k_page + g.head * c.k_head + slot * c.k_slot
+                              : pg * c.v_page + g.head * c.v_head + slot * c.v_slot;
+          if constexpr (FP8) {
+            const unsigned char* sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot
+                                                : c.vs + pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot;
+            pend = *sc;
+          }
+        }
+      }
+    };
+    auto issue = [&](int t) {  // starts the copies of tile t, located by the call before
+      const uint32_t base = ring + (t % S) * Cfg::kStage;
+      if (t < nt) {
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+          const int at = lane + 32 * i, row = at / CH, ch = at % CH;
+          const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
+          int kc, vc;
+          if constexpr (FP8) {
+            kc = D == 128 ? ch ^ ((row & 1) << 2) : ch;
+            vc = D == 128 ? ch ^ (row & 6) : ch ^ ((row >> 1) & 3);
+          } else {
+            kc = vc = ch ^ (row & 7);
+          }
+          cp_async16(base + row * Cfg::kRowBytes + kc * 16, c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
+          cp_async16(base + (16 + row) * Cfg::kRowBytes + vc * 16, c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+        }
+        if constexpr (FP8) pend_at = base + 32 * Cfg::kRowBytes + lane;
+      }
+      cp_async_commit();
+    };
+    auto settle = [&]() {  // the scale byte requested with the last located tile goes into that tile's stage
+      if constexpr (FP8) {
+        if (pend_at != 0u) asm volatile("st.shared.u8 [%0], %1;" ::"r"(pend_at), "r"(row_off >= 0 ? pend : 0u) : "memory");
+        pend_at = 0u;
+      }
+    };
+    for (int t = 0; t < S - 1; ++t) {
+      locate(t);
+      issue(t);
+      settle();
+    }
+    locate(S - 1);
+
+    for (int t = 0; t < nt; ++t) {
+      cp_async_wait<S - 2>();
+      __syncwarp();
+      const uint32_t kb = ring + (t % S) * Cfg::kStage, vb = kb + 16 * Cfg::kRowBytes;
+      issue(t + S - 1);  // into the stage that the warp finished reading one tile ago
+      settle();
+
+      // ---- S^T = K Q^T: thread holds keys oct, oct + 8 of rows 2 * quad, 2 * quad + 1 of each block
+      float s[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const int ch = quad + 4 * i;
+          const uint4 r0 = lds16(kb + oct * Cfg::kRowBytes + (D == 128 ? ch ^ ((oct & 1) << 2) : ch) * 16);
+          const uint4 r1 = lds16(kb + (oct + 8) * Cfg::kRowBytes + (D == 128 ? ch ^ ((oct & 1) << 2) : ch) * 16);
+          const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a[4];
+            Widen<T>::four(w0[j], a[0], a[2]);
+            Widen<T>::four(w1[j], a[1], a[3]);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              if (nb < nb_used) Mma<T>::run(s[nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t a[4];
+          const int row = lane & 15, ch = 2 * ks + (lane >> 4);
+          ldsm_x4(kb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            if (nb < nb_used) Mma<T>::run(s[nb], a, qf[nb][ks][0], qf[nb][ks][1]);
+        }
+      }
+
+      // ---- softmax
+      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16 + oct;
+      float f0 = p.scale_log2, f1 = p.scale_log2, pv0 = 1.f, pv1 = 1.f;  // of keys oct, oct + 8
+      if constexpr (FP8) {
+        uint32_t b[4];
+        const uint32_t at = kb + 32 * Cfg::kRowBytes + oct;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[0]) : "r"(at) : "memory");
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[1]) : "r"(at + 8) : "memory");
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[2]) : "r"(at + 16) : "memory");
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[3]) : "r"(at + 24) : "memory");
+        constexpr float up = Widen<T>::kScaled ? kUp : 1.f;
+        f0 *= pow2_of(b[0]) * up;
+        f1 *= pow2_of(b[1]) * up;
+        if constexpr (Widen<T>::kScaled) {
+          pv0 = pow2_of(b[2]) * up;
+          pv1 = pow2_of(b[3]) * up;
+        }
+      }
+      uint32_t pf[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if (nb >= nb_used) continue;
+        float x[4];
+        bool more = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + (e >> 1) * 8;
+          const bool seen = key <= last_key[nb][e & 1] && key >= first_key[nb][e & 1];
+          x[e] = seen ? s[nb][e] * (e < 2 ? f0 : f1) : -INFINITY;
+          more |= x[e] > m[nb][e & 1] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(x[e], x[e + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float top = fmaxf(m[nb][e], mx);
+            const float keep = m[nb][e] == -INFINITY ? 0.f : exp2_fast(m[nb][e] - top);
+            m[nb][e] = top;
+            l[nb][e] *= keep;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+              o[nb][mb][e] *= keep;
+              o[nb][mb][e + 2] *= keep;
+            }
+          }
+        }
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float mm = m[nb][e & 1];
+          pr[e] = exp2_fast(x[e] - (mm == -INFINITY ? 0.f : mm));
+          l[nb][e & 1] += pr[e];
+        }
+        pf[nb][0] = transpose8x8(Mma<T>::pack(pr[0] * pv0, pr[1] * pv0));
+        pf[nb][1] = transpose8x8(Mma<T>::pack(pr[2] * pv1, pr[3] * pv1));
+      }
+
+      // ---- O^T += V^T P^T
+      if constexpr (FP8) {
+        uint32_t sc[2] = {0u, 0u};  // f16: the rows' powers of two, keys (2 quad, 2 quad + 1) and those + 8
+        if constexpr (!Widen<T>::kScaled) {
+          uint32_t b0, b1;
+          const uint32_t at = kb + 32 * Cfg::kRowBytes + 16 + 2 * quad;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(b0) : "r"(at) : "memory");
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(b1) : "r"(at + 8) : "memory");
+          sc[0] = Mma<T>::pack(pow2_of(b0 & 0xffu), pow2_of(b0 >> 8));
+          sc[1] = Mma<T>::pack(pow2_of(b1 & 0xffu), pow2_of(b1 >> 8));
+        }
+        constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (head_dim = 16 * oct + ..., or 8 * oct + ...)
+        uint32_t w[4][W];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 2 * quad + (r & 1) + (r >> 1) * 8;
+          if constexpr (D == 128) {
+            const uint4 v = lds16(vb + row * Cfg::kRowBytes + (oct ^ (row & 6)) * 16);
+            w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+          } else {
+            const uint2 v = lds8(vb + row * Cfg::kRowBytes + ((oct >> 1) ^ ((row >> 1) & 3)) * 16 + (oct & 1) * 8);
+            w[r][0] = v.x; w[r][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          uint32_t lo[4], hi[4];
+          Widen<T>::cross(w[0][j], w[1][j], lo);
+          Widen<T>::cross(w[2][j], w[3][j], hi);
+          if constexpr (!Widen<T>::kScaled) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              *reinterpret_cast<__half2*>(&lo[e]) = __hmul2(*reinterpret_cast<__half2*>(&lo[e]), *reinterpret_cast<__half2*>(&sc[0]));
+              *reinterpret_cast<__half2*>(&hi[e]) = __hmul2(*reinterpret_cast<__half2*>(&hi[e]), *reinterpret_cast<__half2*>(&sc[1]));
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              if (nb < nb_used) Mma<T>::run(o[nb][2 * j + h], a, pf[nb][0], pf[nb][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          uint32_t a[4];
+          const int row = (lane & 7) + ((lane >> 4) << 3), ch = 2 * mb + ((lane >> 3) & 1);
+          ldsm_x4_t(vb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            if (nb < nb_used) Mma<T>::run(o[nb][mb], a, pf[nb][0], pf[nb][1]);
+        }
+      }
+      __syncwarp();          // every lane has read the stage before the next issue overwrites it
+      locate(t + S);
+    }
+    cp_async_wait<0>();
+
+    // ---- the four warps' states become one
+    __syncthreads();
+    float* const mo = reinterpret_cast<float*>(smem);                      // [warp][row][kPad]
+    float* const mm = mo + kRowsWarps * Cfg::kRows * Cfg::kPad;             // [warp][row]
+    float* const ml = mm + kRowsWarps * Cfg::kRows;
+    constexpr float kDown = FP8 && Widen<T>::kScaled ? kUp : 1.f;           // what is left of 2^-120 in the accumulators
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      if (nb >= nb_used) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = nb * 8 + 2 * quad + e;
+        float sum = l[nb][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (oct == 0) {
+          mm[warp * Cfg::kRows + row] = m[nb][e];
+          ml[warp * Cfg::kRows + row] = sum;
+        }
+        float* const dst = mo + (warp * Cfg::kRows + row) * Cfg::kPad;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          const int d0 = FP8 ? (D / 8) * oct + 2 * mb : 16 * mb + oct, d1 = FP8 ? d0 + 1 : d0 + 8;
+          dst[d0] = o[nb][mb][e] * kDown;
+          dst[d1] = o[nb][mb][e + 2] * kDown;
+        }
+      }
+    }
+    __syncthreads();
+    const int slot = part_slot(blockIdx.x, g.starts);
+    for (int i = tid; i < rows * (D / 4); i += kRowsThreads) {
+      const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, mm[w * Cfg::kRows + row]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) {
+        const float f = exp2_fast(mm[w * Cfg::kRows + row] - base);
+        sum += f * ml[w * Cfg::kRows + row];
+        const float4 v = *reinterpret_cast<const float4*>(mo + (w * Cfg::kRows + row) * Cfg::kPad + d);
+        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      }
+      if (g.whole) {
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const int tok = row / p.group, head = g.head * p.group + row - tok * p.group;
+        const int64_t t = g.s.t0 + g.tok0 + tok;
+        *reinterpret_cast<uint2*>(p.out + t * p.o_tok + head * p.o_head + 2 * d) =
+            make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
+        if (p.lse && d == 0) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (base + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * Cfg::kRows + row) * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * Cfg::kRows + row) * 2) = make_float2(top, sum);
+      }
+    }
+    if (g.starts && !g.whole && tid == 0) p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows);
+    __syncthreads();
+  }
+}
+
+}  // namespace llg

@@ -22,6 +22,7 @@ enum : uint32_t {
   ST_SKINNY_CONVERT_WAIT = 7,  // skinny GEMV: activation converters waited for a stage to land
   ST_SKINNY_COMPUTE_WAIT = 8,  // skinny GEMV: compute warps waited for a full stage
   ST_ALLREDUCE_WAIT = 16,      // all-reduce: a peer's signal did not arrive
+  ST_BAD_PAGE = 32,            // paged cache: a page table entry named no page of the cache (its rows read as zeros)
 };
 unsigned int* status_word_device_ptr();  // device address of the status word of the current device (cached)
 
@@ -115,6 +116,19 @@ struct GatedExtra {
   int64_t ldact;
 };
 cudaError_t quant_launch(const llg_quant_args& a, const GatedExtra& g, cudaStream_t s);
+
+// ---- paged key/value cache (kv_cache.cu, attn_*.cu) --------------------------------------------------------------
+struct PagedKV;
+struct AttnDev;
+PagedKV paged_view(const llg_paged_kv& a, unsigned* status);
+cudaError_t kv_append_launch(const llg_kv_append_args& a, unsigned* status, cudaStream_t s);
+cudaError_t kv_read_launch(const llg_kv_read_args& a, unsigned* status, cudaStream_t s);
+int64_t attn_workspace(const llg_attn_args& a);
+cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s);
+cudaError_t attn_rows_launch_bf16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_rows_launch_f16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
+// ctas: those of the kernel that left the partial results; tile_rows: rows of one of its tiles.
+cudaError_t attn_combine_launch(const AttnDev& p, bool f16, int ctas, int tile_rows, cudaStream_t s);
 
 // ---- block-scale layouts (relayout.cu) ---------------------------------------------------------------------------
 // Row-major [rows, cols] bytes (row pitch ld) <-> tiles of 128 rows x 4 columns, 512 bytes each, padded to whole tiles.

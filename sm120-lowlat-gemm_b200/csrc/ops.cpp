@@ -1,7 +1,8 @@
 // torch.ops.lowlat_gemm.* as a C++ torch extension (module lowlat_gemm._C): the thin layer between tensors and the C ABI
 // of libllg_core.so.
 //
-// Stands in for the reference's binding layer csrc/ops.cpp:420-451 - the same seven schemas, CUDA implementations for the
+// Stands in for the reference's binding layer csrc/ops.cpp:420-451 - the same seven schemas (and three for the paged key/value
+// cache, which the reference has not), CUDA implementations for the
 // compute ops, a Meta implementation for the functional skinny op, an empty Python module whose import registers them.
 // Each op checks what only a tensor knows (device, dtype, rank, contiguity), puts raw pointers, sizes and strides into
 // the C-ABI descriptor and calls the library on the current CUDA stream of the operand's device, under a device guard.
@@ -242,6 +243,133 @@ void quant(const Tensor& x, Tensor& q, const OptTensor& sf, const OptTensor& sca
   lib_check(llg_quant(&a, stream_of(x)));
 }
 
+// ---- paged key/value cache ---------------------------------------------------------------------------------------
+
+int kv_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? LLG_DT_E4M3 : t == at::kFloat ? LLG_DT_NONE : dt_code(t); }
+
+void cache_side(const Tensor& ref, const Tensor& t, const OptTensor& scale, bool e4m3, const char* name, const char* scale_name, void** ptr,
+                int64_t* stride, void** sptr, int64_t* sstride) {
+  on_device_of(ref, t, name);
+  TORCH_CHECK(t.dim() == 4 && t.stride(3) == 1, "lowlat_gemm: ", name, " must be [pages, kv_heads, page_size, head_dim] with unit last stride");
+  *ptr = t.data_ptr();
+  for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+  TORCH_CHECK(scale.has_value() == e4m3, "lowlat_gemm: ", scale_name, e4m3 ? " is needed with an e4m3 cache" : " belongs to an e4m3 cache");
+  if (!e4m3) return;
+  on_device_of(ref, *scale, scale_name);
+  TORCH_CHECK((scale->scalar_type() == at::kFloat8_e8m0fnu || scale->scalar_type() == at::kByte) && scale->dim() == 3 &&
+                  scale->size(0) == t.size(0) && scale->size(1) == t.size(1) && scale->size(2) == t.size(2),
+              "lowlat_gemm: ", scale_name, " must be a float8_e8m0fnu (or uint8) tensor [", t.size(0), ", ", t.size(1), ", ", t.size(2), "]");
+  *sptr = scale->data_ptr();
+  for (int i = 0; i < 3; ++i) sstride[i] = scale->stride(i);
+}
+
+llg_paged_kv paged(const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scale, const OptTensor& v_scale,
+                   const Tensor& page_table, const Tensor& kv_lens, const OptTensor& q_starts, int64_t tokens) {
+  TORCH_CHECK(k_cache.is_cuda(), "lowlat_gemm: k_cache must be on CUDA");
+  llg_paged_kv c{};
+  c.dtype = kv_code(k_cache.scalar_type());
+  TORCH_CHECK(c.dtype != LLG_DT_NONE && v_cache.scalar_type() == k_cache.scalar_type(),
+              "lowlat_gemm: k_cache and v_cache must both be bfloat16, float16 or float8_e4m3fn, got ", k_cache.scalar_type(), " and ",
+              v_cache.scalar_type());
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "lowlat_gemm: k_cache and v_cache must have one shape, got ", k_cache.sizes(), " and ",
+              v_cache.sizes());
+  const bool e4m3 = c.dtype == LLG_DT_E4M3;
+  cache_side(k_cache, k_cache, k_scale, e4m3, "k_cache", "k_scale", &c.k, c.k_stride, &c.k_scale, c.k_scale_stride);
+  cache_side(k_cache, v_cache, v_scale, e4m3, "v_cache", "v_scale", &c.v, c.v_stride, &c.v_scale, c.v_scale_stride);
+  on_device_of(k_cache, page_table, "page_table");
+  on_device_of(k_cache, kv_lens, "kv_lens");
+  TORCH_CHECK(kv_lens.scalar_type() == at::kInt && kv_lens.dim() == 1 && kv_lens.is_contiguous(),
+              "lowlat_gemm: kv_lens must be a contiguous int32 vector");
+  const int64_t batch = kv_lens.size(0);
+  TORCH_CHECK(page_table.scalar_type() == at::kInt && page_table.dim() == 2 && page_table.size(0) == batch &&
+                  (page_table.stride(1) == 1 || page_table.size(1) <= 1),
+              "lowlat_gemm: page_table must be int32 [", batch, ", pages per sequence] with unit last stride");
+  if (q_starts.has_value()) {
+    on_device_of(k_cache, *q_starts, "q_starts");
+    TORCH_CHECK(q_starts->scalar_type() == at::kInt && q_starts->dim() == 1 && q_starts->is_contiguous() && q_starts->size(0) == batch + 1,
+                "lowlat_gemm: q_starts must be a contiguous int32 vector of ", batch + 1, " elements");
+    c.q_starts = q_starts->data_ptr<int32_t>();
+  }
+  for (int64_t v : {k_cache.size(0), k_cache.size(1), k_cache.size(2), page_table.size(1), batch, tokens})
+    TORCH_CHECK(v <= INT32_MAX, "lowlat_gemm: paged cache: a size does not fit 32 bits");
+  c.page_table = page_table.data_ptr<int32_t>();
+  c.table_stride = page_table.stride(0);
+  c.kv_lens = kv_lens.data_ptr<int32_t>();
+  c.pages = (int32_t)k_cache.size(0); c.kv_heads = (int32_t)k_cache.size(1); c.page_size = (int32_t)k_cache.size(2);
+  c.head_dim = (int32_t)k_cache.size(3);
+  c.table_width = (int32_t)page_table.size(1); c.batch = (int32_t)batch; c.tokens = (int32_t)tokens;
+  return c;
+}
+
+void kv_append(const Tensor& k, const Tensor& v, Tensor& k_cache, Tensor& v_cache, const OptTensor& k_scale, const OptTensor& v_scale,
+               const Tensor& page_table, const Tensor& kv_lens, const OptTensor& q_starts) {
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.stride(2) == 1 && v.stride(2) == 1 && k.sizes() == v.sizes(),
+              "lowlat_gemm: k and v must be [tokens, kv_heads, head_dim] with unit last stride");
+  llg_kv_append_args a{};
+  a.kv = paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, k.size(0));
+  on_device_of(k_cache, k, "k");
+  on_device_of(k_cache, v, "v");
+  TORCH_CHECK(k.size(1) == k_cache.size(1) && k.size(2) == k_cache.size(3), "lowlat_gemm: k is ", k.sizes(), " but the cache holds ",
+              k_cache.size(1), " heads of ", k_cache.size(3));
+  TORCH_CHECK(dt_code(k.scalar_type()) != LLG_DT_NONE && v.scalar_type() == k.scalar_type(),
+              "lowlat_gemm: k and v must both be bfloat16, float16 or float32");
+  a.k_in = k.data_ptr(); a.v_in = v.data_ptr();
+  a.in_dtype = dt_code(k.scalar_type());
+  for (int i = 0; i < 2; ++i) { a.k_in_stride[i] = k.stride(i); a.v_in_stride[i] = v.stride(i); }
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  lib_check(llg_kv_append(&a, stream_of(k_cache)));
+}
+
+void kv_read(Tensor& k_out, Tensor& v_out, const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scale, const OptTensor& v_scale,
+             const Tensor& page_table, const Tensor& kv_lens) {
+  llg_kv_read_args a{};
+  a.kv = paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, std::nullopt, 0);
+  on_device_of(k_cache, k_out, "k_out");
+  on_device_of(k_cache, v_out, "v_out");
+  TORCH_CHECK(k_out.dim() == 4 && k_out.is_contiguous() && v_out.is_contiguous() && k_out.sizes() == v_out.sizes() &&
+                  k_out.size(0) == kv_lens.size(0) && k_out.size(2) == k_cache.size(1) && k_out.size(3) == k_cache.size(3),
+              "lowlat_gemm: k_out and v_out must be contiguous [", kv_lens.size(0), ", max_len, ", k_cache.size(1), ", ", k_cache.size(3), "]");
+  TORCH_CHECK(dt_code(k_out.scalar_type()) != LLG_DT_NONE && v_out.scalar_type() == k_out.scalar_type() && k_out.size(1) <= INT32_MAX,
+              "lowlat_gemm: k_out and v_out must both be bfloat16, float16 or float32");
+  a.k_out = k_out.data_ptr(); a.v_out = v_out.data_ptr();
+  a.max_len = (int32_t)k_out.size(1); a.out_dtype = dt_code(k_out.scalar_type());
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  lib_check(llg_kv_read(&a, stream_of(k_cache)));
+}
+
+void paged_attention(Tensor& out, const OptTensor& lse, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scale,
+                     const OptTensor& v_scale, const Tensor& page_table, const Tensor& kv_lens, const OptTensor& q_starts, double scale,
+                     bool causal, int64_t window) {
+  TORCH_CHECK(q.dim() == 3 && out.dim() == 3 && q.stride(2) == 1 && out.stride(2) == 1 && q.sizes() == out.sizes(),
+              "lowlat_gemm: q and out must be [tokens, heads, head_dim] with unit last stride");
+  llg_attn_args a{};
+  a.kv = paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, q.size(0));
+  on_device_of(k_cache, q, "q");
+  on_device_of(k_cache, out, "out");
+  TORCH_CHECK(q.size(2) == k_cache.size(3), "lowlat_gemm: q has head_dim ", q.size(2), " but the cache ", k_cache.size(3));
+  TORCH_CHECK(out.scalar_type() == q.scalar_type(), "lowlat_gemm: out must have q's type");
+  TORCH_CHECK(q.size(1) <= INT32_MAX && window >= 0 && window <= INT32_MAX, "lowlat_gemm: paged_attention: heads or window out of range");
+  a.q = q.data_ptr(); a.out = out.data_ptr();
+  for (int i = 0; i < 2; ++i) { a.q_stride[i] = q.stride(i); a.out_stride[i] = out.stride(i); }
+  if (lse.has_value()) {
+    on_device_of(k_cache, *lse, "lse");
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == q.size(0) && lse->size(1) == q.size(1) &&
+                    (lse->stride(1) == 1 || lse->size(1) <= 1), "lowlat_gemm: lse must be float32 [tokens, heads] with unit last stride");
+    a.lse = lse->data_ptr<float>();
+    a.lse_stride = lse->stride(0);
+  }
+  a.q_dtype = dt_code(q.scalar_type()); a.heads = (int32_t)q.size(1);
+  a.scale = (float)scale; a.causal = causal; a.window = (int32_t)window;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const int64_t need = llg_paged_attention_ws(&a);
+  TORCH_CHECK(need >= 0, llg_last_error());
+  // Scratch of this call alone, from the caching allocator: it belongs to the stream (and, in a capture, to the graph's own
+  // pool), so calls on other streams and other graphs never share it.
+  const Tensor ws = at::empty({need}, k_cache.options().dtype(at::kByte));
+  a.ws = ws.data_ptr(); a.ws_bytes = need;
+  lib_check(llg_paged_attention(&a, stream_of(k_cache)));
+}
+
 // ---- facts and switches ------------------------------------------------------------------------------------------
 
 std::vector<int64_t> tc_info(int64_t kind, int64_t cfg) {
@@ -264,6 +392,12 @@ TORCH_LIBRARY(lowlat_gemm, m) {
         "Tensor? alpha_t, float alpha, int kind, bool swap, bool bias_on_p, int cfg, int stages, int ksplit, Tensor ws, "
         "Tensor counters, bool cluster=False, Tensor? prefetch=None, int prefetch_bytes=0) -> ()");
   m.def("quant(Tensor x, Tensor(a!) q, Tensor(b!)? sf, Tensor? scale_in, Tensor(c!)? scale_out, int mode, float min_scale) -> ()");
+  m.def("kv_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, "
+        "Tensor page_table, Tensor kv_lens, Tensor? q_starts) -> ()");
+  m.def("kv_read(Tensor(a!) k_out, Tensor(b!) v_out, Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, "
+        "Tensor page_table, Tensor kv_lens) -> ()");
+  m.def("paged_attention(Tensor(a!) out, Tensor(b!)? lse, Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, "
+        "Tensor page_table, Tensor kv_lens, Tensor? q_starts, float scale, bool causal, int window) -> ()");
   m.def("tc_info(int kind, int cfg) -> int[]", &tc_info);
   m.def("set_pdl(bool on) -> ()", &set_pdl);
   m.def("pdl_enabled() -> bool", &pdl_enabled);
@@ -274,6 +408,9 @@ TORCH_LIBRARY_IMPL(lowlat_gemm, CUDA, m) {
   m.impl("skinny_out", &skinny_out);
   m.impl("tc_gemm", &tc_gemm);
   m.impl("quant", &quant);
+  m.impl("kv_append", &kv_append);
+  m.impl("kv_read", &kv_read);
+  m.impl("paged_attention", &paged_attention);
 }
 
 TORCH_LIBRARY_IMPL(lowlat_gemm, Meta, m) { m.impl("skinny", &skinny_meta); }

@@ -1,0 +1,236 @@
+// What the cache writer, the cache reader and the attention kernels share: the device view of a paged key/value cache and the
+// split of a ragged attention problem into equal shares of key tiles.
+//
+// Cache rows: token j of sequence i is row (page_table[i, j / page_size], head, j % page_size) of k and v. Page, head and slot
+// strides are 64-bit byte offsets. An e4m3 cache holds beside each row of head_dim values one e8m0 byte b, the row's power of
+// two 2^(b - 127): e4m3 has the same relative step at every scale inside its normal range, so a power of two loses nothing
+// against an amax / 448 scale, and value * 2^(b - 127) is exact in bf16 and fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "llg_internal.h"
+#include "ptx_sm100.cuh"
+
+namespace llg {
+
+struct PagedKV {
+  unsigned char *k, *v;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;          // bytes
+  unsigned char *ks, *vs;
+  int64_t ks_page, ks_head, ks_slot, vs_page, vs_head, vs_slot;    // bytes
+  const int* table;
+  int64_t table_stride;
+  const int* lens;
+  const int* starts;  // or null: every sequence has q_len new tokens
+  int pages, kv_heads, page_size, head_dim, table_width, batch, tokens, q_len;
+  unsigned* status;
+};
+
+struct SeqView {
+  int t0, n, len;  // first row of its new tokens in q / k / v, their number, tokens in the cache with them
+};
+
+// Offsets that point outside the call's tensors are cut to them, lengths to what the page table can name.
+__device__ __forceinline__ SeqView seq_view(const PagedKV& c, int i) {
+  SeqView s;
+  if (c.starts) {
+    s.t0 = min(max(c.starts[i], 0), c.tokens);
+    s.n = min(max(c.starts[i + 1], s.t0), c.tokens) - s.t0;
+  } else {
+    s.t0 = i * c.q_len;
+    s.n = c.q_len;
+  }
+  const int64_t most = (int64_t)c.table_width * c.page_size;
+  s.len = (int)min((int64_t)max(c.lens[i], 0), most);
+  return s;
+}
+
+// Page of token j, or -1 (recorded in the status word) when the table's entry names no page of the cache.
+__device__ __forceinline__ int page_of(const PagedKV& c, int seq, int block) {
+  const int pg = c.table[(int64_t)seq * c.table_stride + block];
+  if ((unsigned)pg < (unsigned)c.pages) return pg;
+  atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+  return -1;
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------
+// Rows of a sequence are packed token-major over the query heads that share a key/value head: row = token * group + head in
+// group. An item is (sequence, kv head, tile of whole tokens); it walks the key tiles that any of its rows sees. All items'
+// key tiles, counted through, are cut into equal shares, one per CTA: every CTA streams the same number of tiles whatever the
+// lengths are. An item that a share boundary cuts leaves one partial result per CTA (unnormalised sums in fp32, row maximum,
+// row sum); attn_combine_kernel adds them in order of the CTAs, so results do not depend on timing.
+struct AttnDev {
+  PagedKV c;
+  const unsigned char* q;
+  int64_t q_tok, q_head;  // bytes
+  unsigned char* out;
+  int64_t o_tok, o_head;  // bytes
+  float* lse;
+  int64_t lse_tok;        // elements; heads are contiguous
+  int group;              // query heads per kv head
+  int causal, window;
+  float scale_log2;       // softmax scale * log2(e)
+  int row_min, row_max;   // this launch serves sequences with row_min < new tokens * group <= row_max
+  int tok_tile;           // whole tokens per row tile
+  float* part_o;          // [slots][rows per tile][head_dim]
+  float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
+  int4* split;            // [CTAs]: the item that starts, cut, at the end of a CTA's share: {parts, first token, kv head, rows}
+};
+
+// Keys [lo, hi) that any row of token tile [tf, tf + cnt) sees.
+struct KeyRange {
+  int lo, hi;
+};
+__device__ __forceinline__ KeyRange key_range(const AttnDev& p, const SeqView& s, int tf, int cnt) {
+  KeyRange r;
+  r.hi = p.causal ? min(max(s.len - s.n + tf + cnt, 0), s.len) : s.len;
+  r.lo = p.window > 0 ? max(s.len - s.n + tf + 1 - p.window, 0) : 0;
+  r.lo = min(r.lo, r.hi);
+  return r;
+}
+template <int KT>
+__device__ __forceinline__ int key_tiles(const KeyRange& r) {
+  return max((r.hi + KT - 1) / KT - r.lo / KT, 1);  // an item without keys still writes its rows
+}
+
+__device__ __forceinline__ int token_tiles(const AttnDev& p, const SeqView& s) {
+  const int64_t rows = (int64_t)s.n * p.group;
+  return rows > p.row_min && rows <= p.row_max ? (s.n + p.tok_tile - 1) / p.tok_tile : 0;
+}
+
+// Key tiles of one kv head of a sequence, over all of its token tiles.
+template <int KT>
+__device__ __forceinline__ long long seq_units(const AttnDev& p, const SeqView& s) {
+  long long u = 0;
+  const int nt = token_tiles(p, s);
+  for (int r = 0; r < nt; ++r) {
+    const int tf = r * p.tok_tile;
+    u += key_tiles<KT>(key_range(p, s, tf, min(p.tok_tile, s.n - tf)));
+  }
+  return u;
+}
+
+// A CTA's share of the key tiles and its place in the walk.
+struct Share {
+  long long u, end, per;  // next unit, end of the share, units per CTA
+  int seq;
+  long long off;          // units of `seq` (over all kv heads) before u
+};
+
+// Every thread of the CTA takes part. scratch: NT / 32 + 4 long longs of shared memory.
+template <int KT, int NT>
+__device__ __forceinline__ Share find_share(const AttnDev& p, long long* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  long long* part = scratch;             // NT / 32 warp sums
+  long long* found = scratch + NT / 32;  // {seq, units before the sequence}
+  long long mine = 0, first = 0;
+  for (int i = tid; i < p.c.batch; i += NT) {
+    const long long u = seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
+    if (i == tid) first = u;
+    mine += u;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) part[warp] = mine;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) total += part[w];
+  __syncthreads();
+  Share sh;
+  sh.per = (total + gridDim.x - 1) / gridDim.x;
+  sh.u = sh.per * blockIdx.x;
+  sh.end = min(total, sh.u + sh.per);
+  sh.seq = 0;
+  sh.off = 0;
+  if (sh.u >= sh.end) return sh;
+  long long base = 0;
+  for (int c0 = 0; c0 < p.c.batch; c0 += NT) {
+    const int i = c0 + tid;
+    const long long x = i >= p.c.batch ? 0 : c0 == 0 ? first : seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
+    long long inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    long long before = base, chunk = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) before += part[w];
+      chunk += part[w];
+    }
+    const long long lo = before + inc - x;
+    if (x > 0 && lo <= sh.u && sh.u < lo + x) {
+      found[0] = i;
+      found[1] = sh.u - lo;
+    }
+    __syncthreads();
+    if (found[0] >= 0) break;
+    base += chunk;
+  }
+  sh.seq = (int)found[0];
+  sh.off = found[1];
+  __syncthreads();
+  return sh;
+}
+
+// The next piece of the walk: key tiles [tile0, tile1) of one item.
+struct Segment {
+  int seq, head, tok0, toks;   // sequence, kv head, first token within the sequence's new ones, tokens
+  SeqView s;
+  KeyRange keys;
+  int tile0, tile1;            // key tiles, counted from key 0
+  bool starts, whole;          // the segment begins its item / is all of it
+  int parts;                   // CTAs that share the item, when this segment begins it
+};
+
+template <int KT>
+__device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segment& g) {
+  if (sh.u >= sh.end) return false;
+  long long per_head;
+  for (;;) {
+    if (sh.seq >= p.c.batch) return false;
+    g.s = seq_view(p.c, sh.seq);
+    per_head = seq_units<KT>(p, g.s);
+    if (per_head > 0) break;
+    ++sh.seq;  // nothing of this sequence belongs to this launch
+    sh.off = 0;
+  }
+  g.seq = sh.seq;
+  g.head = (int)(sh.off / per_head);
+  long long rem = sh.off - g.head * per_head;
+  int units;
+  for (int r = 0;; ++r) {
+    g.tok0 = r * p.tok_tile;
+    g.toks = min(p.tok_tile, g.s.n - g.tok0);
+    g.keys = key_range(p, g.s, g.tok0, g.toks);
+    units = key_tiles<KT>(g.keys);
+    if (rem < units) break;
+    rem -= units;
+  }
+  const long long left = sh.end - sh.u;
+  const int take = (int)min((long long)units - rem, left);
+  g.tile0 = g.keys.lo / KT + (int)rem;
+  g.tile1 = g.tile0 + take;
+  g.starts = rem == 0;
+  g.whole = g.starts && take == units;
+  g.parts = g.starts ? (int)((sh.u + units - 1) / sh.per - blockIdx.x) + 1 : 0;
+  sh.u += take;
+  sh.off += take;
+  if (sh.off == per_head * p.c.kv_heads) {
+    ++sh.seq;
+    sh.off = 0;
+  }
+  return true;
+}
+
+// A cut item's part of this CTA: slot 1 when the CTA begins the item (at the end of its share), else slot 0.
+__device__ __forceinline__ int part_slot(int cta, bool starts) { return 2 * cta + (starts ? 1 : 0); }
+
+}  // namespace llg

@@ -58,6 +58,33 @@ class PushArgs(C.Structure):
                 ("flags", c_ptr * 8), ("done", c_ptr)]
 
 
+class PagedKV(C.Structure):
+    _fields_ = [
+        ("k", c_ptr), ("v", c_ptr), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("k_scale", c_ptr), ("v_scale", c_ptr), ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("page_table", c_ptr), ("table_stride", c_i64), ("kv_lens", c_ptr), ("q_starts", c_ptr),
+        ("dtype", c_i32), ("pages", c_i32), ("kv_heads", c_i32), ("page_size", c_i32), ("head_dim", c_i32),
+        ("table_width", c_i32), ("batch", c_i32), ("tokens", c_i32),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("kv", PagedKV), ("k_in", c_ptr), ("v_in", c_ptr), ("k_in_stride", c_i64 * 2), ("v_in_stride", c_i64 * 2),
+                ("in_dtype", c_i32)]
+
+
+class KvReadArgs(C.Structure):
+    _fields_ = [("kv", PagedKV), ("k_out", c_ptr), ("v_out", c_ptr), ("max_len", c_i32), ("out_dtype", c_i32)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [
+        ("kv", PagedKV), ("q", c_ptr), ("q_stride", c_i64 * 2), ("out", c_ptr), ("out_stride", c_i64 * 2),
+        ("lse", c_ptr), ("lse_stride", c_i64), ("q_dtype", c_i32), ("heads", c_i32), ("scale", c_f32),
+        ("causal", c_i32), ("window", c_i32), ("ws", c_ptr), ("ws_bytes", c_i64),
+    ]
+
+
 # every symbol include/llg_core.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "llg_skinny": (c_i32, [C.POINTER(SkinnyArgs), c_ptr]),
@@ -79,6 +106,11 @@ SYMBOLS = {
     "llg_set_wait_limit": (None, [c_i64]),
     "llg_sf_relayout": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_i64, c_i32, c_ptr]),
     "llg_tc_gemm_host": (c_i32, [C.POINTER(TcArgs), c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_ptr]),
+    "llg_kv_append": (c_i32, [C.POINTER(KvAppendArgs), c_ptr]),
+    "llg_kv_read": (c_i32, [C.POINTER(KvReadArgs), c_ptr]),
+    "llg_paged_attention": (c_i32, [C.POINTER(AttnArgs), c_ptr]),
+    "llg_paged_attention_ws": (c_i64, [C.POINTER(AttnArgs)]),
+    "llg_attn_struct_sizes": (None, [C.POINTER(c_i32 * 4)]),
     "llg_device_status": (c_i32, [C.POINTER(C.c_uint32)]),
     "llg_struct_sizes": (None, [C.POINTER(c_i32 * 5)]),
     "llg_last_error": (C.c_char_p, []),
@@ -111,6 +143,11 @@ def _load() -> C.CDLL:
     sizes = (c_i32 * 5)()
     lib.llg_struct_sizes(C.byref(sizes))
     want = (C.sizeof(SkinnyArgs), C.sizeof(TcArgs), C.sizeof(QuantArgs), C.sizeof(GatedQuantArgs), C.sizeof(PushArgs))
+    if tuple(sizes) != want:
+        raise ImportError(f"lowlat_gemm: struct layout mismatch, library {tuple(sizes)} vs binding {want}")
+    sizes = (c_i32 * 4)()
+    lib.llg_attn_struct_sizes(C.byref(sizes))
+    want = (C.sizeof(PagedKV), C.sizeof(KvAppendArgs), C.sizeof(KvReadArgs), C.sizeof(AttnArgs))
     if tuple(sizes) != want:
         raise ImportError(f"lowlat_gemm: struct layout mismatch, library {tuple(sizes)} vs binding {want}")
     return lib

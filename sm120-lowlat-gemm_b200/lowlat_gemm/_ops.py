@@ -1,7 +1,8 @@
 """torch.ops.lowlat_gemm.*: the custom-op boundary, with the schema strings of the reference's TORCH_LIBRARY block
 (csrc/ops.cpp:420-440) so callers written against it (tests, tools, serving hooks) work unchanged.
 
-Two registrations of the same seven ops exist, both thin layers over the C ABI of libllg_core:
+Two registrations of the same ops exist - the reference's seven and three for the paged key/value cache - both thin layers
+over the C ABI of libllg_core:
   * the C++ torch extension lowlat_gemm._C (csrc/ops.cpp, the counterpart of the reference's extension module): used
     whenever it has been built;
   * this module's torch.library registration over ctypes: the torch-free binding's sibling, used when _C is absent or
@@ -49,6 +50,12 @@ if BACKEND == "ctypes":
                 "int prefetch_bytes=0) -> ()")
     _lib.define("quant(Tensor x, Tensor(a!) q, Tensor(b!)? sf, Tensor? scale_in, Tensor(c!)? scale_out, int mode, "
                 "float min_scale) -> ()")
+    _lib.define("kv_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, "
+                "Tensor page_table, Tensor kv_lens, Tensor? q_starts) -> ()")
+    _lib.define("kv_read(Tensor(a!) k_out, Tensor(b!) v_out, Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, "
+                "Tensor page_table, Tensor kv_lens) -> ()")
+    _lib.define("paged_attention(Tensor(a!) out, Tensor(b!)? lse, Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scale, "
+                "Tensor? v_scale, Tensor page_table, Tensor kv_lens, Tensor? q_starts, float scale, bool causal, int window) -> ()")
     _lib.define("tc_info(int kind, int cfg) -> int[]")
     _lib.define("set_pdl(bool on) -> ()")
     _lib.define("pdl_enabled() -> bool")
@@ -245,6 +252,106 @@ def _quant(x, q, sf, scale_in, scale_out, mode, min_scale):
         N.check(N.lib.llg_quant(C.byref(a), _stream(x)))
 
 
+_KV_DT = {torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 4}
+_SCALE_DT = (torch.uint8, getattr(torch, "float8_e8m0fnu", torch.uint8))
+
+
+def _paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, tokens: int) -> N.PagedKV:
+    _need(k_cache.is_cuda, "k_cache must be on CUDA")
+    _need(k_cache.dtype in _KV_DT and v_cache.dtype == k_cache.dtype, "k_cache and v_cache must both be bfloat16, float16 or "
+          f"float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
+    _need(k_cache.shape == v_cache.shape, f"k_cache and v_cache must have one shape, got {list(k_cache.shape)} and {list(v_cache.shape)}")
+    c = N.PagedKV()
+    c.dtype = _KV_DT[k_cache.dtype]
+    e4m3 = c.dtype == 4
+    for name, t, scale in (("k", k_cache, k_scale), ("v", v_cache, v_scale)):
+        _same_device(k_cache, t, f"{name}_cache")
+        _need(t.dim() == 4 and t.stride(3) == 1, f"{name}_cache must be [pages, kv_heads, page_size, head_dim] with unit last stride")
+        _need((scale is not None) == e4m3, f"{name}_scale is needed with an e4m3 cache" if e4m3 else f"{name}_scale belongs to an e4m3 cache")
+        setattr(c, name, t.data_ptr())
+        setattr(c, name + "_stride", (C.c_int64 * 3)(*t.stride()[:3]))
+        if e4m3:
+            _same_device(k_cache, scale, f"{name}_scale")
+            _need(scale.dtype in _SCALE_DT and scale.shape == t.shape[:3],
+                  f"{name}_scale must be a float8_e8m0fnu (or uint8) tensor {list(t.shape[:3])}")
+            setattr(c, name + "_scale", scale.data_ptr())
+            setattr(c, name + "_scale_stride", (C.c_int64 * 3)(*scale.stride()))
+    _same_device(k_cache, page_table, "page_table")
+    _same_device(k_cache, kv_lens, "kv_lens")
+    _need(kv_lens.dtype == torch.int32 and kv_lens.dim() == 1 and kv_lens.is_contiguous(), "kv_lens must be a contiguous int32 vector")
+    batch = kv_lens.shape[0]
+    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == batch
+          and (page_table.stride(1) == 1 or page_table.shape[1] <= 1),
+          f"page_table must be int32 [{batch}, pages per sequence] with unit last stride")
+    if q_starts is not None:
+        _same_device(k_cache, q_starts, "q_starts")
+        _need(q_starts.dtype == torch.int32 and q_starts.dim() == 1 and q_starts.is_contiguous() and q_starts.shape[0] == batch + 1,
+              f"q_starts must be a contiguous int32 vector of {batch + 1} elements")
+        c.q_starts = q_starts.data_ptr()
+    _need(max(*k_cache.shape[:3], page_table.shape[1], batch, tokens) < 2**31, "paged cache: a size does not fit 32 bits")
+    c.page_table, c.table_stride, c.kv_lens = page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr()
+    c.pages, c.kv_heads, c.page_size, c.head_dim = k_cache.shape
+    c.table_width, c.batch, c.tokens = page_table.shape[1], batch, tokens
+    return c
+
+
+def _kv_append(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts):
+    _need(k.dim() == 3 and v.dim() == 3 and k.stride(2) == 1 and v.stride(2) == 1 and k.shape == v.shape,
+          "k and v must be [tokens, kv_heads, head_dim] with unit last stride")
+    a = N.KvAppendArgs()
+    a.kv = _paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, k.shape[0])
+    _same_device(k_cache, k, "k")
+    _same_device(k_cache, v, "v")
+    _need(k.shape[1] == k_cache.shape[1] and k.shape[2] == k_cache.shape[3],
+          f"k is {list(k.shape)} but the cache holds {k_cache.shape[1]} heads of {k_cache.shape[3]}")
+    _need(k.dtype in _DT and v.dtype == k.dtype, "k and v must both be bfloat16, float16 or float32")
+    a.k_in, a.v_in, a.in_dtype = k.data_ptr(), v.data_ptr(), _DT[k.dtype]
+    a.k_in_stride, a.v_in_stride = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
+    with torch.cuda.device(k_cache.device):
+        N.check(N.lib.llg_kv_append(C.byref(a), _stream(k_cache)))
+
+
+def _kv_read(k_out, v_out, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens):
+    a = N.KvReadArgs()
+    a.kv = _paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, None, 0)
+    _same_device(k_cache, k_out, "k_out")
+    _same_device(k_cache, v_out, "v_out")
+    _need(k_out.dim() == 4 and k_out.is_contiguous() and v_out.is_contiguous() and k_out.shape == v_out.shape
+          and k_out.shape[0] == kv_lens.shape[0] and k_out.shape[2] == k_cache.shape[1] and k_out.shape[3] == k_cache.shape[3],
+          f"k_out and v_out must be contiguous [{kv_lens.shape[0]}, max_len, {k_cache.shape[1]}, {k_cache.shape[3]}]")
+    _need(k_out.dtype in _DT and v_out.dtype == k_out.dtype and k_out.shape[1] < 2**31,
+          "k_out and v_out must both be bfloat16, float16 or float32")
+    a.k_out, a.v_out, a.max_len, a.out_dtype = k_out.data_ptr(), v_out.data_ptr(), k_out.shape[1], _DT[k_out.dtype]
+    with torch.cuda.device(k_cache.device):
+        N.check(N.lib.llg_kv_read(C.byref(a), _stream(k_cache)))
+
+
+def _paged_attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, scale, causal, window):
+    _need(q.dim() == 3 and out.dim() == 3 and q.stride(2) == 1 and out.stride(2) == 1 and q.shape == out.shape,
+          "q and out must be [tokens, heads, head_dim] with unit last stride")
+    a = N.AttnArgs()
+    a.kv = _paged(k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts, q.shape[0])
+    _same_device(k_cache, q, "q")
+    _same_device(k_cache, out, "out")
+    _need(q.shape[2] == k_cache.shape[3], f"q has head_dim {q.shape[2]} but the cache {k_cache.shape[3]}")
+    _need(out.dtype == q.dtype, "out must have q's type")
+    _need(q.shape[1] < 2**31 and 0 <= window < 2**31, "paged_attention: heads or window out of range")
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.q_stride, a.out_stride = (C.c_int64 * 2)(*q.stride()[:2]), (C.c_int64 * 2)(*out.stride()[:2])
+    if lse is not None:
+        _same_device(k_cache, lse, "lse")
+        _need(lse.dtype == torch.float32 and lse.shape == q.shape[:2] and (lse.stride(1) == 1 or lse.shape[1] <= 1),
+              "lse must be float32 [tokens, heads] with unit last stride")
+        a.lse, a.lse_stride = lse.data_ptr(), lse.stride(0)
+    a.q_dtype, a.heads, a.scale, a.causal, a.window = _DT.get(q.dtype, 0), q.shape[1], scale, int(causal), window
+    with torch.cuda.device(k_cache.device):
+        need = N.lib.llg_paged_attention_ws(C.byref(a))
+        N.check(min(need, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=k_cache.device)  # this call's alone: other streams and graphs never share it
+        a.ws, a.ws_bytes = ws.data_ptr(), need
+        N.check(N.lib.llg_paged_attention(C.byref(a), _stream(k_cache)))
+
+
 def _tc_info(kind, cfg):
     return list(N.tc_info(kind, cfg))
 
@@ -263,6 +370,9 @@ if BACKEND == "ctypes":
     _lib.impl("skinny_out", _skinny_out, "CUDA")
     _lib.impl("tc_gemm", _tc_gemm, "CUDA")
     _lib.impl("quant", _quant, "CUDA")
+    _lib.impl("kv_append", _kv_append, "CUDA")
+    _lib.impl("kv_read", _kv_read, "CUDA")
+    _lib.impl("paged_attention", _paged_attention, "CUDA")
     _lib.impl("tc_info", _tc_info, "CompositeExplicitAutograd")
     _lib.impl("set_pdl", _set_pdl, "CompositeExplicitAutograd")
     _lib.impl("pdl_enabled", _pdl_enabled, "CompositeExplicitAutograd")
