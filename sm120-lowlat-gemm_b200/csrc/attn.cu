@@ -1,37 +1,58 @@
 // Attention over a paged cache: what is launched for a call, and where its scratch lies.
+#include <cmath>
+
 #include "paged_kv.cuh"
 
 namespace llg {
 namespace {
 
-constexpr int kRowsMax = 32;  // rows of a few-row tile
+// Sequences with more query rows (new tokens * heads per kv head) than this go to the tile kernel.
+constexpr int kRowsMax = 32;
+constexpr int kTileRows = 256;
 
+struct Part {  // one kernel's CTAs and scratch
+  int ctas, rows, tok_tile;
+  int64_t split, part_ml, part_o;  // offsets
+};
 struct Plan {
-  int blocks;      // few-row kernel: blocks of eight rows per tile
-  int rows_ctas;
-  int64_t split, part_o, part_ml, bytes;  // scratch offsets
+  bool few, many;
+  Part f, m;
+  int64_t bytes;
 };
 
 int64_t pad(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Depends on numbers the host has - never on lengths or offsets, which only the device reads.
+void lay_out(Part* q, int64_t units, int ctas, int rows, int head_dim, int64_t* at) {
+  q->ctas = (int)(units < ctas ? units : ctas);
+  q->rows = rows;
+  q->split = *at;
+  q->part_ml = q->split + pad((int64_t)q->ctas * 16);
+  q->part_o = q->part_ml + pad((int64_t)q->ctas * 2 * rows * 8);
+  *at = q->part_o + pad((int64_t)q->ctas * 2 * rows * head_dim * 4);
+}
+
+// Depends on numbers the host has - never on lengths or offsets, which only the device reads. Without offsets every sequence
+// has the same number of rows and one kernel serves them all; with offsets both are launched and each takes its own.
 Plan plan_of(const llg_attn_args& a) {
   const llg_paged_kv& c = a.kv;
   Plan p{};
-  const int group = a.heads / c.kv_heads;
-  // Rows per tile: a sequence's rows when all have the same number of new tokens, as wide as it gets when they may differ.
-  const int64_t rows = c.q_starts ? (int64_t)c.tokens * group : (int64_t)(c.tokens / c.batch) * group;
-  p.blocks = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  if (group > 8 * p.blocks) p.blocks = group <= 16 ? 2 : 4;
-  const int tile = p.blocks * 8;
-  const int tok_tile = tile / group;
-  const int64_t tiles = (c.tokens + tok_tile - 1) / tok_tile + c.batch;
-  const int64_t units = tiles * c.kv_heads * (((int64_t)c.table_width * c.page_size + 63) / 64 + 1);
-  p.rows_ctas = (int)(units < 2 * sm_count() ? units : 2 * sm_count());
-  p.split = 0;
-  p.part_ml = pad((int64_t)p.rows_ctas * 16);
-  p.part_o = p.part_ml + pad((int64_t)p.rows_ctas * 2 * tile * 8);
-  p.bytes = p.part_o + (int64_t)p.rows_ctas * 2 * tile * c.head_dim * 4;
+  const int group = a.heads / c.kv_heads, sms = sm_count();
+  const int64_t most = c.q_starts ? (int64_t)c.tokens * group : (int64_t)(c.tokens / c.batch) * group;
+  const int64_t keys = (int64_t)c.table_width * c.page_size;
+  p.few = c.q_starts || most <= kRowsMax;
+  p.many = most > kRowsMax;
+  if (p.few) {
+    const int64_t rows = most < kRowsMax ? most : kRowsMax;
+    const int blocks = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.f.tok_tile = blocks * 8 / group;
+    const int64_t tiles = (c.tokens + p.f.tok_tile - 1) / p.f.tok_tile + c.batch;
+    lay_out(&p.f, tiles * c.kv_heads * ((keys + 63) / 64 + 1), 2 * sms, blocks * 8, c.head_dim, &p.bytes);
+  }
+  if (p.many) {
+    p.m.tok_tile = kTileRows / group;
+    const int64_t tiles = (c.tokens + p.m.tok_tile - 1) / p.m.tok_tile + c.batch;
+    lay_out(&p.m, tiles * c.kv_heads * ((keys + 127) / 128 + 1), sms, kTileRows, c.head_dim, &p.bytes);
+  }
   return p;
 }
 
@@ -55,19 +76,40 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
   p.group = a.heads / a.kv.kv_heads;
   p.causal = a.causal != 0;
   p.window = a.window;
-  p.scale_log2 = a.scale * 1.44269504088896341f;
-  p.row_min = 0;
-  p.row_max = INT32_MAX;
-  p.tok_tile = plan.blocks * 8 / p.group;
-  unsigned char* const ws = static_cast<unsigned char*>(a.ws);
-  p.split = reinterpret_cast<int4*>(ws + plan.split);
-  p.part_ml = reinterpret_cast<float*>(ws + plan.part_ml);
-  p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
   const bool fp8 = a.kv.dtype == LLG_DT_E4M3, f16 = a.q_dtype == LLG_DT_F16;
-  const cudaError_t e = f16 ? attn_rows_launch_f16(p, fp8, plan.blocks, plan.rows_ctas, pdl_on(), s)
-                            : attn_rows_launch_bf16(p, fp8, plan.blocks, plan.rows_ctas, pdl_on(), s);
-  if (e != cudaSuccess) return e;
-  return attn_combine_launch(p, f16, plan.rows_ctas, plan.blocks * 8, s);
+  const float scale_log2 = a.scale * 1.44269504088896341f;
+  unsigned char* const ws = static_cast<unsigned char*>(a.ws);
+  auto use = [&](const Part& q) {
+    p.tok_tile = q.tok_tile;
+    p.split = reinterpret_cast<int4*>(ws + q.split);
+    p.part_ml = reinterpret_cast<float*>(ws + q.part_ml);
+    p.part_o = reinterpret_cast<float*>(ws + q.part_o);
+  };
+  if (plan.many) {
+    use(plan.m);
+    p.row_min = plan.few ? kRowsMax : 0;
+    p.row_max = INT32_MAX;
+    // the tile kernel takes the maximum of unscaled scores: a positive scale (1e-30 for 0), the sign goes to q
+    p.negate = scale_log2 < 0.f;
+    p.scale_log2 = fmaxf(fabsf(scale_log2), 1e-30f);
+    cudaError_t e = f16 ? attn_tiles_launch_f16(p, fp8, plan.m.ctas, pdl_on(), s) : attn_tiles_launch_bf16(p, fp8, plan.m.ctas, pdl_on(), s);
+    if (e != cudaSuccess) return e;
+    e = attn_combine_launch(p, f16, plan.m.ctas, kTileRows, s);
+    if (e != cudaSuccess) return e;
+  }
+  if (plan.few) {
+    use(plan.f);
+    p.row_min = 0;
+    p.row_max = kRowsMax;
+    p.negate = 0;
+    p.scale_log2 = scale_log2;
+    const int blocks = plan.f.rows / 8;
+    cudaError_t e = f16 ? attn_rows_launch_f16(p, fp8, blocks, plan.f.ctas, pdl_on(), s) : attn_rows_launch_bf16(p, fp8, blocks, plan.f.ctas, pdl_on(), s);
+    if (e != cudaSuccess) return e;
+    e = attn_combine_launch(p, f16, plan.f.ctas, plan.f.rows, s);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace llg

@@ -31,8 +31,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
   __shared__ float part[kWarps][D + 2];
   pdl_trigger();
   pdl_wait();
-  const int4 item = p.split[blockIdx.x];
+  int4 item = p.split[blockIdx.x];
   if (item.x == 0) return;
+  const int twice = item.w >> 16;  // two parts per CTA
+  item.w &= 0xffff;
+  item.x <<= twice;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SPREAD;
   const int row = blockIdx.y * (kWarps / SPREAD) + warp / SPREAD;
   const bool live = row < item.w;
@@ -44,7 +47,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
       float2 ml = make_float2(-INFINITY, 0.f);
       int64_t at = 0;
       if (i < item.x) {
-        at = (int64_t)(i == 0 ? part_slot(blockIdx.x, true) : part_slot(blockIdx.x + i, false)) * tile_rows + row;
+        const int cta = i >> twice;
+        at = (int64_t)part_slot(blockIdx.x + cta, cta == 0) * tile_rows + row + (twice & i ? 128 : 0);
         ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
       }
       float mx = ml.x;
@@ -62,6 +66,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
       for (int j = 0; j < n; ++j) {
         const float f = __shfl_sync(0xffffffffu, w, j);
         const int64_t a = __shfl_sync(0xffffffffu, at, j);
+        if (f == 0.f) continue;  // a part without keys has no sums
         const float* const src = p.part_o + a * D + lane * V;
         if constexpr (V == 4) {
           const float4 x = *reinterpret_cast<const float4*>(src);

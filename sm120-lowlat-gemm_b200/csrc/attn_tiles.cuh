@@ -1,0 +1,661 @@
+// Attention of many query rows per key/value head over a paged cache (prompt chunks): bound by the tensor cores.
+//
+// One persistent CTA per SM walks its share of (item, 128-key tile) units; an item is up to 256 packed query rows of one
+// sequence and kv head, held as two 128-row streams A and B.
+//   S = Q K^T   tcgen05.mma 128 x 128, both operands in shared memory (K-major, 128-byte swizzle)
+//   P           softmax in registers, one thread per row: no shuffles; P goes back over S in tensor memory, 16 bit
+//   O += P V    tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (rows of head_dim: MN-major B)
+// Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). Warps 0-3 and 4-7: softmax of A and B; 8-11:
+// loaders; 12: MMA issue. While one stream's softmax runs, the other stream's products do: per key tile and stream the tensor
+// core needs 2 x 128 x 128 x head_dim / 4096 cycles (1024 at head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the
+// two streams alternate between units that are equally busy.
+// Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
+// even key tiles, B the odd ones, and each leaves a partial result of its own.
+// The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
+// Loaders gather whole rows page by page: 16-bit rows with cp.async straight into the swizzled tile, e4m3 rows through a
+// staging ring private to each thread, widened with their power of two applied (exact) on the way to the tile.
+// P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
+#pragma once
+
+#include <climits>
+#include <type_traits>
+
+#include "attn_rows.cuh"
+
+namespace llg {
+
+constexpr int kTilesKT = 128;     // keys per unit
+constexpr int kTilesRows = 256;   // rows per item
+constexpr int kTilesThreads = 416;
+
+template <typename T, bool FP8, int D>
+struct TilesCfg {
+  static constexpr int kHalf = 128 * 128;                 // 128 rows x 64 elements, one swizzle-atom column
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTile = kHalves * kHalf;           // a 128-row tile of Q, K or V
+  static constexpr int kSlots = FP8 ? 3 : 4;              // ring of K and V tiles
+  static constexpr int kStageRing = FP8 ? 3 : 0;          // staged e4m3 tiles
+  static constexpr int kStage = 128 * D;
+  static constexpr int kQ = 1024;                         // header before
+  static constexpr int kRing = kQ + 2 * kTile;
+  static constexpr int kStageAt = kRing + kSlots * kTile;
+  static constexpr int kScaleAt = kStageAt + kStageRing * kStage;  // [kStageRing][128] bytes
+  static constexpr int kSmem = kScaleAt + kStageRing * 128 + 1024;  // + alignment slack
+};
+
+// Shared-memory descriptor of V: rows of 64 elements (128 bytes, 128-byte swizzle) along K, 8 rows every 1024 bytes, the next
+// 64 columns `half` bytes on (MN-major operand).
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t addr, uint32_t half) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3ffffu) >> 4);
+  d |= (uint64_t)(half >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+// Waits for the tensor-memory loads issued so far; naming the values keeps their uses behind the wait.
+__device__ __forceinline__ void tmem_wait_ld32(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Ring of mbarrier phases: slot i of n, used round after round.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Barriers in the header: word offsets of 8 bytes from the start of shared memory.
+enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24 };
+
+// How an item uses the two streams.
+enum : int { MODE_ROWS = 0, MODE_ONE = 1, MODE_KEYS = 2 };  // B: rows 128 and on / idle / odd key tiles
+__device__ __forceinline__ int tiles_mode(const Segment& g, int group) {
+  return g.toks * group > 128 ? MODE_ROWS : g.whole ? MODE_ONE : MODE_KEYS;
+}
+
+template <typename T, bool FP8, int D>
+__global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ AttnDev p) {
+  using Cfg = TilesCfg<T, FP8, D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ long long scratch[kTilesThreads / 32 + 4];
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile uint32_t abort_word, drain_word;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto bar = [&](int i) { return base + 8u * i; };
+  if (tid == 0) {
+    abort_word = drain_word = 0u;
+    for (int i = 0; i < Cfg::kSlots; ++i) {
+      mbar_init(bar(BAR_KV_FULL + i), 128);
+      mbar_init(bar(BAR_KV_EMPTY + i), 1);
+    }
+    mbar_init(bar(BAR_Q_FULL), 128);
+    mbar_init(bar(BAR_Q_EMPTY), 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(BAR_S_FULL + s), 1);
+      mbar_init(bar(BAR_P_FULL + s), 128);
+      mbar_init(bar(BAR_PV_DONE + s), 1);
+    }
+    mbar_init(bar(BAR_DONE), 1);
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(&tmem_holder), 512);
+    tmem_relinquish();
+  }
+  pdl_trigger();
+  pdl_wait();
+  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  tc_fence_before();
+  Share share = find_share<kTilesKT, kTilesThreads>(p, scratch);  // synchronises the CTA
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  const PagedKV& c = p.c;
+  volatile uint32_t* const abort_at = &abort_word;
+  Segment g{};
+  bool ok = true;
+  auto wait = [&](int b, uint32_t parity, uint32_t code) {
+    if (!ok) return;
+    if (!mbar_wait(bar(b), parity, abort_at)) {
+      ok = false;
+      atomicCAS(c.status, 0u, code);
+    }
+  };
+
+  if (warp >= 8 && warp < 12) {
+    // ================================================================================================ loaders
+    const int lt = tid - 256, lw = warp - 8;
+    Ring ring;
+    uint32_t q_phase = 1;  // the first wait for an empty Q passes
+    // arrivals owed for groups of copies that may still be in flight, oldest first (0: none)
+    uint32_t owed0 = 0, owed1 = 0;
+    auto settle = [&]() {
+      if (owed0 | owed1) {
+        cp_async_wait<0>();
+        fence_async_shared();
+        if (owed0) mbar_arrive(owed0);
+        if (owed1) mbar_arrive(owed1);
+        owed0 = owed1 = 0u;
+      }
+    };
+    auto owe = [&](uint32_t b) {
+      cp_async_commit();
+      cp_async_wait<2>();
+      if (owed0) {
+        fence_async_shared();
+        mbar_arrive(owed0);
+      }
+      owed0 = owed1;
+      owed1 = b;
+    };
+    int64_t k_off = -1, v_off = -1;  // byte offsets of row `lt` of the tile located last
+    uint32_t k_sc = 0, v_sc = 0;
+    // The page table's entry for row `lt` is requested a tile before it is used.
+    int entry = 0;
+    auto in_use = [&](int j) {
+      const int key = j * kTilesKT + lt;
+      return j < g.tile1 && key >= g.keys.lo && key < g.keys.hi;
+    };
+    auto look_up = [&](int j) {
+      if (in_use(j)) entry = c.table[(int64_t)g.seq * c.table_stride + (j * kTilesKT + lt) / c.page_size];
+    };
+    auto locate = [&](int j) {
+      const int key = j * kTilesKT + lt;
+      k_off = v_off = -1;
+      k_sc = v_sc = 0u;
+      const int pg = entry;
+      look_up(j + 1);
+      if (in_use(j)) {
+        const int slot = key % c.page_size;
+        if ((unsigned)pg >= (unsigned)c.pages) {
+          atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+        } else {
+          k_off = pg * c.k_page + g.head * c.k_head + slot * c.k_slot;
+          v_off = pg * c.v_page + g.head * c.v_head + slot * c.v_slot;
+          if constexpr (FP8) {
+            k_sc = c.ks[pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot];
+            v_sc = c.vs[pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot];
+          }
+        }
+      }
+    };
+    // 16-bit rows: straight into slot `ring.slot`
+    auto copy16 = [&](const unsigned char* src, int64_t off) {
+      if (!mbar_try(bar(BAR_KV_EMPTY + ring.slot), ring.phase ^ 1u)) {
+        settle();
+        wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
+      }
+      if (!ok) return;
+      const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
+      constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte pieces per row, rows per warp instruction
+#pragma unroll
+      for (int i = 0; i < 32 / RP; ++i) {
+        const int r = i * RP + lane / CH, ch = lane % CH, row = lw * 32 + r;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+        cp_async16(dst + (ch >> 3) * Cfg::kHalf + row * 128 + (((ch & 7) ^ (row & 7)) << 4), src + (o >= 0 ? o + ch * 16 : 0), o >= 0 ? 16u : 0u);
+      }
+      owe(bar(BAR_KV_FULL + ring.slot));
+      ring.next(Cfg::kSlots);
+    };
+    // e4m3 rows: `stage` fetches into the thread's own staging bytes, `widen` converts them into the ring
+    constexpr int CH8 = D / 16, RP8 = 32 / CH8, IT8 = 32 / RP8;
+    int staged = 0, widened = 0;
+    auto stage = [&](const unsigned char* src, int64_t off, uint32_t sc) {
+      const int at = staged % 3;
+      const uint32_t dst = base + Cfg::kStageAt + at * Cfg::kStage + lt * 16;
+#pragma unroll
+      for (int i = 0; i < IT8; ++i) {
+        const int r = i * RP8 + lane / CH8, ch = lane % CH8;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+        cp_async16(dst + i * 2048, src + (o >= 0 ? o + ch * 16 : 0), o >= 0 ? 16u : 0u);
+      }
+      cp_async_commit();
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 128 + lt), "r"(sc) : "memory");
+      ++staged;
+    };
+    auto widen = [&](bool last) {
+      if (last) cp_async_wait<0>();
+      else cp_async_wait<1>();
+      __syncwarp();
+      wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_CONVERT_WAIT);
+      if (!ok) return;
+      const int at = widened % 3;
+      const uint32_t src = base + Cfg::kStageAt + at * Cfg::kStage + lt * 16;
+      const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
+#pragma unroll
+      for (int i = 0; i < IT8; ++i) {
+        const int r = i * RP8 + lane / CH8, ch = lane % CH8, row = lw * 32 + r;
+        const uint4 raw = lds16(src + i * 2048);
+        uint32_t b;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(base + Cfg::kScaleAt + at * 128 + row) : "memory");
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Widen<T>::four(w[j], o[2 * j], o[2 * j + 1]);
+        if constexpr (kBf16) {
+          // 2^120 * 2^e in two factors, each a bf16: e up to 7 in the first
+          const int e = (int)b - 127;
+          const __nv_bfloat162 f0 = __float2bfloat162_rn(__uint_as_float((uint32_t)(min(e, 7) + 120 + 127) << 23));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) *reinterpret_cast<__nv_bfloat162*>(&o[j]) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[j]), f0);
+          if (__any_sync(0xffffffffu, e > 7)) {
+            const __nv_bfloat162 f1 = __float2bfloat162_rn(__uint_as_float((uint32_t)(max(e - 7, 0) + 127) << 23));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<__nv_bfloat162*>(&o[j]) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[j]), f1);
+          }
+        } else {
+          const __half2 f = __float2half2_rn(pow2_of(b));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) *reinterpret_cast<__half2*>(&o[j]) = __hmul2(*reinterpret_cast<__half2*>(&o[j]), f);
+        }
+        const uint32_t at0 = dst + (ch >> 2) * Cfg::kHalf + row * 128;
+        const int c0 = 2 * (ch & 3);
+        // lanes of the two halves write alternate pieces first: eight lanes then fall on eight different bank groups
+        const bool odd = (ch >> 2) & 1;
+        const uint32_t a0 = at0 + (((c0 + (odd ? 1 : 0)) ^ (row & 7)) << 4), a1 = at0 + (((c0 + (odd ? 0 : 1)) ^ (row & 7)) << 4);
+        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+        const uint4 x = odd ? hi : lo, y = odd ? lo : hi;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a0), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a1), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+      }
+      fence_async_shared();
+      mbar_arrive(bar(BAR_KV_FULL + ring.slot));
+      ring.next(Cfg::kSlots);
+      ++widened;
+      __syncwarp();  // the stage may be fetched into again
+    };
+    auto load_q = [&]() {
+      settle();
+      wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
+      q_phase ^= 1u;
+      if (!ok) return;
+      const int rows = g.toks * p.group;
+      constexpr int CH = D / 8;
+      const uint32_t flip = p.negate ? 0x80008000u : 0u;
+#pragma unroll 4
+      for (int i = lt; i < kTilesRows * CH; i += 128) {
+        const int row = i / CH, ch = i % CH;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) {
+          const int tok = row / p.group, hh = row - tok * p.group;
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head + ch * 16);
+          v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        }
+        const uint32_t dst = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      }
+      fence_async_shared();
+      mbar_arrive(bar(BAR_Q_FULL));
+    };
+    while (ok && next_segment<kTilesKT>(p, share, g)) {
+      const bool keys = tiles_mode(g, p.group) == MODE_KEYS;
+      // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
+      look_up(g.tile0);
+      if constexpr (!FP8) {
+        locate(g.tile0);
+        int64_t v_prev = -1;
+        for (int j = g.tile0; j < g.tile1; ++j) {
+          const int64_t ko = k_off, vo = v_off;
+          locate(j + 1);
+          copy16(c.k, ko);
+          if (j == g.tile0) load_q();
+          if (keys) {
+            if (j > g.tile0) copy16(c.v, v_prev);
+            v_prev = vo;
+          } else {
+            copy16(c.v, vo);
+          }
+        }
+        if (keys) copy16(c.v, v_prev);
+      } else {
+        // the same sequence, every tile fetched two places ahead of its widening
+        const int n = 2 * (g.tile1 - g.tile0);
+        int64_t v_at[2] = {-1, -1};
+        uint32_t v_scale[2] = {0u, 0u};
+        int next_k = g.tile0;
+        auto is_k = [&](int i) { return keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0; };
+        int vq_in = 0, vq_out = 0;
+        auto fetch = [&](int i) {
+          if (is_k(i)) {
+            locate(next_k++);
+            stage(c.k, k_off, k_sc);
+            if (vq_in & 1) {
+              v_at[1] = v_off;
+              v_scale[1] = v_sc;
+            } else {
+              v_at[0] = v_off;
+              v_scale[0] = v_sc;
+            }
+            ++vq_in;
+          } else {
+            stage(c.v, (vq_out & 1) ? v_at[1] : v_at[0], (vq_out & 1) ? v_scale[1] : v_scale[0]);
+            ++vq_out;
+          }
+        };
+        fetch(0);
+        load_q();
+        fetch(1);
+        for (int i = 0; i < n && ok; ++i) {
+          widen(i + 1 >= n);
+          if (i + 2 < n) fetch(i + 2);
+        }
+      }
+    }
+    settle();
+    cp_async_wait<0>();
+  } else if (warp == 12) {
+    // ================================================================================================ MMA issue
+    constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t kIdescS = umma_idesc(1, kFmt, kFmt, 128, 128);
+    constexpr uint32_t kIdescO = umma_idesc(1, kFmt, kFmt, 128, D) | (1u << 16);  // B is MN-major
+    Ring ring;
+    uint32_t q_phase = 0, p_phase[2] = {0u, 0u};
+    const bool leader = elect_one();
+    auto scores = [&](int s, int qt, uint32_t kslot) {  // S_s = Q_qt K^T
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * Cfg::kHalf + (ks & 3) * 32;
+          mma_ss_f16(tmem + s * 128, umma_desc_sw128(base + Cfg::kQ + qt * Cfg::kTile + off),
+                     umma_desc_sw128(base + Cfg::kRing + kslot * Cfg::kTile + off), kIdescS, ks > 0);
+        }
+        umma_commit(bar(BAR_S_FULL + s));
+      }
+      __syncwarp();
+    };
+    auto values = [&](int s, uint32_t vslot, bool first) {  // O_s (+)= P_s V
+      wait(BAR_P_FULL + s, p_phase[s], ST_MMA_FULL_WAIT);
+      p_phase[s] ^= 1u;
+      if (!ok) return;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+          mma_ts_f16(tmem + 256 + s * D, tmem + s * 128 + ks * 8,
+                     umma_desc_mn128(base + Cfg::kRing + vslot * Cfg::kTile + ks * 2048, Cfg::kHalf), kIdescO, !first || ks > 0);
+        umma_commit(bar(BAR_PV_DONE + s));
+      }
+      __syncwarp();
+    };
+    auto full = [&]() -> int {  // waits for the next tile of the ring
+      wait(BAR_KV_FULL + ring.slot, ring.phase, ST_MMA_FULL_WAIT);
+      if (ok) tc_fence_after();
+      const int s = ring.slot;
+      ring.next(Cfg::kSlots);
+      return s;
+    };
+    auto release = [&](int b) {
+      if (leader) umma_commit(bar(b));
+      __syncwarp();
+    };
+    while (ok && next_segment<kTilesKT>(p, share, g)) {
+      const int mode = tiles_mode(g, p.group);
+      const int nt = g.tile1 - g.tile0;
+      int k = full();
+      wait(BAR_Q_FULL, q_phase, ST_MMA_FULL_WAIT);
+      q_phase ^= 1u;
+      if (!ok) break;
+      tc_fence_after();
+      scores(0, 0, k);
+      if (mode == MODE_ROWS) scores(1, 1, k);
+      release(BAR_KV_EMPTY + k);
+      if (mode == MODE_KEYS && nt > 1) {
+        k = full();
+        if (!ok) break;
+        scores(1, 0, k);
+        release(BAR_KV_EMPTY + k);
+      }
+      if (nt == 1 || (mode == MODE_KEYS && nt == 2)) release(BAR_Q_EMPTY);
+      for (int j = 0; j < nt && ok; ++j) {
+        const int v = full();
+        if (!ok) break;
+        if (mode == MODE_KEYS) {
+          const int s = j & 1;
+          values(s, v, j < 2);
+          release(BAR_KV_EMPTY + v);
+          if (j + 2 < nt) {
+            k = full();
+            if (!ok) break;
+            scores(s, 0, k);
+            release(BAR_KV_EMPTY + k);
+            if (j + 3 == nt) release(BAR_Q_EMPTY);
+          }
+        } else {
+          const bool more = j + 1 < nt;
+          values(0, v, j == 0);
+          if (more) {
+            k = full();
+            if (!ok) break;
+            scores(0, 0, k);
+          }
+          if (mode == MODE_ROWS) {
+            values(1, v, j == 0);
+            if (!ok) break;
+            if (more) scores(1, 1, k);
+          }
+          release(BAR_KV_EMPTY + v);
+          if (more) release(BAR_KV_EMPTY + k);
+          if (j + 2 == nt) release(BAR_Q_EMPTY);
+        }
+      }
+    }
+    // nothing of this CTA may be in flight when its tensor memory goes
+    release(BAR_DONE);
+    mbar_wait(bar(BAR_DONE), 0, &drain_word);
+  } else if (warp < 8) {
+    // ================================================================================================ softmax
+    const int s = warp >> 2;                                   // stream
+    const int row_in = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + s * 128, tO = tmem + lanes + 256 + s * D;
+    uint32_t s_phase = 0, pv_phase = 0;
+    const float c_log2 = p.scale_log2;
+    const uint64_t c2 = pack_f32x2(c_log2, c_log2);
+    while (ok && next_segment<kTilesKT>(p, share, g)) {
+      const int mode = tiles_mode(g, p.group);
+      if (mode == MODE_ONE && s == 1) continue;
+      const int rows = g.toks * p.group;
+      const int row = mode == MODE_ROWS ? s * 128 + row_in : row_in;
+      const int step = mode == MODE_KEYS ? 2 : 1;
+      const bool live = row < rows;
+      const int tok = row / p.group;
+      const int pos = g.s.len - g.s.n + g.tok0 + tok;
+      // rows of no token see everything: they keep no tile from the unmasked path, and nobody reads them
+      const int last = !live ? INT_MAX : p.causal ? min(pos, g.s.len - 1) : g.s.len - 1;
+      const int first = live && p.window > 0 ? pos - p.window + 1 : 0;
+      float m = -INFINITY;                                       // running maximum, times c_log2
+      uint64_t l2 = 0;                                           // two partial row sums
+      int done = 0;                                              // key tiles of this stream behind us
+      for (int j = g.tile0 + (mode == MODE_KEYS ? s : 0); j < g.tile1 && ok; j += step, ++done) {
+        wait(BAR_S_FULL + s, s_phase, ST_EPILOGUE_WAIT);
+        s_phase ^= 1u;
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = j * kTilesKT;
+        // does any row of the warp see only a part of the tile?
+        const bool edge = __any_sync(0xffffffffu, key0 + kTilesKT - 1 > last || key0 < first);
+        const int hi = last - key0, lo = first - key0;           // columns [lo, hi] are seen
+        float x[2][32];
+        float mx = -INFINITY;
+        tmem_ld32(tS, x[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_wait_ld32(x[q & 1]);
+          if (q < 3) tmem_ld32(tS + 32 * (q + 1), x[(q + 1) & 1]);
+          float (&v)[32] = x[q & 1];
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 32 * q + i <= hi && 32 * q + i >= lo ? v[i] : -INFINITY;
+          }
+          float a = fmaxf(v[0], v[1]), b = fmaxf(v[2], v[3]);
+#pragma unroll
+          for (int i = 4; i < 32; i += 4) {
+            a = fmaxf(a, fmaxf(v[i], v[i + 1]));
+            b = fmaxf(b, fmaxf(v[i + 2], v[i + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(a, b));
+        }
+        const float top = mx * c_log2;
+        const bool move = top > m + 8.f || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, move)) {
+          const float now = move ? top : m;
+          const float keep = m == -INFINITY ? 0.f : exp2_fast(m - now);
+          if (done > 0) {  // rescale what has been added up so far
+            wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              tmem_ld32(tO + 32 * q, x[0]);
+              tmem_wait_ld32(x[0]);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[0][i] = keep == 0.f ? 0.f : x[0][i] * keep;
+              tmem_st32(tO + 32 * q, x[0]);
+            }
+            float a, b;
+            unpack_f32x2(l2, a, b);
+            l2 = pack_f32x2(a * keep, b * keep);
+          }
+          m = now;
+        }
+        const float base_m = m == -INFINITY ? 0.f : m;
+        const uint64_t neg = pack_f32x2(-base_m, -base_m);
+        tmem_ld32(tS, x[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_wait_ld32(x[q & 1]);
+          if (q < 3) tmem_ld32(tS + 32 * (q + 1), x[(q + 1) & 1]);
+          float (&v)[32] = x[q & 1];
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 32 * q + i <= hi && 32 * q + i >= lo ? v[i] : -INFINITY;
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a, b;
+            unpack_f32x2(fma_f32x2(pack_f32x2(v[2 * i], v[2 * i + 1]), c2, neg), a, b);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+            l2 = add_f32x2(l2, pack_f32x2(a, b));
+            w[i] = Mma<T>::pack(a, b);
+          }
+          tmem_st16(tS + 16 * q, w);  // columns 16 q .. of P lie over columns of S that this thread has read
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(BAR_P_FULL + s));
+        pv_phase ^= 1u;
+      }
+      if (!ok) break;
+      // ---- the row's result
+      float sum0, sum1;
+      unpack_f32x2(l2, sum0, sum1);
+      const float sum = sum0 + sum1;
+      const int tok_row = tok;
+      const int head = g.head * p.group + row - tok_row * p.group;
+      const int64_t t = g.s.t0 + g.tok0 + tok_row;
+      const float inv = g.whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
+      const int64_t slot_row = (int64_t)part_slot(blockIdx.x, g.starts) * kTilesRows + (mode == MODE_KEYS ? s * 128 + row_in : row);
+      if (done > 0) {
+        wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          float x[32];
+          tmem_ld32(tO + 32 * q, x);
+          tmem_wait_ld32(x);
+          if (!live) continue;
+          if (g.whole) {
+            uint4* const dst = reinterpret_cast<uint4*>(p.out + t * p.o_tok + head * p.o_head + 64 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[i] = make_uint4(Mma<T>::pack(x[8 * i] * inv, x[8 * i + 1] * inv), Mma<T>::pack(x[8 * i + 2] * inv, x[8 * i + 3] * inv),
+                                  Mma<T>::pack(x[8 * i + 4] * inv, x[8 * i + 5] * inv), Mma<T>::pack(x[8 * i + 6] * inv, x[8 * i + 7] * inv));
+          } else {
+            float4* const dst = reinterpret_cast<float4*>(p.part_o + slot_row * D + 32 * q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      if (live) {
+        if (!g.whole) *reinterpret_cast<float2*>(p.part_ml + slot_row * 2) = make_float2(done > 0 ? m : -INFINITY, sum);
+        else if (p.lse) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (m + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+      }
+      if (tid == 0 && g.starts && !g.whole)
+        p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows | (mode == MODE_KEYS ? 1 << 16 : 0));
+    }
+  }
+  __syncthreads();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace llg

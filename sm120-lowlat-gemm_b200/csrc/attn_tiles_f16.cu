@@ -1,0 +1,8 @@
+// Many-row attention over a paged cache, f16 queries (see attn_tiles.cuh).
+#include "attn_tiles_launch.cuh"
+
+namespace llg {
+cudaError_t attn_tiles_launch_f16(const AttnDev& p, bool fp8, int ctas, bool pdl, cudaStream_t s) {
+  return attn_tiles_dispatch<__half>(p, fp8, ctas, pdl, s);
+}
+}  // namespace llg

@@ -127,6 +127,8 @@ int64_t attn_workspace(const llg_attn_args& a);
 cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s);
 cudaError_t attn_rows_launch_bf16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_rows_launch_f16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_tiles_launch_bf16(const AttnDev& p, bool fp8, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_tiles_launch_f16(const AttnDev& p, bool fp8, int ctas, bool pdl, cudaStream_t s);
 // ctas: those of the kernel that left the partial results; tile_rows: rows of one of its tiles.
 cudaError_t attn_combine_launch(const AttnDev& p, bool f16, int ctas, int tile_rows, cudaStream_t s);
 

@@ -71,12 +71,14 @@ struct AttnDev {
   int64_t lse_tok;        // elements; heads are contiguous
   int group;              // query heads per kv head
   int causal, window;
-  float scale_log2;       // softmax scale * log2(e)
+  float scale_log2;       // softmax scale * log2(e); its magnitude in the tile kernel ...
+  int negate;             // ... which turns the signs of q around for a negative scale
   int row_min, row_max;   // this launch serves sequences with row_min < new tokens * group <= row_max
   int tok_tile;           // whole tokens per row tile
   float* part_o;          // [slots][rows per tile][head_dim]
   float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
-  int4* split;            // [CTAs]: the item that starts, cut, at the end of a CTA's share: {parts, first token, kv head, rows}
+  int4* split;            // [CTAs]: the item that starts, cut, at the end of a CTA's share: {CTAs, first token, kv head, rows};
+                          // 1 << 16 in the last: every CTA left two parts, the second 128 rows behind the first
 };
 
 // Keys [lo, hi) that any row of token tile [tf, tf + cnt) sees.
@@ -117,6 +119,8 @@ struct Share {
   long long u, end, per;  // next unit, end of the share, units per CTA
   int seq;
   long long off;          // units of `seq` (over all kv heads) before u
+  int known;              // sequence whose units of one kv head `per_head` holds
+  long long per_head;
 };
 
 // Every thread of the CTA takes part. scratch: NT / 32 + 4 long longs of shared memory.
@@ -146,6 +150,8 @@ __device__ __forceinline__ Share find_share(const AttnDev& p, long long* scratch
   sh.end = min(total, sh.u + sh.per);
   sh.seq = 0;
   sh.off = 0;
+  sh.known = -1;
+  sh.per_head = 0;
   if (sh.u >= sh.end) return sh;
   long long base = 0;
   for (int c0 = 0; c0 < p.c.batch; c0 += NT) {
@@ -197,7 +203,11 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
   for (;;) {
     if (sh.seq >= p.c.batch) return false;
     g.s = seq_view(p.c, sh.seq);
-    per_head = seq_units<KT>(p, g.s);
+    if (sh.known != sh.seq) {
+      sh.per_head = seq_units<KT>(p, g.s);
+      sh.known = sh.seq;
+    }
+    per_head = sh.per_head;
     if (per_head > 0) break;
     ++sh.seq;  // nothing of this sequence belongs to this launch
     sh.off = 0;
