@@ -6,7 +6,9 @@
 //   P           softmax in registers, one thread per row: no shuffles; P goes back over S in tensor memory, 16 bit
 //   O += P V    tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (rows of head_dim: MN-major B)
 // Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). Warps 0-3 and 4-7: softmax of A and B; 8-11:
-// loaders; 12: MMA issue. While one stream's softmax runs, the other stream's products do: per key tile and stream the tensor
+// loaders; 12: MMA issue; 13:
+// the walk, published as segments in shared memory (14 and 15 fill the warpgroup: registers move between warpgroups, so that a
+// row of 128 scores stays in the softmax threads). While one stream's softmax runs, the other stream's products do: per key tile and stream the tensor
 // core needs 2 x 128 x 128 x head_dim / 4096 cycles (1024 at head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the
 // two streams alternate between units that are equally busy.
 // Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
@@ -26,7 +28,7 @@ namespace llg {
 
 constexpr int kTilesKT = 128;     // keys per unit
 constexpr int kTilesRows = 256;   // rows per item
-constexpr int kTilesThreads = 416;
+constexpr int kTilesThreads = 512;
 
 template <typename T, bool FP8, int D>
 struct TilesCfg {
@@ -67,17 +69,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
-      : "memory");
-}
 // Waits for the tensor-memory loads issued so far; naming the values keeps their uses behind the wait.
 __device__ __forceinline__ void tmem_wait_ld32(float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -91,6 +82,19 @@ __device__ __forceinline__ void tmem_wait_ld32(float (&v)[32]) {
                :
                : "memory");
 }
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+// Moves registers between the warpgroups of a CTA. All four warps of a warpgroup execute it; the counts of all warpgroups
+// together stay within what the CTA was launched with.
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
@@ -128,7 +132,10 @@ struct Ring {
 };
 
 // Barriers in the header: word offsets of 8 bytes from the start of shared memory.
-enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24 };
+enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24,
+             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29 };
+constexpr int kSegRing = 4;        // segments published ahead of the roles that work on them
+constexpr int kSegReaders = 13;    // warps that read a segment
 
 // How an item uses the two streams.
 enum : int { MODE_ROWS = 0, MODE_ONE = 1, MODE_KEYS = 2 };  // B: rows 128 and on / idle / odd key tiles
@@ -143,6 +150,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   extern __shared__ unsigned char smem_raw[];
   __shared__ long long scratch[kTilesThreads / 32 + 4];
   __shared__ uint32_t tmem_holder;
+  __shared__ Segment segments[kSegRing];
   __shared__ volatile uint32_t abort_word, drain_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -161,6 +169,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       mbar_init(bar(BAR_PV_DONE + s), 1);
     }
     mbar_init(bar(BAR_DONE), 1);
+    for (int i = 0; i < kSegRing; ++i) {
+      mbar_init(bar(BAR_SEG_FULL + i), 1);
+      mbar_init(bar(BAR_SEG_EMPTY + i), kSegReaders);
+    }
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -177,7 +189,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   const uint32_t tmem = tmem_holder;
   const PagedKV& c = p.c;
   volatile uint32_t* const abort_at = &abort_word;
-  Segment g{};
   bool ok = true;
   auto wait = [&](int b, uint32_t parity, uint32_t code) {
     if (!ok) return;
@@ -186,9 +197,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       atomicCAS(c.status, 0u, code);
     }
   };
+  // The segments that warp 13 publishes, in order: next_item() waits for one (null behind the last), done_item() hands it back.
+  Ring items;
+  auto next_item = [&]() -> const Segment* {
+    wait(BAR_SEG_FULL + items.slot, items.phase, ST_MMA_FULL_WAIT);
+    return ok && segments[items.slot].tile0 >= 0 ? &segments[items.slot] : nullptr;
+  };
+  auto done_item = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(BAR_SEG_EMPTY + items.slot));
+    items.next(kSegRing);
+  };
 
   if (warp >= 8 && warp < 12) {
     // ================================================================================================ loaders
+    regs_down<64>();  // 512 threads start with 128 each: 2 x 200 (softmax) + 64 + 48 = 4 x 128
     const int lt = tid - 256, lw = warp - 8;
     Ring ring;
     uint32_t q_phase = 1;  // the first wait for an empty Q passes
@@ -215,14 +238,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     };
     int64_t k_off = -1, v_off = -1;  // byte offsets of row `lt` of the tile located last
     uint32_t k_sc = 0, v_sc = 0;
+    const Segment* seg = nullptr;
     // The page table's entry for row `lt` is requested a tile before it is used.
     int entry = 0;
     auto in_use = [&](int j) {
       const int key = j * kTilesKT + lt;
-      return j < g.tile1 && key >= g.keys.lo && key < g.keys.hi;
+      return j < seg->tile1 && key >= seg->keys.lo && key < seg->keys.hi;
     };
     auto look_up = [&](int j) {
-      if (in_use(j)) entry = c.table[(int64_t)g.seq * c.table_stride + (j * kTilesKT + lt) / c.page_size];
+      if (in_use(j)) entry = c.table[(int64_t)seg->seq * c.table_stride + (j * kTilesKT + lt) / c.page_size];
     };
     auto locate = [&](int j) {
       const int key = j * kTilesKT + lt;
@@ -235,11 +259,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if ((unsigned)pg >= (unsigned)c.pages) {
           atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
         } else {
-          k_off = pg * c.k_page + g.head * c.k_head + slot * c.k_slot;
-          v_off = pg * c.v_page + g.head * c.v_head + slot * c.v_slot;
+          k_off = pg * c.k_page + seg->head * c.k_head + slot * c.k_slot;
+          v_off = pg * c.v_page + seg->head * c.v_head + slot * c.v_slot;
           if constexpr (FP8) {
-            k_sc = c.ks[pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot];
-            v_sc = c.vs[pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot];
+            k_sc = c.ks[pg * c.ks_page + seg->head * c.ks_head + slot * c.ks_slot];
+            v_sc = c.vs[pg * c.vs_page + seg->head * c.vs_head + slot * c.vs_slot];
           }
         }
       }
@@ -253,7 +277,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       if (!ok) return;
       const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
       constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte pieces per row, rows per warp instruction
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 32 / RP; ++i) {
         const int r = i * RP + lane / CH, ch = lane % CH, row = lw * 32 + r;
         const int64_t o = __shfl_sync(0xffffffffu, off, r);
@@ -334,7 +358,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
       if (!ok) return;
-      const int rows = g.toks * p.group;
+      const int rows = seg->toks * p.group;
       constexpr int CH = D / 8;
       const uint32_t flip = p.negate ? 0x80008000u : 0u;
 #pragma unroll 4
@@ -343,7 +367,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows) {
           const int tok = row / p.group, hh = row - tok * p.group;
-          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head + ch * 16);
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(seg->s.t0 + seg->tok0 + tok) * p.q_tok + (int64_t)(seg->head * p.group + hh) * p.q_head + ch * 16);
           v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
         }
         const uint32_t dst = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
@@ -352,20 +376,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       fence_async_shared();
       mbar_arrive(bar(BAR_Q_FULL));
     };
-    while (ok && next_segment<kTilesKT>(p, share, g)) {
-      const bool keys = tiles_mode(g, p.group) == MODE_KEYS;
+    while ((seg = next_item()) != nullptr) {
+      const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
       // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
-      look_up(g.tile0);
+      look_up(seg->tile0);
       if constexpr (!FP8) {
-        locate(g.tile0);
+        locate(seg->tile0);
         int64_t v_prev = -1;
-        for (int j = g.tile0; j < g.tile1; ++j) {
+        for (int j = seg->tile0; j < seg->tile1; ++j) {
           const int64_t ko = k_off, vo = v_off;
           locate(j + 1);
           copy16(c.k, ko);
-          if (j == g.tile0) load_q();
+          if (j == seg->tile0) load_q();
           if (keys) {
-            if (j > g.tile0) copy16(c.v, v_prev);
+            if (j > seg->tile0) copy16(c.v, v_prev);
             v_prev = vo;
           } else {
             copy16(c.v, vo);
@@ -374,10 +398,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (keys) copy16(c.v, v_prev);
       } else {
         // the same sequence, every tile fetched two places ahead of its widening
-        const int n = 2 * (g.tile1 - g.tile0);
+        const int n = 2 * (seg->tile1 - seg->tile0);
         int64_t v_at[2] = {-1, -1};
         uint32_t v_scale[2] = {0u, 0u};
-        int next_k = g.tile0;
+        int next_k = seg->tile0;
         auto is_k = [&](int i) { return keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0; };
         int vq_in = 0, vq_out = 0;
         auto fetch = [&](int i) {
@@ -405,10 +429,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           if (i + 2 < n) fetch(i + 2);
         }
       }
+      done_item();
     }
     settle();
     cp_async_wait<0>();
-  } else if (warp == 12) {
+  } else if (warp >= 12) {
+    regs_down<48>();
+    if (warp == 12) {
     // ================================================================================================ MMA issue
     constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
     constexpr uint32_t kIdescS = umma_idesc(1, kFmt, kFmt, 128, 128);
@@ -418,11 +445,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     const bool leader = elect_one();
     auto scores = [&](int s, int qt, uint32_t kslot) {  // S_s = Q_qt K^T
       if (leader) {
+        // descriptors differ in the low word's address only; opaque, so that no call site keeps its sixteen of them
+        uint32_t qa = (base + Cfg::kQ + qt * Cfg::kTile) >> 4, ka = (base + Cfg::kRing + kslot * Cfg::kTile) >> 4;
+        asm volatile("" : "+r"(qa), "+r"(ka));
+        const uint64_t hi = umma_desc_sw128(0);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * Cfg::kHalf + (ks & 3) * 32;
-          mma_ss_f16(tmem + s * 128, umma_desc_sw128(base + Cfg::kQ + qt * Cfg::kTile + off),
-                     umma_desc_sw128(base + Cfg::kRing + kslot * Cfg::kTile + off), kIdescS, ks > 0);
+          const uint32_t off = ((ks >> 2) * Cfg::kHalf + (ks & 3) * 32) >> 4;
+          mma_ss_f16(tmem + s * 128, hi | (qa + off), hi | (ka + off), kIdescS, ks > 0);
         }
         umma_commit(bar(BAR_S_FULL + s));
       }
@@ -434,10 +464,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       if (!ok) return;
       tc_fence_after();
       if (leader) {
+        uint32_t va = (base + Cfg::kRing + vslot * Cfg::kTile) >> 4;
+        asm volatile("" : "+r"(va));
+        const uint64_t hi = umma_desc_mn128(0, Cfg::kHalf);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)
-          mma_ts_f16(tmem + 256 + s * D, tmem + s * 128 + ks * 8,
-                     umma_desc_mn128(base + Cfg::kRing + vslot * Cfg::kTile + ks * 2048, Cfg::kHalf), kIdescO, !first || ks > 0);
+          mma_ts_f16(tmem + 256 + s * D, tmem + s * 128 + ks * 8, hi | (va + ks * 128), kIdescO, !first || ks > 0);
         umma_commit(bar(BAR_PV_DONE + s));
       }
       __syncwarp();
@@ -453,9 +485,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       if (leader) umma_commit(bar(b));
       __syncwarp();
     };
-    while (ok && next_segment<kTilesKT>(p, share, g)) {
-      const int mode = tiles_mode(g, p.group);
-      const int nt = g.tile1 - g.tile0;
+    while (const Segment* seg = next_item()) {
+      const int mode = tiles_mode(*seg, p.group);
+      const int nt = seg->tile1 - seg->tile0;
+      done_item();
       int k = full();
       wait(BAR_Q_FULL, q_phase, ST_MMA_FULL_WAIT);
       q_phase ^= 1u;
@@ -507,8 +540,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     // nothing of this CTA may be in flight when its tensor memory goes
     release(BAR_DONE);
     mbar_wait(bar(BAR_DONE), 0, &drain_word);
-  } else if (warp < 8) {
+    } else if (warp == 13) {
+    // ================================================================================================ schedule
+    while (ok) {
+      wait(BAR_SEG_EMPTY + items.slot, items.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
+      Segment g;
+      const bool more = ok && next_segment<kTilesKT>(p, share, g);
+      if (!more) g.tile0 = -1;
+      if (lane == 0) {
+        segments[items.slot] = g;
+        mbar_arrive(bar(BAR_SEG_FULL + items.slot));
+      }
+      __syncwarp();
+      items.next(kSegRing);
+      if (!more) break;
+    }
+    }
+  } else {
     // ================================================================================================ softmax
+    regs_up<200>();
     const int s = warp >> 2;                                   // stream
     const int row_in = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -516,9 +566,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     uint32_t s_phase = 0, pv_phase = 0;
     const float c_log2 = p.scale_log2;
     const uint64_t c2 = pack_f32x2(c_log2, c_log2);
-    while (ok && next_segment<kTilesKT>(p, share, g)) {
+    while (const Segment* seg = next_item()) {
+      const Segment& g = *seg;
       const int mode = tiles_mode(g, p.group);
-      if (mode == MODE_ONE && s == 1) continue;
+      if (mode == MODE_ONE && s == 1) {
+        done_item();
+        continue;
+      }
       const int rows = g.toks * p.group;
       const int row = mode == MODE_ROWS ? s * 128 + row_in : row_in;
       const int step = mode == MODE_KEYS ? 2 : 1;
@@ -540,26 +594,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         // does any row of the warp see only a part of the tile?
         const bool edge = __any_sync(0xffffffffu, key0 + kTilesKT - 1 > last || key0 < first);
         const int hi = last - key0, lo = first - key0;           // columns [lo, hi] are seen
-        float x[2][32];
-        float mx = -INFINITY;
-        tmem_ld32(tS, x[0]);
+        float x[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, x[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_wait_ld32(x[q]);
+        if (edge) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[q][i] = 32 * q + i <= hi && 32 * q + i >= lo ? x[q][i] : -INFINITY;
+        }
+        float part[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tmem_wait_ld32(x[q & 1]);
-          if (q < 3) tmem_ld32(tS + 32 * (q + 1), x[(q + 1) & 1]);
-          float (&v)[32] = x[q & 1];
-          if (edge) {
+          part[q] = fmaxf(x[q][0], x[q][1]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 32 * q + i <= hi && 32 * q + i >= lo ? v[i] : -INFINITY;
-          }
-          float a = fmaxf(v[0], v[1]), b = fmaxf(v[2], v[3]);
-#pragma unroll
-          for (int i = 4; i < 32; i += 4) {
-            a = fmaxf(a, fmaxf(v[i], v[i + 1]));
-            b = fmaxf(b, fmaxf(v[i + 2], v[i + 3]));
-          }
-          mx = fmaxf(mx, fmaxf(a, b));
+          for (int i = 2; i < 32; i += 2) part[q] = fmaxf(part[q], fmaxf(x[q][i], x[q][i + 1]));
         }
+        const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
         const float top = mx * c_log2;
         const bool move = top > m + 8.f || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
@@ -569,13 +622,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);
             if (!ok) break;
             tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t o[16];
+              tmem_ld16(tO + 16 * q, o);
+              tmem_wait_ld16(o);
 #pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              tmem_ld32(tO + 32 * q, x[0]);
-              tmem_wait_ld32(x[0]);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[0][i] = keep == 0.f ? 0.f : x[0][i] * keep;
-              tmem_st32(tO + 32 * q, x[0]);
+              for (int i = 0; i < 16; ++i) o[i] = keep == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st16(tO + 16 * q, o);
             }
             float a, b;
             unpack_f32x2(l2, a, b);
@@ -585,27 +639,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         }
         const float base_m = m == -INFINITY ? 0.f : m;
         const uint64_t neg = pack_f32x2(-base_m, -base_m);
-        tmem_ld32(tS, x[0]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tmem_wait_ld32(x[q & 1]);
-          if (q < 3) tmem_ld32(tS + 32 * (q + 1), x[(q + 1) & 1]);
-          float (&v)[32] = x[q & 1];
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 32 * q + i <= hi && 32 * q + i >= lo ? v[i] : -INFINITY;
-          }
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float a, b;
-            unpack_f32x2(fma_f32x2(pack_f32x2(v[2 * i], v[2 * i + 1]), c2, neg), a, b);
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[q][2 * i], x[q][2 * i + 1]), c2, neg), a, b);
             a = exp2_fast(a);
             b = exp2_fast(b);
             l2 = add_f32x2(l2, pack_f32x2(a, b));
             w[i] = Mma<T>::pack(a, b);
           }
-          tmem_st16(tS + 16 * q, w);  // columns 16 q .. of P lie over columns of S that this thread has read
+          tmem_st16(tS + 16 * q, w);  // P lies over the first half of S, which this thread holds in registers
         }
         tmem_wait_st();
         tc_fence_before();
@@ -652,6 +698,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       }
       if (tid == 0 && g.starts && !g.whole)
         p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows | (mode == MODE_KEYS ? 1 << 16 : 0));
+      done_item();
     }
   }
   __syncthreads();

@@ -5,6 +5,8 @@
     python -m lowlat_gemm.profile_case step  --kind fp8 --tokens 8 --layers 2        (one-GPU decode step, push form)
     python -m lowlat_gemm.profile_case allreduce --rows 8 --cols 8192                (pull-form kernels, one rank on local memory)
     python -m lowlat_gemm.profile_case relayout --rows 28672 --cols 512              (block-scale layout converter)
+    python -m lowlat_gemm.profile_case attention --batch 32 --new 1 --kv 4096 --heads 64 --kv-heads 8 --cache e4m3
+    python -m lowlat_gemm.profile_case cache --batch 8 --new 1024 --kv 4096 --kv-heads 8 --cache e4m3   (append and read)
 
 Every call of `gemm` reads a different copy of the weight and the copies together exceed the L2 cache, so DRAM counters
 mean what they mean in a decode step, while the whole case holds well under 2 GB on the device and launches only a
@@ -108,6 +110,42 @@ def run_relayout(a) -> None:
     print(f"scale relayout [{a.rows}, {a.cols}]: {a.calls} round trips, restored={ok}")
 
 
+def _paged(a):
+    """A cache of a.batch sequences of a.kv tokens, pages of 64 in random order: (cache arguments, page table, lengths)."""
+    dev = torch.device("cuda", 0)
+    g = torch.Generator(device=dev).manual_seed(4)
+    per = -(-a.kv // 64)
+    table = torch.randperm(a.batch * per, generator=g, device=dev, dtype=torch.int32).view(a.batch, per)
+    shape = (a.batch * per, a.kv_heads, 64, a.dim)
+    kv = [torch.randn(shape, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2)]
+    scales = {}
+    if a.cache == "e4m3":
+        kv = [(x * 64).clamp(-448, 448).to(torch.float8_e4m3fn) for x in kv]
+        scales = {n: torch.full(shape[:3], 121, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu) for n in ("k_scale", "v_scale")}
+    return kv, scales, table, torch.full((a.batch,), a.kv, dtype=torch.int32, device=dev), g
+
+
+def run_attention(a) -> None:
+    kv, scales, table, lens, g = _paged(a)
+    q = torch.randn(a.batch * a.new, a.heads, a.dim, generator=g, device=lens.device).to(torch.bfloat16)
+    for _ in range(a.calls):
+        y = L.paged_attention(q, *kv, table, lens, window=a.window, **scales)
+    torch.cuda.synchronize()
+    print(f"attention batch={a.batch} new={a.new} kv={a.kv} heads={a.heads}/{a.kv_heads} {a.cache}: {a.calls} calls, "
+          f"|y| sum {float(y.float().abs().sum()):.4g}")
+
+
+def run_cache(a) -> None:
+    kv, scales, table, lens, g = _paged(a)
+    k = torch.randn(a.batch * a.new, a.kv_heads, a.dim, generator=g, device=lens.device).to(torch.bfloat16)
+    for _ in range(a.calls):
+        L.kv_append(k, k, *kv, table, lens, **scales)
+        back, _ = L.kv_read(*kv, table, lens, a.kv, **scales)
+    torch.cuda.synchronize()
+    print(f"cache batch={a.batch} new={a.new} kv={a.kv} kv_heads={a.kv_heads} {a.cache}: {a.calls} calls, "
+          f"|k| sum {float(back.float().abs().sum()):.4g}")
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="what", required=True)
@@ -138,8 +176,19 @@ def main() -> None:
     t.add_argument("--rows", type=int, default=28672)
     t.add_argument("--cols", type=int, default=512)
     t.add_argument("--calls", type=int, default=6)
+    for name in ("attention", "cache"):
+        c = sub.add_parser(name)
+        c.add_argument("--batch", type=int, default=32)
+        c.add_argument("--new", type=int, default=1)
+        c.add_argument("--kv", type=int, default=4096)
+        c.add_argument("--kv-heads", type=int, default=8)
+        c.add_argument("--heads", type=int, default=64)
+        c.add_argument("--dim", type=int, default=128)
+        c.add_argument("--window", type=int, default=0)
+        c.add_argument("--cache", choices=("e4m3", "bf16"), default="e4m3")
+        c.add_argument("--calls", type=int, default=4)
     a = ap.parse_args()
-    {"gemm": run_gemm, "quant": run_quant, "step": run_step, "allreduce": run_allreduce, "relayout": run_relayout}[a.what](a)
+    {"attention": run_attention, "cache": run_cache, "gemm": run_gemm, "quant": run_quant, "step": run_step, "allreduce": run_allreduce, "relayout": run_relayout}[a.what](a)
 
 
 if __name__ == "__main__":
