@@ -92,7 +92,17 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     // the tile kernel takes the maximum of unscaled scores: a positive scale (1e-30 for 0), the sign goes to q
     p.negate = scale_log2 < 0.f;
     p.scale_log2 = fmaxf(fabsf(scale_log2), 1e-30f);
-    cudaError_t e = f16 ? attn_tiles_launch_f16(p, fp8, plan.m.ctas, pdl_on(), s) : attn_tiles_launch_bf16(p, fp8, plan.m.ctas, pdl_on(), s);
+    // boxes of rows that share a page, at most a loader warp's 32 and at least the 8 of a swizzle atom
+    CUtensorMap mk{}, mv{};
+    int box = 32;
+    while (p.c.page_size % box) box /= 2;
+    const int es = fp8 ? 1 : 2;
+    const int64_t ks[3] = {p.c.k_page, p.c.k_head, p.c.k_slot}, vs[3] = {p.c.v_page, p.c.v_head, p.c.v_slot};
+    const bool maps = box >= 8 && p.c.pages > 0 && make_paged_map(&mk, p.c.k, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, ks, box) &&
+                      make_paged_map(&mv, p.c.v, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, vs, box);
+    p.box = maps ? box : 0;
+    cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s)
+                        : attn_tiles_launch_bf16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s);
     if (e != cudaSuccess) return e;
     e = attn_combine_launch(p, f16, plan.m.ctas, kTileRows, s);
     if (e != cudaSuccess) return e;

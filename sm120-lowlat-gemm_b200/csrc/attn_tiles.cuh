@@ -14,8 +14,11 @@
 // Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
 // even key tiles, B the odd ones, and each leaves a partial result of its own.
 // The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
-// Loaders gather whole rows page by page: 16-bit rows with cp.async straight into the swizzled tile, e4m3 rows through a
-// staging ring private to each thread, widened with their power of two applied (exact) on the way to the tile.
+// Loaders: each of four warps fills a quarter of a tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
+// of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. 16-bit rows land in the swizzled
+// tile; e4m3 rows land in a staging ring and are widened into the tile with their power of two applied (exact).
+// (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
+// waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
 // P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
 #pragma once
 
@@ -119,6 +122,14 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Box of a page: x = element, then slot, head, page.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int slot, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(x), "r"(slot), "r"(head), "r"(page)
+      : "memory");
+}
+
 // Ring of mbarrier phases: slot i of n, used round after round.
 struct Ring {
   int slot = 0;
@@ -133,7 +144,7 @@ struct Ring {
 
 // Barriers in the header: word offsets of 8 bytes from the start of shared memory.
 enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24,
-             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29 };
+             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29, BAR_RAW_FULL = 33 };
 constexpr int kSegRing = 4;        // segments published ahead of the roles that work on them
 constexpr int kSegReaders = 13;    // warps that read a segment
 
@@ -144,7 +155,8 @@ __device__ __forceinline__ int tiles_mode(const Segment& g, int group) {
 }
 
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ AttnDev p) {
+__global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v) {
   using Cfg = TilesCfg<T, FP8, D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   if (tid == 0) {
     abort_word = drain_word = 0u;
     for (int i = 0; i < Cfg::kSlots; ++i) {
-      mbar_init(bar(BAR_KV_FULL + i), 128);
+      mbar_init(bar(BAR_KV_FULL + i), 4);
       mbar_init(bar(BAR_KV_EMPTY + i), 1);
     }
     mbar_init(bar(BAR_Q_FULL), 128);
@@ -169,6 +181,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       mbar_init(bar(BAR_PV_DONE + s), 1);
     }
     mbar_init(bar(BAR_DONE), 1);
+    for (int i = 0; i < 4 * Cfg::kStageRing; ++i) mbar_init(bar(BAR_RAW_FULL + i), 1);
     for (int i = 0; i < kSegRing; ++i) {
       mbar_init(bar(BAR_SEG_FULL + i), 1);
       mbar_init(bar(BAR_SEG_EMPTY + i), kSegReaders);
@@ -212,34 +225,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   if (warp >= 8 && warp < 12) {
     // ================================================================================================ loaders
     regs_down<64>();  // 512 threads start with 128 each: 2 x 200 (softmax) + 64 + 48 = 4 x 128
-    const int lt = tid - 256, lw = warp - 8;
+    const int lt = tid - 256, lw = warp - 8;                       // this warp fills rows 32 lw .. 32 lw + 31 of every tile
     Ring ring;
     uint32_t q_phase = 1;  // the first wait for an empty Q passes
-    // arrivals owed for groups of copies that may still be in flight, oldest first (0: none)
-    uint32_t owed0 = 0, owed1 = 0;
-    auto settle = [&]() {
-      if (owed0 | owed1) {
-        cp_async_wait<0>();
-        fence_async_shared();
-        if (owed0) mbar_arrive(owed0);
-        if (owed1) mbar_arrive(owed1);
-        owed0 = owed1 = 0u;
-      }
-    };
-    auto owe = [&](uint32_t b) {
-      cp_async_commit();
-      cp_async_wait<2>();
-      if (owed0) {
-        fence_async_shared();
-        mbar_arrive(owed0);
-      }
-      owed0 = owed1;
-      owed1 = b;
-    };
-    int64_t k_off = -1, v_off = -1;  // byte offsets of row `lt` of the tile located last
-    uint32_t k_sc = 0, v_sc = 0;
     const Segment* seg = nullptr;
-    // The page table's entry for row `lt` is requested a tile before it is used.
+    // A tile's row 32 lw + lane: its page (-1: no row, reads as zeros) and slot. The page table's entry is requested a tile ahead.
+    struct Row {
+      int pg, slot;
+      uint32_t k_sc, v_sc;
+    };
     int entry = 0;
     auto in_use = [&](int j) {
       const int key = j * kTilesKT + lt;
@@ -249,75 +243,104 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       if (in_use(j)) entry = c.table[(int64_t)seg->seq * c.table_stride + (j * kTilesKT + lt) / c.page_size];
     };
     auto locate = [&](int j) {
-      const int key = j * kTilesKT + lt;
-      k_off = v_off = -1;
-      k_sc = v_sc = 0u;
+      Row r{-1, 0, 0u, 0u};
       const int pg = entry;
       look_up(j + 1);
       if (in_use(j)) {
-        const int slot = key % c.page_size;
+        r.slot = (j * kTilesKT + lt) % c.page_size;
         if ((unsigned)pg >= (unsigned)c.pages) {
           atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
         } else {
-          k_off = pg * c.k_page + seg->head * c.k_head + slot * c.k_slot;
-          v_off = pg * c.v_page + seg->head * c.v_head + slot * c.v_slot;
+          r.pg = pg;
           if constexpr (FP8) {
-            k_sc = c.ks[pg * c.ks_page + seg->head * c.ks_head + slot * c.ks_slot];
-            v_sc = c.vs[pg * c.vs_page + seg->head * c.vs_head + slot * c.vs_slot];
+            r.k_sc = c.ks[pg * c.ks_page + seg->head * c.ks_head + r.slot * c.ks_slot];
+            r.v_sc = c.vs[pg * c.vs_page + seg->head * c.vs_head + r.slot * c.vs_slot];
           }
         }
       }
+      return r;
     };
-    // 16-bit rows: straight into slot `ring.slot`
-    auto copy16 = [&](const unsigned char* src, int64_t off) {
-      if (!mbar_try(bar(BAR_KV_EMPTY + ring.slot), ring.phase ^ 1u)) {
-        settle();
-        wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
-      }
+    // byte offset of a row of K or V, -1 for none
+    auto offset = [&](const Row& r, bool is_v) -> int64_t {
+      if (r.pg < 0) return -1;
+      return is_v ? r.pg * c.v_page + seg->head * c.v_head + r.slot * c.v_slot : r.pg * c.k_page + seg->head * c.k_head + r.slot * c.k_slot;
+    };
+    const int box = p.box;                                         // rows of a TMA box, 0: gather every row
+    // Whole quarter tiles come by TMA, boxes of rows that lie in one page; quarters with rows that are not there are gathered.
+    auto by_tma = [&](const Row& r) { return box > 0 && __all_sync(0xffffffffu, r.pg >= 0); };
+    // 16-bit rows: straight into slot `ring.slot`, swizzled
+    auto copy16 = [&](const Row& r, bool is_v) {
+      wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
       if (!ok) return;
-      const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
-      constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte pieces per row, rows per warp instruction
+      const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile, full = bar(BAR_KV_FULL + ring.slot);
+      if (by_tma(r)) {
+        if (lane == 0) mbar_expect_tx(full, 32 * D * 2);
+        const int at = (lane / Cfg::kHalves) * box, half = lane % Cfg::kHalves;
+        const int pg = __shfl_sync(0xffffffffu, r.pg, at & 31), slot = __shfl_sync(0xffffffffu, r.slot, at & 31);
+        if (at < 32) tma_load_4d(dst + half * Cfg::kHalf + (lw * 32 + at) * 128, is_v ? &map_v : &map_k, full, half * 64, slot, seg->head, pg);
+      } else {
+        const int64_t off = offset(r, is_v);
+        const unsigned char* const src = is_v ? c.v : c.k;
+        constexpr int CH = D / 8, RP = 32 / CH;                    // 16-byte pieces per row, rows per warp instruction
 #pragma unroll 4
-      for (int i = 0; i < 32 / RP; ++i) {
-        const int r = i * RP + lane / CH, ch = lane % CH, row = lw * 32 + r;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        cp_async16(dst + (ch >> 3) * Cfg::kHalf + row * 128 + (((ch & 7) ^ (row & 7)) << 4), src + (o >= 0 ? o + ch * 16 : 0), o >= 0 ? 16u : 0u);
+        for (int i = 0; i < 32 / RP; ++i) {
+          const int q = i * RP + lane / CH, ch = lane % CH, row = lw * 32 + q;
+          const int64_t o = __shfl_sync(0xffffffffu, off, q);
+          cp_async16(dst + (ch >> 3) * Cfg::kHalf + row * 128 + (((ch & 7) ^ (row & 7)) << 4), src + (o >= 0 ? o + ch * 16 : 0), o >= 0 ? 16u : 0u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
       }
-      owe(bar(BAR_KV_FULL + ring.slot));
+      __syncwarp();
       ring.next(Cfg::kSlots);
     };
-    // e4m3 rows: `stage` fetches into the thread's own staging bytes, `widen` converts them into the ring
-    constexpr int CH8 = D / 16, RP8 = 32 / CH8, IT8 = 32 / RP8;
-    int staged = 0, widened = 0;
-    auto stage = [&](const unsigned char* src, int64_t off, uint32_t sc) {
+    // e4m3 rows: `stage` fetches the warp's quarter as it is, `widen` converts it into the ring
+    constexpr int CH8 = D / 16, RP8 = 32 / CH8, IT8 = 32 / RP8;    // 16-byte pieces per row, rows per warp instruction, instructions
+    int staged = 0;
+    Ring raw;
+    auto stage = [&](const Row& r, bool is_v) {
       const int at = staged % 3;
-      const uint32_t dst = base + Cfg::kStageAt + at * Cfg::kStage + lt * 16;
-#pragma unroll
-      for (int i = 0; i < IT8; ++i) {
-        const int r = i * RP8 + lane / CH8, ch = lane % CH8;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        cp_async16(dst + i * 2048, src + (o >= 0 ? o + ch * 16 : 0), o >= 0 ? 16u : 0u);
+      const uint32_t dst = base + Cfg::kStageAt + at * Cfg::kStage + lw * (32 * D), full = bar(BAR_RAW_FULL + 4 * at + lw);
+      if (by_tma(r)) {
+        if (lane == 0) mbar_expect_tx(full, 32 * D);
+        const int q = lane * box;
+        const int pg = __shfl_sync(0xffffffffu, r.pg, q & 31), slot = __shfl_sync(0xffffffffu, r.slot, q & 31);
+        if (q < 32) tma_load_4d(dst + q * D, is_v ? &map_v : &map_k, full, 0, slot, seg->head, pg);
+      } else {
+        const int64_t off = offset(r, is_v);
+        const unsigned char* const src = is_v ? c.v : c.k;
+#pragma unroll 4
+        for (int i = 0; i < IT8; ++i) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, i * RP8 + lane / CH8);
+          cp_async16(dst + i * 512 + lane * 16, src + (o >= 0 ? o + (lane % CH8) * 16 : 0), o >= 0 ? 16u : 0u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_shared();  // a later TMA writes here
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
       }
-      cp_async_commit();
-      asm volatile("st.shared.u8 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 128 + lt), "r"(sc) : "memory");
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 128 + lt), "r"(is_v ? r.v_sc : r.k_sc) : "memory");
+      __syncwarp();
       ++staged;
     };
-    auto widen = [&](bool last) {
-      if (last) cp_async_wait<0>();
-      else cp_async_wait<1>();
-      __syncwarp();
+    auto widen = [&]() {
+      wait(BAR_RAW_FULL + 4 * raw.slot + lw, raw.phase, ST_CONVERT_WAIT);
       wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_CONVERT_WAIT);
       if (!ok) return;
-      const int at = widened % 3;
-      const uint32_t src = base + Cfg::kStageAt + at * Cfg::kStage + lt * 16;
+      const uint32_t src = base + Cfg::kStageAt + raw.slot * Cfg::kStage + lw * (32 * D) + lane * 16;
+      const uint32_t scales = base + Cfg::kScaleAt + raw.slot * 128 + lw * 32;
       const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < IT8; ++i) {
-        const int r = i * RP8 + lane / CH8, ch = lane % CH8, row = lw * 32 + r;
-        const uint4 raw = lds16(src + i * 2048);
+        const int q = i * RP8 + lane / CH8, ch = lane % CH8, row = lw * 32 + q;
+        const uint4 v = lds16(src + i * 512);
         uint32_t b;
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(base + Cfg::kScaleAt + at * 128 + row) : "memory");
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(scales + q) : "memory");
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) Widen<T>::four(w[j], o[2 * j], o[2 * j + 1]);
@@ -348,13 +371,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a1), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
       }
       fence_async_shared();
-      mbar_arrive(bar(BAR_KV_FULL + ring.slot));
+      __syncwarp();  // and the stage may be fetched into again
+      if (lane == 0) mbar_arrive(bar(BAR_KV_FULL + ring.slot));
       ring.next(Cfg::kSlots);
-      ++widened;
-      __syncwarp();  // the stage may be fetched into again
+      raw.next(3);
     };
     auto load_q = [&]() {
-      settle();
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
       if (!ok) return;
@@ -380,59 +402,45 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
       // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
       look_up(seg->tile0);
+      Row next = locate(seg->tile0), held{};
       if constexpr (!FP8) {
-        locate(seg->tile0);
-        int64_t v_prev = -1;
         for (int j = seg->tile0; j < seg->tile1; ++j) {
-          const int64_t ko = k_off, vo = v_off;
-          locate(j + 1);
-          copy16(c.k, ko);
+          const Row row = next;
+          next = locate(j + 1);
+          copy16(row, false);
           if (j == seg->tile0) load_q();
-          if (keys) {
-            if (j > seg->tile0) copy16(c.v, v_prev);
-            v_prev = vo;
-          } else {
-            copy16(c.v, vo);
-          }
+          if (!keys) copy16(row, true);
+          else if (j > seg->tile0) copy16(held, true);
+          held = row;
         }
-        if (keys) copy16(c.v, v_prev);
+        if (keys) copy16(held, true);
       } else {
-        // the same sequence, every tile fetched two places ahead of its widening
+        // the same sequence, every tile fetched three places ahead of its widening
         const int n = 2 * (seg->tile1 - seg->tile0);
-        int64_t v_at[2] = {-1, -1};
-        uint32_t v_scale[2] = {0u, 0u};
-        int next_k = seg->tile0;
-        auto is_k = [&](int i) { return keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0; };
-        int vq_in = 0, vq_out = 0;
+        int at = seg->tile0;
+        Row older{};  // rows whose V is still to come: `older` (when the streams take turns), then `held`
         auto fetch = [&](int i) {
-          if (is_k(i)) {
-            locate(next_k++);
-            stage(c.k, k_off, k_sc);
-            if (vq_in & 1) {
-              v_at[1] = v_off;
-              v_scale[1] = v_sc;
-            } else {
-              v_at[0] = v_off;
-              v_scale[0] = v_sc;
-            }
-            ++vq_in;
+          const bool is_k = keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0;
+          if (is_k) {
+            older = held;
+            held = next;
+            next = locate(++at);
+            stage(held, false);
           } else {
-            stage(c.v, (vq_out & 1) ? v_at[1] : v_at[0], (vq_out & 1) ? v_scale[1] : v_scale[0]);
-            ++vq_out;
+            stage(keys && i < n - 1 ? older : held, true);
           }
         };
         fetch(0);
         load_q();
         fetch(1);
+        if (n > 2) fetch(2);
         for (int i = 0; i < n && ok; ++i) {
-          widen(i + 1 >= n);
-          if (i + 2 < n) fetch(i + 2);
+          widen();
+          if (i + 3 < n) fetch(i + 3);
         }
       }
       done_item();
     }
-    settle();
-    cp_async_wait<0>();
   } else if (warp >= 12) {
     regs_down<48>();
     if (warp == 12) {
