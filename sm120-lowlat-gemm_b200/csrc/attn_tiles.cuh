@@ -228,7 +228,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     const int lt = tid - 256, lw = warp - 8;                       // this warp fills rows 32 lw .. 32 lw + 31 of every tile
     Ring ring;
     uint32_t q_phase = 1;  // the first wait for an empty Q passes
-    const Segment* seg = nullptr;
+    // The segment at hand. Its fields are copied: the tensor core's operand reads fill the shared-memory pipe, and every load from
+    // there costs the loaders hundreds of cycles.
+    int tile0 = 0, tile1 = 0, key_lo = 0, key_hi = 0, kv_head = 0;
+    const int* table_row = nullptr;
     // A tile's row 32 lw + lane: its page (-1: no row, reads as zeros) and slot. The page table's entry is requested a tile ahead.
     struct Row {
       int pg, slot;
@@ -237,10 +240,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     int entry = 0;
     auto in_use = [&](int j) {
       const int key = j * kTilesKT + lt;
-      return j < seg->tile1 && key >= seg->keys.lo && key < seg->keys.hi;
+      return j < tile1 && key >= key_lo && key < key_hi;
     };
     auto look_up = [&](int j) {
-      if (in_use(j)) entry = c.table[(int64_t)seg->seq * c.table_stride + (j * kTilesKT + lt) / c.page_size];
+      if (in_use(j)) entry = table_row[(j * kTilesKT + lt) / c.page_size];
     };
     auto locate = [&](int j) {
       Row r{-1, 0, 0u, 0u};
@@ -253,8 +256,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         } else {
           r.pg = pg;
           if constexpr (FP8) {
-            r.k_sc = c.ks[pg * c.ks_page + seg->head * c.ks_head + r.slot * c.ks_slot];
-            r.v_sc = c.vs[pg * c.vs_page + seg->head * c.vs_head + r.slot * c.vs_slot];
+            r.k_sc = c.ks[pg * c.ks_page + kv_head * c.ks_head + r.slot * c.ks_slot];
+            r.v_sc = c.vs[pg * c.vs_page + kv_head * c.vs_head + r.slot * c.vs_slot];
           }
         }
       }
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     // byte offset of a row of K or V, -1 for none
     auto offset = [&](const Row& r, bool is_v) -> int64_t {
       if (r.pg < 0) return -1;
-      return is_v ? r.pg * c.v_page + seg->head * c.v_head + r.slot * c.v_slot : r.pg * c.k_page + seg->head * c.k_head + r.slot * c.k_slot;
+      return is_v ? r.pg * c.v_page + kv_head * c.v_head + r.slot * c.v_slot : r.pg * c.k_page + kv_head * c.k_head + r.slot * c.k_slot;
     };
     const int box = p.box;                                         // rows of a TMA box, 0: gather every row
     // Whole quarter tiles come by TMA, boxes of rows that lie in one page; quarters with rows that are not there are gathered.
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (lane == 0) mbar_expect_tx(full, 32 * D * 2);
         const int at = (lane / Cfg::kHalves) * box, half = lane % Cfg::kHalves;
         const int pg = __shfl_sync(0xffffffffu, r.pg, at & 31), slot = __shfl_sync(0xffffffffu, r.slot, at & 31);
-        if (at < 32) tma_load_4d(dst + half * Cfg::kHalf + (lw * 32 + at) * 128, is_v ? &map_v : &map_k, full, half * 64, slot, seg->head, pg);
+        if (at < 32) tma_load_4d(dst + half * Cfg::kHalf + (lw * 32 + at) * 128, is_v ? &map_v : &map_k, full, half * 64, slot, kv_head, pg);
       } else {
         const int64_t off = offset(r, is_v);
         const unsigned char* const src = is_v ? c.v : c.k;
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (lane == 0) mbar_expect_tx(full, 32 * D);
         const int q = lane * box;
         const int pg = __shfl_sync(0xffffffffu, r.pg, q & 31), slot = __shfl_sync(0xffffffffu, r.slot, q & 31);
-        if (q < 32) tma_load_4d(dst + q * D, is_v ? &map_v : &map_k, full, 0, slot, seg->head, pg);
+        if (q < 32) tma_load_4d(dst + q * D, is_v ? &map_v : &map_k, full, 0, slot, kv_head, pg);
       } else {
         const int64_t off = offset(r, is_v);
         const unsigned char* const src = is_v ? c.v : c.k;
@@ -376,11 +379,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       ring.next(Cfg::kSlots);
       raw.next(3);
     };
-    auto load_q = [&]() {
+    auto load_q = [&](const Segment& g) {
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
       if (!ok) return;
-      const int rows = seg->toks * p.group;
+      const int rows = g.toks * p.group;
+      const int64_t first = g.s.t0 + g.tok0;
       constexpr int CH = D / 8;
       const uint32_t flip = p.negate ? 0x80008000u : 0u;
 #pragma unroll 4
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows) {
           const int tok = row / p.group, hh = row - tok * p.group;
-          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(seg->s.t0 + seg->tok0 + tok) * p.q_tok + (int64_t)(seg->head * p.group + hh) * p.q_head + ch * 16);
+          v = *reinterpret_cast<const uint4*>(p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16);
           v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
         }
         const uint32_t dst = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
@@ -398,26 +402,32 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       fence_async_shared();
       mbar_arrive(bar(BAR_Q_FULL));
     };
-    while ((seg = next_item()) != nullptr) {
+    while (const Segment* const seg = next_item()) {
+      tile0 = seg->tile0;
+      tile1 = seg->tile1;
+      key_lo = seg->keys.lo;
+      key_hi = seg->keys.hi;
+      kv_head = seg->head;
+      table_row = c.table + (int64_t)seg->seq * c.table_stride;
       const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
       // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
-      look_up(seg->tile0);
-      Row next = locate(seg->tile0), held{};
+      look_up(tile0);
+      Row next = locate(tile0), held{};
       if constexpr (!FP8) {
-        for (int j = seg->tile0; j < seg->tile1; ++j) {
+        for (int j = tile0; j < tile1; ++j) {
           const Row row = next;
           next = locate(j + 1);
           copy16(row, false);
-          if (j == seg->tile0) load_q();
+          if (j == tile0) load_q(*seg);
           if (!keys) copy16(row, true);
-          else if (j > seg->tile0) copy16(held, true);
+          else if (j > tile0) copy16(held, true);
           held = row;
         }
         if (keys) copy16(held, true);
       } else {
         // the same sequence, every tile fetched three places ahead of its widening
-        const int n = 2 * (seg->tile1 - seg->tile0);
-        int at = seg->tile0;
+        const int n = 2 * (tile1 - tile0);
+        int at = tile0;
         Row older{};  // rows whose V is still to come: `older` (when the streams take turns), then `held`
         auto fetch = [&](int i) {
           const bool is_k = keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0;
@@ -431,7 +441,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           }
         };
         fetch(0);
-        load_q();
+        load_q(*seg);
         fetch(1);
         if (n > 2) fetch(2);
         for (int i = 0; i < n && ok; ++i) {
@@ -517,23 +527,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (!ok) break;
         if (mode == MODE_KEYS) {
           const int s = j & 1;
+          const bool more = j + 2 < nt;
+          if (more) k = full();
+          if (!ok) break;
           values(s, v, j < 2);
+          if (!ok) break;
+          if (more) scores(s, 0, k);
           release(BAR_KV_EMPTY + v);
-          if (j + 2 < nt) {
-            k = full();
-            if (!ok) break;
-            scores(s, 0, k);
-            release(BAR_KV_EMPTY + k);
-            if (j + 3 == nt) release(BAR_Q_EMPTY);
-          }
+          if (more) release(BAR_KV_EMPTY + k);
+          if (j + 3 == nt) release(BAR_Q_EMPTY);
         } else {
+          // both tiles are waited for ahead of P: between the products a barrier's latency would leave the tensor core idle
           const bool more = j + 1 < nt;
+          if (more) k = full();
+          if (!ok) break;
           values(0, v, j == 0);
-          if (more) {
-            k = full();
-            if (!ok) break;
-            scores(0, 0, k);
-          }
+          if (!ok) break;
+          if (more) scores(0, 0, k);
           if (mode == MODE_ROWS) {
             values(1, v, j == 0);
             if (!ok) break;
@@ -593,7 +603,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       float m = -INFINITY;                                       // running maximum, times c_log2
       uint64_t l2 = 0;                                           // two partial row sums
       int done = 0;                                              // key tiles of this stream behind us
-      for (int j = g.tile0 + (mode == MODE_KEYS ? s : 0); j < g.tile1 && ok; j += step, ++done) {
+      const int tile1 = g.tile1;
+      for (int j = g.tile0 + (mode == MODE_KEYS ? s : 0); j < tile1 && ok; j += step, ++done) {
         wait(BAR_S_FULL + s, s_phase, ST_EPILOGUE_WAIT);
         s_phase ^= 1u;
         if (!ok) break;
