@@ -46,7 +46,8 @@ Plan plan_of(const llg_attn_args& a) {
     const int blocks = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     p.f.tok_tile = blocks * 8 / group;
     const int64_t tiles = (c.tokens + p.f.tok_tile - 1) / p.f.tok_tile + c.batch;
-    lay_out(&p.f, tiles * c.kv_heads * ((keys + 63) / 64 + 1), 2 * sms, blocks * 8, c.head_dim, &p.bytes);
+    lay_out(&p.f, tiles * c.kv_heads * ((keys + 63) / 64 + 1),
+            rows_ctas_per_sm(c.dtype == LLG_DT_E4M3, c.head_dim, blocks) * sms, blocks * 8, c.head_dim, &p.bytes);
   }
   if (p.many) {
     p.m.tok_tile = kTileRows / group;

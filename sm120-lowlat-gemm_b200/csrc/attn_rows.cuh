@@ -9,14 +9,18 @@
 //   16-bit cache: K by ldmatrix, V by ldmatrix.trans.
 //   e4m3 cache: 16-byte reads of a row give a thread 16 neighbouring values; the order of head_dim inside a product is free, so
 //     they serve four consecutive k steps of K Q^T (Q is read in the same order) and eight row blocks of V^T without any
-//     transposition. bf16: the byte's exponent and mantissa are put into a bf16 as they are, which reads as value * 2^-120
-//     (subnormals included); Q and P carry 2^60 each and the fp32 results the rest, so no multiply is spent per value.
-//     f16: cvt gives the value itself. The row's power of two multiplies the score (K, in fp32) and the probability (V, bf16,
-//     exact there) or the value (V, f16, whose range is too small for the probability to carry it).
+//     transposition. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's type is: a bf16 row of
+//     q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less lose bits). The scores
+//     take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the running maximum is that of
+//     s + e, so p 2^e <= 2^8 and keeps f16's 11 bits where it matters.
 // P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
 // The running maximum moves only when a score exceeds it by more than 2^8: p <= 256 then, and the shuffles and the rescaling of
 // O are skipped for almost every tile.
+// Where 16 keys share a page (page sizes that are a multiple of 16) a tile needs one page and one address; else one per row.
 #pragma once
+
+#include <climits>
+#include <type_traits>
 
 #include "paged_kv.cuh"
 
@@ -25,7 +29,6 @@ namespace llg {
 constexpr int kRowsKT = 64;       // keys per unit, 16 per warp
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = 32 * kRowsWarps;
-constexpr int kRowsSmem = 96 * 1024;  // two CTAs per SM
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -98,24 +101,15 @@ template <typename T>
 struct Widen;
 template <>
 struct Widen<__nv_bfloat16> {
-  static constexpr bool kScaled = true;
   // bytes 1 and 3 of `w` -> bf16 pair
   static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7f007f00u) >> 4) | (w & 0x80008000u); }
   static __device__ __forceinline__ void four(uint32_t w, uint32_t& lo, uint32_t& hi) {  // bytes 0,1 -> lo; 2,3 -> hi
     lo = odd(__byte_perm(w, 0u, 0x1404));
     hi = odd(__byte_perm(w, 0u, 0x3424));
   }
-  // (a.b0, b.b0) (a.b1, b.b1) (a.b2, b.b2) (a.b3, b.b3)
-  static __device__ __forceinline__ void cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
-    o[0] = odd(__byte_perm(a, b, 0x4404));
-    o[1] = odd(__byte_perm(a, b, 0x5515));
-    o[2] = odd(__byte_perm(a, b, 0x6626));
-    o[3] = odd(__byte_perm(a, b, 0x7737));
-  }
 };
 template <>
 struct Widen<__half> {
-  static constexpr bool kScaled = false;
   static __device__ __forceinline__ uint32_t pair(uint32_t v) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
@@ -125,6 +119,7 @@ struct Widen<__half> {
     lo = pair(w & 0xffffu);
     hi = pair(w >> 16);
   }
+  // (a.b0, b.b0) (a.b1, b.b1) (a.b2, b.b2) (a.b3, b.b3)
   static __device__ __forceinline__ void cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
     const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
     o[0] = pair(x & 0xffffu);
@@ -138,11 +133,13 @@ __device__ __forceinline__ float pow2_of(uint32_t biased) { return __uint_as_flo
 
 template <typename T, bool FP8, int D, int NB>
 struct RowsCfg {
+  using Op = typename std::conditional<FP8, __half, T>::type;   // operand type of the products
+  static constexpr int kCtas = rows_ctas_per_sm(FP8, D, NB);
   static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
   static constexpr int kChunks = kRowBytes / 16;      // 16-byte pieces per row
   static constexpr int kStage = 2 * 16 * kRowBytes + (FP8 ? 32 : 0);  // per warp: K, V, the rows' scale bytes
   static constexpr int kStages = [] {
-    const int n = kRowsSmem / kRowsWarps / kStage;
+    const int n = (226 * 1024 / kCtas - 2048) / kRowsWarps / kStage;
     return n > 8 ? 8 : n;
   }();
   static constexpr int kRing = kStages * kStage;      // per warp
@@ -153,8 +150,10 @@ struct RowsCfg {
 };
 
 template <typename T, bool FP8, int D, int NB>
-__global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid_constant__ AttnDev p) {
+__global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas)) attn_rows_kernel(const __grid_constant__ AttnDev p) {
   using Cfg = RowsCfg<T, FP8, D, NB>;
+  using Op = typename Cfg::Op;
+  constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;
   constexpr int S = Cfg::kStages, CH = Cfg::kChunks, KS = D / 16, MB = D / 16;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long scratch[kRowsWarps + 4];
@@ -166,7 +165,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
   Share share = find_share<kRowsKT, kRowsThreads>(p, scratch);
   const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
   const PagedKV& c = p.c;
-  constexpr float kUp = 1.152921504606846976e18f;  // 2^60
+  const bool one_page = c.page_size % 16 == 0;  // 16 keys from a multiple of 16 on share a page
 
   Segment g;
   while (next_segment<kRowsKT>(p, share, g)) {
@@ -176,6 +175,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
 
     // ---- queries: B fragments of K Q^T, row oct of each block
     uint32_t qf[NB][KS][2];
+    float row_f[NB][2];                     // what turns a product of those rows into log2 units
     int first_key[NB][2], last_key[NB][2];  // keys that rows 2 * quad, 2 * quad + 1 of a block see: [first, last]
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -195,16 +195,35 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
             v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
           }
         }
-        if constexpr (FP8 && Widen<T>::kScaled) {
-          const __nv_bfloat162 up = __floats2bfloat162_rn(kUp, kUp);
-          *reinterpret_cast<__nv_bfloat162*>(&v.x) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v.x), up);
-          *reinterpret_cast<__nv_bfloat162*>(&v.y) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v.y), up);
-        }
         qf[nb][ks][0] = v.x;
         qf[nb][ks][1] = v.y;
       }
+      float mine = p.scale_log2;              // of row oct
+      if constexpr (kToF16) {
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
+        const float up = __uint_as_float((268u - e) << 23);  // 2^(14 - exponent of the row's largest value)
+        mine *= __uint_as_float((e - 14u) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
+            qf[nb][ks][h] = Mma<__half>::pack(f.x * up, f.y * up);
+          }
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        row_f[nb][e] = __shfl_sync(0xffffffffu, mine, (2 * quad + e) * 4);
         const int r = nb * 8 + 2 * quad + e;
         const int pos = pos0 + r / p.group;
         last_key[nb][e] = r < rows ? (p.causal ? min(pos, g.s.len - 1) : g.s.len - 1) : -1;
@@ -227,39 +246,92 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
     int64_t row_off = -1;   // lanes 0-15: byte offset of K's row for key `lane` of the next tile; 16-31: of V's row; -1: no row
     uint32_t pend = 0;      // scale byte of the row loaded last
     uint32_t pend_at = 0;
+    // one page per tile: the tile's rows [row_lo, row_hi) exist; the page table's entry is requested a tile ahead
+    int block = 0, slot0 = 0, entry = -1, row_lo = 0, row_hi = 0;
+    const int64_t x_page = lane < 16 ? c.k_page : c.v_page, x_slot = lane < 16 ? c.k_slot : c.v_slot;
+    const int64_t x_base = g.head * (lane < 16 ? c.k_head : c.v_head) + (lane & 15) * x_slot;
+    constexpr int RI = 32 / CH;             // rows per warp instruction
+    const int64_t k_lane = (lane / CH) * c.k_slot + (lane % CH) * 16, v_lane = (lane / CH) * c.v_slot + (lane % CH) * 16;
+    auto enter = [&](int t) {               // requests the entry of tile t's page
+      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
+      entry = t < nt && key0 < g.keys.hi && key0 + 16 > g.keys.lo ? c.table[(int64_t)g.seq * c.table_stride + block] : INT_MIN;
+    };
+    if (one_page) {
+      const int key0 = g.tile0 * kRowsKT + warp * 16;
+      block = key0 / c.page_size;
+      slot0 = key0 - block * c.page_size;
+      enter(0);
+    }
     auto locate = [&](int t) {  // fills row_off (and starts the load of the scale byte) for tile t
-      const int key = (g.tile0 + t) * kRowsKT + warp * 16 + (lane & 15);
       row_off = -1;
-      if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
-        const int block = key / c.page_size, slot = key - block * c.page_size;
-        const int pg = page_of(c, g.seq, block);
-        if (pg >= 0) {
-          row_off = lane < 16 ? pg * c.k_page + g.head * c.k_head + slot * c.k_slot
-                              : pg * c.v_page + g.head * c.v_head + slot * c.v_slot;
+      if (one_page) {
+        const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
+        const int pg = entry, at = slot0;
+        slot0 += kRowsKT;
+        while (slot0 >= c.page_size) {
+          slot0 -= c.page_size;
+          ++block;
+        }
+        enter(t + 1);
+        row_lo = max(g.keys.lo - key0, 0);
+        row_hi = min(g.keys.hi - key0, 16);
+        if (pg == INT_MIN) {
+          row_hi = 0;
+        } else if ((unsigned)pg >= (unsigned)c.pages) {
+          atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+          row_hi = 0;
+        } else {
+          row_off = pg * x_page + at * x_slot + x_base;
           if constexpr (FP8) {
-            const unsigned char* sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot
-                                                : c.vs + pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot;
+            const unsigned char* const sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + (at + lane) * c.ks_slot
+                                                      : c.vs + pg * c.vs_page + g.head * c.vs_head + (at + lane - 16) * c.vs_slot;
+            pend = *sc;
+          }
+        }
+        return;
+      }
+      const int key = (g.tile0 + t) * kRowsKT + warp * 16 + (lane & 15);
+      if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
+        const int b = key / c.page_size, slot = key - b * c.page_size;
+        const int pg = page_of(c, g.seq, b);
+        if (pg >= 0) {
+          row_off = pg * x_page + g.head * (lane < 16 ? c.k_head : c.v_head) + slot * x_slot;
+          if constexpr (FP8) {
+            const unsigned char* const sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot
+                                                      : c.vs + pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot;
             pend = *sc;
           }
         }
       }
     };
+    auto swizzled = [&](int row, int ch, bool is_v) {
+      if constexpr (!FP8) return ch ^ (row & 7);
+      else if constexpr (D == 128) return is_v ? ch ^ (row & 6) : ch ^ ((row & 1) << 2);
+      else return is_v ? ch ^ ((row >> 1) & 3) : ch;
+    };
     auto issue = [&](int t) {  // starts the copies of tile t, located by the call before
       const uint32_t base = ring + (t % S) * Cfg::kStage;
       if (t < nt) {
+        if (one_page) {
+          const int64_t k0 = max(__shfl_sync(0xffffffffu, row_off, 0), (int64_t)0), v0 = max(__shfl_sync(0xffffffffu, row_off, 16), (int64_t)0);
+          const unsigned char *ksrc = c.k + k0 + k_lane, *vsrc = c.v + v0 + v_lane;
 #pragma unroll
-        for (int i = 0; i < CH / 2; ++i) {
-          const int at = lane + 32 * i, row = at / CH, ch = at % CH;
-          const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
-          int kc, vc;
-          if constexpr (FP8) {
-            kc = D == 128 ? ch ^ ((row & 1) << 2) : ch;
-            vc = D == 128 ? ch ^ (row & 6) : ch ^ ((row >> 1) & 3);
-          } else {
-            kc = vc = ch ^ (row & 7);
+          for (int i = 0; i < CH / 2; ++i) {
+            const int row = lane / CH + i * RI, ch = lane % CH;
+            const uint32_t n = row >= row_lo && row < row_hi ? 16u : 0u;
+            cp_async16(base + row * Cfg::kRowBytes + swizzled(row, ch, false) * 16, ksrc, n);
+            cp_async16(base + (16 + row) * Cfg::kRowBytes + swizzled(row, ch, true) * 16, vsrc, n);
+            ksrc += RI * c.k_slot;
+            vsrc += RI * c.v_slot;
           }
-          cp_async16(base + row * Cfg::kRowBytes + kc * 16, c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
-          cp_async16(base + (16 + row) * Cfg::kRowBytes + vc * 16, c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH / 2; ++i) {
+            const int row = lane / CH + i * RI, ch = lane % CH;
+            const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
+            cp_async16(base + row * Cfg::kRowBytes + swizzled(row, ch, false) * 16, c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
+            cp_async16(base + (16 + row) * Cfg::kRowBytes + swizzled(row, ch, true) * 16, c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+          }
         }
         if constexpr (FP8) pend_at = base + 32 * Cfg::kRowBytes + lane;
       }
@@ -299,11 +371,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t a[4];
-            Widen<T>::four(w0[j], a[0], a[2]);
-            Widen<T>::four(w1[j], a[1], a[3]);
+            Widen<Op>::four(w0[j], a[0], a[2]);
+            Widen<Op>::four(w1[j], a[1], a[3]);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (nb < nb_used) Mma<T>::run(s[nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
+              if (nb < nb_used) Mma<Op>::run(s[nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
           }
         }
       } else {
@@ -314,26 +386,23 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
           ldsm_x4(kb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            if (nb < nb_used) Mma<T>::run(s[nb], a, qf[nb][ks][0], qf[nb][ks][1]);
+            if (nb < nb_used) Mma<Op>::run(s[nb], a, qf[nb][ks][0], qf[nb][ks][1]);
         }
       }
 
       // ---- softmax
       const int key0 = (g.tile0 + t) * kRowsKT + warp * 16 + oct;
-      float f0 = p.scale_log2, f1 = p.scale_log2, pv0 = 1.f, pv1 = 1.f;  // of keys oct, oct + 8
+      float kf[2] = {1.f, 1.f}, vf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};  // keys oct, oct + 8: 2^e of K, 2^e and e of V
       if constexpr (FP8) {
-        uint32_t b[4];
         const uint32_t at = kb + 32 * Cfg::kRowBytes + oct;
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[0]) : "r"(at) : "memory");
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[1]) : "r"(at + 8) : "memory");
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[2]) : "r"(at + 16) : "memory");
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b[3]) : "r"(at + 24) : "memory");
-        constexpr float up = Widen<T>::kScaled ? kUp : 1.f;
-        f0 *= pow2_of(b[0]) * up;
-        f1 *= pow2_of(b[1]) * up;
-        if constexpr (Widen<T>::kScaled) {
-          pv0 = pow2_of(b[2]) * up;
-          pv1 = pow2_of(b[3]) * up;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t bk, bv;
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk) : "r"(at + 8 * e) : "memory");
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv) : "r"(at + 16 + 8 * e) : "memory");
+          kf[e] = pow2_of(bk);
+          vf[e] = pow2_of(bv);
+          ve[e] = __uint_as_float(0x4b000000u + max(bv, 27u)) - 8388735.f;  // e, not below -100: bits of 2^23 + b, less 2^23 + 127
         }
       }
       uint32_t pf[NB][2];
@@ -346,13 +415,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
         for (int e = 0; e < 4; ++e) {
           const int key = key0 + (e >> 1) * 8;
           const bool seen = key <= last_key[nb][e & 1] && key >= first_key[nb][e & 1];
-          x[e] = seen ? s[nb][e] * (e < 2 ? f0 : f1) : -INFINITY;
-          more |= x[e] > m[nb][e & 1] + 8.f;
+          x[e] = seen ? s[nb][e] * (row_f[nb][e & 1] * kf[e >> 1]) : -INFINITY;
+          more |= x[e] + ve[e >> 1] > m[nb][e & 1] + 8.f;
         }
         if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[e], x[e + 2]);
+            float mx = fmaxf(x[e] + ve[0], x[e + 2] + ve[1]);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -374,21 +443,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
           pr[e] = exp2_fast(x[e] - (mm == -INFINITY ? 0.f : mm));
           l[nb][e & 1] += pr[e];
         }
-        pf[nb][0] = transpose8x8(Mma<T>::pack(pr[0] * pv0, pr[1] * pv0));
-        pf[nb][1] = transpose8x8(Mma<T>::pack(pr[2] * pv1, pr[3] * pv1));
+        pf[nb][0] = transpose8x8(Mma<Op>::pack(pr[0] * vf[0], pr[1] * vf[0]));
+        pf[nb][1] = transpose8x8(Mma<Op>::pack(pr[2] * vf[1], pr[3] * vf[1]));
       }
 
       // ---- O^T += V^T P^T
       if constexpr (FP8) {
-        uint32_t sc[2] = {0u, 0u};  // f16: the rows' powers of two, keys (2 quad, 2 quad + 1) and those + 8
-        if constexpr (!Widen<T>::kScaled) {
-          uint32_t b0, b1;
-          const uint32_t at = kb + 32 * Cfg::kRowBytes + 16 + 2 * quad;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(b0) : "r"(at) : "memory");
-          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(b1) : "r"(at + 8) : "memory");
-          sc[0] = Mma<T>::pack(pow2_of(b0 & 0xffu), pow2_of(b0 >> 8));
-          sc[1] = Mma<T>::pack(pow2_of(b1 & 0xffu), pow2_of(b1 >> 8));
-        }
         constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (head_dim = 16 * oct + ..., or 8 * oct + ...)
         uint32_t w[4][W];
 #pragma unroll
@@ -405,21 +465,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < W; ++j) {
           uint32_t lo[4], hi[4];
-          Widen<T>::cross(w[0][j], w[1][j], lo);
-          Widen<T>::cross(w[2][j], w[3][j], hi);
-          if constexpr (!Widen<T>::kScaled) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              *reinterpret_cast<__half2*>(&lo[e]) = __hmul2(*reinterpret_cast<__half2*>(&lo[e]), *reinterpret_cast<__half2*>(&sc[0]));
-              *reinterpret_cast<__half2*>(&hi[e]) = __hmul2(*reinterpret_cast<__half2*>(&hi[e]), *reinterpret_cast<__half2*>(&sc[1]));
-            }
-          }
+          Widen<Op>::cross(w[0][j], w[1][j], lo);
+          Widen<Op>::cross(w[2][j], w[3][j], hi);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (nb < nb_used) Mma<T>::run(o[nb][2 * j + h], a, pf[nb][0], pf[nb][1]);
+              if (nb < nb_used) Mma<Op>::run(o[nb][2 * j + h], a, pf[nb][0], pf[nb][1]);
           }
         }
       } else {
@@ -430,7 +483,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
           ldsm_x4_t(vb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            if (nb < nb_used) Mma<T>::run(o[nb][mb], a, pf[nb][0], pf[nb][1]);
+            if (nb < nb_used) Mma<Op>::run(o[nb][mb], a, pf[nb][0], pf[nb][1]);
         }
       }
       __syncwarp();          // every lane has read the stage before the next issue overwrites it
@@ -443,7 +496,6 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
     float* const mo = reinterpret_cast<float*>(smem);                      // [warp][row][kPad]
     float* const mm = mo + kRowsWarps * Cfg::kRows * Cfg::kPad;             // [warp][row]
     float* const ml = mm + kRowsWarps * Cfg::kRows;
-    constexpr float kDown = FP8 && Widen<T>::kScaled ? kUp : 1.f;           // what is left of 2^-120 in the accumulators
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       if (nb >= nb_used) continue;
@@ -462,8 +514,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           const int d0 = FP8 ? (D / 8) * oct + 2 * mb : 16 * mb + oct, d1 = FP8 ? d0 + 1 : d0 + 8;
-          dst[d0] = o[nb][mb][e] * kDown;
-          dst[d1] = o[nb][mb][e + 2] * kDown;
+          dst[d0] = o[nb][mb][e];
+          dst[d1] = o[nb][mb][e + 2];
         }
       }
     }

@@ -82,6 +82,12 @@ struct AttnDev {
                           // 1 << 16 in the last: every CTA left two parts, the second 128 rows behind the first
 };
 
+// CTAs of the few-row kernel that fit an SM: four where a tile's key rows and accumulators are small (e4m3 rows, or head_dim 64,
+// with 8 rows), which hides the chain from a load to the next product better than longer rings; three and two otherwise.
+__host__ __device__ constexpr int rows_ctas_per_sm(bool fp8, int head_dim, int blocks) {
+  return fp8 || head_dim == 64 ? (blocks == 1 ? 4 : blocks == 2 ? 3 : 2) : 2;
+}
+
 // Keys [lo, hi) that any row of token tile [tf, tf + cnt) sees.
 struct KeyRange {
   int lo, hi;
