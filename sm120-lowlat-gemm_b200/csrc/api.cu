@@ -118,18 +118,20 @@ bool make_sf_map(CUtensorMap* m, const void* ptr, int64_t row_bytes, int64_t row
 }  // namespace
 
 bool make_paged_map(CUtensorMap* m, const void* ptr, int head_dim, int elem_bytes, int slots, int heads, int pages, const int64_t stride[3],
-                    int box_rows) {
+                    int box_rows, bool swizzle) {
   auto fn = encode_fn();
   if (!fn) return false;
   for (int i = 0; i < 3; ++i)
     if (stride[i] <= 0 || stride[i] % 16 || stride[i] >= (int64_t)1 << 40) return false;
   const bool wide = elem_bytes == 2;
+  const int width = head_dim * elem_bytes > 128 ? 128 : head_dim * elem_bytes;  // bytes
   cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)slots, (cuuint64_t)heads, (cuuint64_t)pages};
   cuuint64_t strides[3] = {(cuuint64_t)stride[2], (cuuint64_t)stride[1], (cuuint64_t)stride[0]};
-  cuuint32_t box[4] = {wide ? 64u : (cuuint32_t)head_dim, (cuuint32_t)box_rows, 1u, 1u};
+  cuuint32_t box[4] = {(cuuint32_t)(width / elem_bytes), (cuuint32_t)box_rows, 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUresult r = fn(m, wide ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides,
-                        box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }

@@ -86,6 +86,13 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     p.part_ml = reinterpret_cast<float*>(ws + q.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + q.part_o);
   };
+  CUtensorMap mk{}, mv{};
+  auto maps = [&](int box, bool swizzle) {
+    const int es = fp8 ? 1 : 2;
+    const int64_t ks[3] = {p.c.k_page, p.c.k_head, p.c.k_slot}, vs[3] = {p.c.v_page, p.c.v_head, p.c.v_slot};
+    return p.c.pages > 0 && make_paged_map(&mk, p.c.k, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, ks, box, swizzle) &&
+           make_paged_map(&mv, p.c.v, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, vs, box, swizzle);
+  };
   if (plan.many) {
     use(plan.m);
     p.row_min = plan.few ? kRowsMax : 0;
@@ -94,14 +101,9 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     p.negate = scale_log2 < 0.f;
     p.scale_log2 = fmaxf(fabsf(scale_log2), 1e-30f);
     // boxes of rows that share a page, at most a loader warp's 32 and at least the 8 of a swizzle atom
-    CUtensorMap mk{}, mv{};
     int box = 32;
     while (p.c.page_size % box) box /= 2;
-    const int es = fp8 ? 1 : 2;
-    const int64_t ks[3] = {p.c.k_page, p.c.k_head, p.c.k_slot}, vs[3] = {p.c.v_page, p.c.v_head, p.c.v_slot};
-    const bool maps = box >= 8 && p.c.pages > 0 && make_paged_map(&mk, p.c.k, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, ks, box) &&
-                      make_paged_map(&mv, p.c.v, p.c.head_dim, es, p.c.page_size, p.c.kv_heads, p.c.pages, vs, box);
-    p.box = maps ? box : 0;
+    p.box = box >= 8 && maps(box, !fp8) ? box : 0;
     cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s)
                         : attn_tiles_launch_bf16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s);
     if (e != cudaSuccess) return e;
@@ -114,8 +116,14 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     p.row_max = kRowsMax;
     p.negate = 0;
     p.scale_log2 = scale_log2;
+    p.box = p.c.page_size % 16 == 0 && maps(16, true) ? 16 : 0;  // a warp's 16 keys
+    auto lined_up = [](const unsigned char* base, int64_t page, int64_t head, int64_t slot) {
+      return reinterpret_cast<uintptr_t>(base) % 16 == 0 && page % 16 == 0 && head % 16 == 0 && slot == 1;
+    };
+    p.scale16 = fp8 && lined_up(p.c.ks, p.c.ks_page, p.c.ks_head, p.c.ks_slot) && lined_up(p.c.vs, p.c.vs_page, p.c.vs_head, p.c.vs_slot);
     const int blocks = plan.f.rows / 8;
-    cudaError_t e = f16 ? attn_rows_launch_f16(p, fp8, blocks, plan.f.ctas, pdl_on(), s) : attn_rows_launch_bf16(p, fp8, blocks, plan.f.ctas, pdl_on(), s);
+    cudaError_t e = f16 ? attn_rows_launch_f16(p, mk, mv, fp8, blocks, plan.f.ctas, pdl_on(), s)
+                        : attn_rows_launch_bf16(p, mk, mv, fp8, blocks, plan.f.ctas, pdl_on(), s);
     if (e != cudaSuccess) return e;
     e = attn_combine_launch(p, f16, plan.f.ctas, plan.f.rows, s);
     if (e != cudaSuccess) return e;

@@ -2,21 +2,22 @@
 //
 //   s = scale * q . k,  m = max s,  l = sum exp(s - m),  o = sum exp(s - m) v / l       one pass, running m, l and o
 //
-// Key tiles of 64 tokens; each of the CTA's four warps owns 16 of them with its own cp.async ring, softmax state and
-// accumulators, so nothing between the loads and the last merge synchronises more than a warp. The products are taken
+// Key tiles of 64 tokens; each of the CTA's four warps owns 16 of them with its own ring of stages, softmax state and
+// accumulators, so nothing between the loads and the last merge synchronises more than a warp. Sixteen rows that are all there and
+// share a page come by TMA, swizzled; others are gathered with cp.async, zeros for the missing. The products are taken
 // transposed, S^T[16 keys x rows] = K Q^T and O^T[head_dim x rows] = V^T P^T, so that the rows - 8 for a group of eight heads
 // and one token - are the narrow side (8) of mma.m16n8k16 and no row of the tensor-core tile is padding.
 //   16-bit cache: K by ldmatrix, V by ldmatrix.trans.
 //   e4m3 cache: 16-byte reads of a row give a thread 16 neighbouring values; the order of head_dim inside a product is free, so
 //     they serve four consecutive k steps of K Q^T (Q is read in the same order) and eight row blocks of V^T without any
-//     transposition. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's type is: a bf16 row of
+//     transposition, and so are the orders of the keys and of head_dim's blocks among the lanes, which keep the reads of the
+//     TMA's swizzle free of bank conflicts. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's type is: a bf16 row of
 //     q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less lose bits). The scores
 //     take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the running maximum is that of
 //     s + e, so p 2^e <= 2^8 and keeps f16's 11 bits where it matters.
 // P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
 // The running maximum moves only when a score exceeds it by more than 2^8: p <= 256 then, and the shuffles and the rescaling of
 // O are skipped for almost every tile.
-// Where 16 keys share a page (page sizes that are a multiple of 16) a tile needs one page and one address; else one per row.
 #pragma once
 
 #include <climits>
@@ -29,6 +30,14 @@ namespace llg {
 constexpr int kRowsKT = 64;       // keys per unit, 16 per warp
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = 32 * kRowsWarps;
+
+// Box of a page: x = element, then slot, head, page.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int slot, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(x), "r"(slot), "r"(head), "r"(page)
+      : "memory");
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -137,33 +146,61 @@ struct RowsCfg {
   static constexpr int kCtas = rows_ctas_per_sm(FP8, D, NB);
   static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
   static constexpr int kChunks = kRowBytes / 16;      // 16-byte pieces per row
-  static constexpr int kStage = 2 * 16 * kRowBytes + (FP8 ? 32 : 0);  // per warp: K, V, the rows' scale bytes
+  static constexpr int kParts = kRowBytes > 128 ? 2 : 1;            // a row lies in pieces of at most 128 bytes ...
+  static constexpr int kPitch = kRowBytes / kParts;                 // ... of this size, 16 rows of a piece together
+  static constexpr int kStage = 2 * 16 * kRowBytes;   // per warp: K, V
   static constexpr int kStages = [] {
-    const int n = (226 * 1024 / kCtas - 2048) / kRowsWarps / kStage;
+    const int n = (226 * 1024 / kCtas - 4096) / kRowsWarps / (kStage + 32);
     return n > 8 ? 8 : n;
   }();
   static constexpr int kRing = kStages * kStage;      // per warp
   static constexpr int kRows = NB * 8;
   static constexpr int kPad = D + 4;                  // floats between rows of the merge buffer
   static constexpr int kMerge = kRowsWarps * kRows * (kPad + 2) * 4;
-  static constexpr int kSmem = kRowsWarps * kRing > kMerge ? kRowsWarps * kRing : kMerge;
+  static constexpr int kSmem = (kRowsWarps * kRing > kMerge ? kRowsWarps * kRing : kMerge) + 1024;  // + alignment slack
 };
 
+// Place of 16-byte piece `ch` of row `row` (< 16) of K or V in a stage: what the TMA's swizzle makes of it.
+template <typename Cfg>
+__device__ __forceinline__ uint32_t rows_at(int row, int ch) {
+  if constexpr (Cfg::kPitch == 128) return (ch >> 3) * 2048 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+  else return row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
+}
+
 template <typename T, bool FP8, int D, int NB>
-__global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas)) attn_rows_kernel(const __grid_constant__ AttnDev p) {
+__global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas)) attn_rows_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v) {
   using Cfg = RowsCfg<T, FP8, D, NB>;
   using Op = typename Cfg::Op;
   constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;
   constexpr int S = Cfg::kStages, CH = Cfg::kChunks, KS = D / 16, MB = D / 16;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
   __shared__ long long scratch[kRowsWarps + 4];
+  __shared__ __align__(8) unsigned long long bars[kRowsWarps * S];
+  __shared__ unsigned char scales[FP8 ? kRowsWarps * S * 32 : 1];
+  __shared__ volatile uint32_t abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int quad = lane & 3, oct = lane >> 2;  // fragment coordinates
+  // e4m3, 128-byte rows: which key a fragment's row `oct` is, and which 16 values of head_dim a lane's V fragments hold
+  constexpr bool kMixed = FP8 && D == 128;
+  const int krow = kMixed ? (oct >> 1) + 4 * (oct & 1) : oct;
+  const int vrow0 = kMixed ? quad : 2 * quad, vrow1 = kMixed ? quad + 4 : 2 * quad + 1;  // keys of k steps 2 quad, 2 quad + 1
+  unsigned char* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  if (tid < kRowsWarps * S) {
+    mbar_init(smem_u32(&bars[tid]), 32);
+    mbar_fence_init();
+  }
+  if (tid == 0) abort_word = 0u;
   pdl_trigger();
   pdl_wait();
   if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
   Share share = find_share<kRowsKT, kRowsThreads>(p, scratch);
-  const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
+  const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing, bar = smem_u32(&bars[warp * S]);
+  const uint32_t scale_at = smem_u32(scales) + warp * S * 32;
+  int put = 0, get = 0;         // stages filled next / read next
+  uint32_t get_phase = 0;
+  bool gathered = false;        // copies of cp.async went into the ring since the last proxy fence
+  bool ok_all = true;
   const PagedKV& c = p.c;
   const bool one_page = c.page_size % 16 == 0;  // 16 keys from a multiple of 16 on share a page
 
@@ -241,20 +278,28 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       l[nb][0] = l[nb][1] = 0.f;
     }
 
-    // ---- the warp's ring: tile t holds keys [64 t + 16 warp, + 16)
+    // ---- the warp's ring: tile t holds keys [64 t + 16 warp, + 16) of the segment
     const int nt = g.tile1 - g.tile0;
-    int64_t row_off = -1;   // lanes 0-15: byte offset of K's row for key `lane` of the next tile; 16-31: of V's row; -1: no row
-    uint32_t pend = 0;      // scale byte of the row loaded last
-    uint32_t pend_at = 0;
-    // one page per tile: the tile's rows [row_lo, row_hi) exist; the page table's entry is requested a tile ahead
-    int block = 0, slot0 = 0, entry = -1, row_lo = 0, row_hi = 0;
-    const int64_t x_page = lane < 16 ? c.k_page : c.v_page, x_slot = lane < 16 ? c.k_slot : c.v_slot;
-    const int64_t x_base = g.head * (lane < 16 ? c.k_head : c.v_head) + (lane & 15) * x_slot;
-    constexpr int RI = 32 / CH;             // rows per warp instruction
-    const int64_t k_lane = (lane / CH) * c.k_slot + (lane % CH) * 16, v_lane = (lane / CH) * c.v_slot + (lane % CH) * 16;
-    auto enter = [&](int t) {               // requests the entry of tile t's page
+    const int head = g.head;
+    const int* const table_row = c.table + (int64_t)g.seq * c.table_stride;
+    // keys that every row of the tile sees: tiles inside need no mask
+    const int all_hi = p.causal ? min(pos0, g.s.len - 1) : g.s.len - 1;
+    const int all_lo = p.window > 0 ? pos0 + g.toks - p.window : 0;
+    // The tile located last. One page (16 keys from a multiple of 16 on): its page (-1: none), first slot, rows [row_lo, row_hi)
+    // that exist; the page table's entry is requested a tile ahead. Else: row_off, lanes 0-15 of K's row, 16-31 of V's, -1: none.
+    int pg = -1, at = 0, row_lo = 0, row_hi = 0;
+    int64_t row_off = -1;
+    int block = 0, slot0 = 0, entry = INT_MIN;
+    uint32_t pend = 0;         // scale byte of the lane's row
+    const bool is_v = lane >= 16;
+    const int my_row = lane & 15;
+    const unsigned char* const sc_base = FP8 ? (is_v ? c.vs + head * c.vs_head + my_row * c.vs_slot : c.ks + head * c.ks_head + my_row * c.ks_slot) : nullptr;
+    auto scale_byte = [&]() -> uint32_t {  // of the lane's row of the page located last
+      return sc_base[pg * (is_v ? c.vs_page : c.ks_page) + at * (is_v ? c.vs_slot : c.ks_slot)];
+    };
+    auto enter = [&](int t) {  // requests the entry of tile t's page
       const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
-      entry = t < nt && key0 < g.keys.hi && key0 + 16 > g.keys.lo ? c.table[(int64_t)g.seq * c.table_stride + block] : INT_MIN;
+      entry = t < nt && key0 < g.keys.hi && key0 + 16 > g.keys.lo ? table_row[block] : INT_MIN;
     };
     if (one_page) {
       const int key0 = g.tile0 * kRowsKT + warp * 16;
@@ -262,100 +307,105 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       slot0 = key0 - block * c.page_size;
       enter(0);
     }
-    auto locate = [&](int t) {  // fills row_off (and starts the load of the scale byte) for tile t
-      row_off = -1;
+    auto locate = [&](int t) {
+      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
       if (one_page) {
-        const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
-        const int pg = entry, at = slot0;
+        pg = entry;
+        at = slot0;
         slot0 += kRowsKT;
         while (slot0 >= c.page_size) {
           slot0 -= c.page_size;
           ++block;
         }
         enter(t + 1);
-        row_lo = max(g.keys.lo - key0, 0);
-        row_hi = min(g.keys.hi - key0, 16);
-        if (pg == INT_MIN) {
-          row_hi = 0;
-        } else if ((unsigned)pg >= (unsigned)c.pages) {
-          atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
-          row_hi = 0;
+        row_lo = g.keys.lo - key0;
+        row_hi = g.keys.hi - key0;
+        if ((unsigned)pg >= (unsigned)c.pages) {
+          if (pg != INT_MIN) atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+          pg = -1;
+        } else if constexpr (FP8) {
+          if (!p.scale16) pend = scale_byte();
+        }
+      } else {
+        const int key = key0 + my_row;
+        row_off = -1;
+        if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
+          const int b = key / c.page_size, slot = key - b * c.page_size;
+          const int q = page_of(c, g.seq, b);
+          if (q >= 0) {
+            row_off = is_v ? q * c.v_page + head * c.v_head + slot * c.v_slot : q * c.k_page + head * c.k_head + slot * c.k_slot;
+            if constexpr (FP8)
+              pend = is_v ? c.vs[q * c.vs_page + head * c.vs_head + slot * c.vs_slot] : c.ks[q * c.ks_page + head * c.ks_head + slot * c.ks_slot];
+          }
+        }
+      }
+    };
+    auto issue = [&](int t) {  // starts the copies of tile t, located by the call before, into stage `put`
+      if (t >= nt) return;
+      const uint32_t dst = ring + put * Cfg::kStage, full = bar + 8u * put;
+      bool there = true;       // the lane's row
+      if (one_page && p.box && pg >= 0 && row_lo <= 0 && row_hi >= 16) {
+        if (gathered) {
+          fence_async_shared();
+          __syncwarp();
+          gathered = false;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(full, Cfg::kStage);
+#pragma unroll
+          for (int h = 0; h < Cfg::kParts; ++h) {
+            tma_load_4d(dst + h * 2048, &map_k, full, h * 64, at, head, pg);
+            tma_load_4d(dst + 16 * Cfg::kRowBytes + h * 2048, &map_v, full, h * 64, at, head, pg);
+          }
+        } else if (FP8 && p.scale16 && lane <= 2) {  // the 16 scale bytes of K (lane 1) and V (lane 2)
+          cp_async16(scale_at + put * 32 + (lane - 1) * 16, lane == 1 ? c.ks + pg * c.ks_page + head * c.ks_head + at : c.vs + pg * c.vs_page + head * c.vs_head + at, 16u);
+          cp_async_arrive_noinc(full);
         } else {
-          row_off = pg * x_page + at * x_slot + x_base;
-          if constexpr (FP8) {
-            const unsigned char* const sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + (at + lane) * c.ks_slot
-                                                      : c.vs + pg * c.vs_page + g.head * c.vs_head + (at + lane - 16) * c.vs_slot;
-            pend = *sc;
-          }
+          mbar_arrive(full);
         }
-        return;
-      }
-      const int key = (g.tile0 + t) * kRowsKT + warp * 16 + (lane & 15);
-      if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
-        const int b = key / c.page_size, slot = key - b * c.page_size;
-        const int pg = page_of(c, g.seq, b);
-        if (pg >= 0) {
-          row_off = pg * x_page + g.head * (lane < 16 ? c.k_head : c.v_head) + slot * x_slot;
-          if constexpr (FP8) {
-            const unsigned char* const sc = lane < 16 ? c.ks + pg * c.ks_page + g.head * c.ks_head + slot * c.ks_slot
-                                                      : c.vs + pg * c.vs_page + g.head * c.vs_head + slot * c.vs_slot;
-            pend = *sc;
-          }
+        if (FP8 && p.scale16) {
+          put = put + 1 == S ? 0 : put + 1;
+          return;
         }
-      }
-    };
-    auto swizzled = [&](int row, int ch, bool is_v) {
-      if constexpr (!FP8) return ch ^ (row & 7);
-      else if constexpr (D == 128) return is_v ? ch ^ (row & 6) : ch ^ ((row & 1) << 2);
-      else return is_v ? ch ^ ((row >> 1) & 3) : ch;
-    };
-    auto issue = [&](int t) {  // starts the copies of tile t, located by the call before
-      const uint32_t base = ring + (t % S) * Cfg::kStage;
-      if (t < nt) {
+      } else {
         if (one_page) {
-          const int64_t k0 = max(__shfl_sync(0xffffffffu, row_off, 0), (int64_t)0), v0 = max(__shfl_sync(0xffffffffu, row_off, 16), (int64_t)0);
-          const unsigned char *ksrc = c.k + k0 + k_lane, *vsrc = c.v + v0 + v_lane;
-#pragma unroll
-          for (int i = 0; i < CH / 2; ++i) {
-            const int row = lane / CH + i * RI, ch = lane % CH;
-            const uint32_t n = row >= row_lo && row < row_hi ? 16u : 0u;
-            cp_async16(base + row * Cfg::kRowBytes + swizzled(row, ch, false) * 16, ksrc, n);
-            cp_async16(base + (16 + row) * Cfg::kRowBytes + swizzled(row, ch, true) * 16, vsrc, n);
-            ksrc += RI * c.k_slot;
-            vsrc += RI * c.v_slot;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < CH / 2; ++i) {
-            const int row = lane / CH + i * RI, ch = lane % CH;
-            const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
-            cp_async16(base + row * Cfg::kRowBytes + swizzled(row, ch, false) * 16, c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
-            cp_async16(base + (16 + row) * Cfg::kRowBytes + swizzled(row, ch, true) * 16, c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
-          }
+          row_off = -1;
+          if (FP8 && pg >= 0 && p.scale16) pend = scale_byte();
+          if (pg >= 0 && my_row >= row_lo && my_row < row_hi)
+            row_off = is_v ? pg * c.v_page + head * c.v_head + (at + my_row) * c.v_slot : pg * c.k_page + head * c.k_head + (at + my_row) * c.k_slot;
         }
-        if constexpr (FP8) pend_at = base + 32 * Cfg::kRowBytes + lane;
+        there = row_off >= 0;
+#pragma unroll 2
+        for (int i = 0; i < CH / 2; ++i) {
+          const int row = lane / CH + i * (32 / CH), ch = lane % CH;
+          const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
+          cp_async16(dst + rows_at<Cfg>(row, ch), c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
+          cp_async16(dst + 16 * Cfg::kRowBytes + rows_at<Cfg>(row, ch), c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+        }
+        cp_async_arrive_noinc(full);
+        gathered = true;
       }
-      cp_async_commit();
-    };
-    auto settle = [&]() {  // the scale byte requested with the last located tile goes into that tile's stage
-      if constexpr (FP8) {
-        if (pend_at != 0u) asm volatile("st.shared.u8 [%0], %1;" ::"r"(pend_at), "r"(row_off >= 0 ? pend : 0u) : "memory");
-        pend_at = 0u;
-      }
+      if constexpr (FP8) asm volatile("st.shared.u8 [%0], %1;" ::"r"(scale_at + put * 32 + lane), "r"(there ? pend : 0u) : "memory");
+      put = put + 1 == S ? 0 : put + 1;
     };
     for (int t = 0; t < S - 1; ++t) {
       locate(t);
       issue(t);
-      settle();
     }
     locate(S - 1);
 
     for (int t = 0; t < nt; ++t) {
-      cp_async_wait<S - 2>();
+      const uint32_t kb = ring + get * Cfg::kStage, vb = kb + 16 * Cfg::kRowBytes, sb = scale_at + get * 32;
+      if (ok_all && !mbar_wait(bar + 8u * get, get_phase, &abort_word)) {
+        ok_all = false;
+        atomicCAS(c.status, 0u, (unsigned)ST_CONVERT_WAIT);
+      }
+      if (++get == S) {
+        get = 0;
+        get_phase ^= 1u;
+      }
       __syncwarp();
-      const uint32_t kb = ring + (t % S) * Cfg::kStage, vb = kb + 16 * Cfg::kRowBytes;
       issue(t + S - 1);  // into the stage that the warp finished reading one tile ago
-      settle();
 
       // ---- S^T = K Q^T: thread holds keys oct, oct + 8 of rows 2 * quad, 2 * quad + 1 of each block
       float s[NB][4];
@@ -365,8 +415,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
           const int ch = quad + 4 * i;
-          const uint4 r0 = lds16(kb + oct * Cfg::kRowBytes + (D == 128 ? ch ^ ((oct & 1) << 2) : ch) * 16);
-          const uint4 r1 = lds16(kb + (oct + 8) * Cfg::kRowBytes + (D == 128 ? ch ^ ((oct & 1) << 2) : ch) * 16);
+          const uint4 r0 = lds16(kb + rows_at<Cfg>(krow, ch)), r1 = lds16(kb + rows_at<Cfg>(krow + 8, ch));
           const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -383,7 +432,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         for (int ks = 0; ks < KS; ++ks) {
           uint32_t a[4];
           const int row = lane & 15, ch = 2 * ks + (lane >> 4);
-          ldsm_x4(kb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
+          ldsm_x4(kb + rows_at<Cfg>(row, ch), a);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
             if (nb < nb_used) Mma<Op>::run(s[nb], a, qf[nb][ks][0], qf[nb][ks][1]);
@@ -391,10 +440,11 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       }
 
       // ---- softmax
-      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16 + oct;
-      float kf[2] = {1.f, 1.f}, vf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};  // keys oct, oct + 8: 2^e of K, 2^e and e of V
+      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
+      const bool inner = key0 >= all_lo && key0 + 15 <= all_hi;
+      float kf[2] = {1.f, 1.f}, vf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};  // keys krow, krow + 8: 2^e of K, 2^e and e of V
       if constexpr (FP8) {
-        const uint32_t at = kb + 32 * Cfg::kRowBytes + oct;
+        const uint32_t at = sb + krow;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t bk, bv;
@@ -413,9 +463,11 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         bool more = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + (e >> 1) * 8;
-          const bool seen = key <= last_key[nb][e & 1] && key >= first_key[nb][e & 1];
-          x[e] = seen ? s[nb][e] * (row_f[nb][e & 1] * kf[e >> 1]) : -INFINITY;
+          x[e] = s[nb][e] * (row_f[nb][e & 1] * kf[e >> 1]);
+          if (!inner) {
+            const int key = key0 + krow + (e >> 1) * 8;
+            if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[e] = -INFINITY;
+          }
           more |= x[e] + ve[e >> 1] > m[nb][e & 1] + 8.f;
         }
         if (__any_sync(0xffffffffu, more)) {
@@ -449,16 +501,16 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
 
       // ---- O^T += V^T P^T
       if constexpr (FP8) {
-        constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (head_dim = 16 * oct + ..., or 8 * oct + ...)
+        constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (of head_dim: 16 * krow + ..., or 8 * oct + ...)
         uint32_t w[4][W];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 2 * quad + (r & 1) + (r >> 1) * 8;
+          const int row = ((r & 1) ? vrow1 : vrow0) + (r >> 1) * 8;
           if constexpr (D == 128) {
-            const uint4 v = lds16(vb + row * Cfg::kRowBytes + (oct ^ (row & 6)) * 16);
+            const uint4 v = lds16(vb + rows_at<Cfg>(row, krow));
             w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
           } else {
-            const uint2 v = lds8(vb + row * Cfg::kRowBytes + ((oct >> 1) ^ ((row >> 1) & 3)) * 16 + (oct & 1) * 8);
+            const uint2 v = lds8(vb + rows_at<Cfg>(row, oct >> 1) + (oct & 1) * 8);
             w[r][0] = v.x; w[r][1] = v.y;
           }
         }
@@ -480,7 +532,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         for (int mb = 0; mb < MB; ++mb) {
           uint32_t a[4];
           const int row = (lane & 7) + ((lane >> 4) << 3), ch = 2 * mb + ((lane >> 3) & 1);
-          ldsm_x4_t(vb + row * Cfg::kRowBytes + ((ch ^ (row & 7)) * 16), a);
+          ldsm_x4_t(vb + rows_at<Cfg>(row, ch), a);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
             if (nb < nb_used) Mma<Op>::run(o[nb][mb], a, pf[nb][0], pf[nb][1]);
@@ -489,8 +541,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       __syncwarp();          // every lane has read the stage before the next issue overwrites it
       locate(t + S);
     }
-    cp_async_wait<0>();
-
     // ---- the four warps' states become one
     __syncthreads();
     float* const mo = reinterpret_cast<float*>(smem);                      // [warp][row][kPad]
@@ -513,7 +563,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         float* const dst = mo + (warp * Cfg::kRows + row) * Cfg::kPad;
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const int d0 = FP8 ? (D / 8) * oct + 2 * mb : 16 * mb + oct, d1 = FP8 ? d0 + 1 : d0 + 8;
+          const int d0 = FP8 ? (D / 8) * krow + 2 * mb : 16 * mb + oct, d1 = FP8 ? d0 + 1 : d0 + 8;
           dst[d0] = o[nb][mb][e];
           dst[d1] = o[nb][mb][e + 2];
         }
@@ -549,7 +599,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       }
     }
     if (g.starts && !g.whole && tid == 0) p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows);
+    fence_async_shared();  // the next segment's TMA writes where the merge was
     __syncthreads();
+    gathered = false;
   }
 }
 

@@ -6,27 +6,27 @@
 namespace llg {
 
 template <typename T, bool FP8, int D, int NB>
-cudaError_t attn_rows_start(const AttnDev& p, int ctas, bool pdl, cudaStream_t s) {
+cudaError_t attn_rows_start(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool pdl, cudaStream_t s) {
   constexpr int smem = RowsCfg<T, FP8, D, NB>::kSmem;
   const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<T, FP8, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return launch_ex(attn_rows_kernel<T, FP8, D, NB>, dim3(ctas), dim3(kRowsThreads), smem, s, pdl, dim3(1, 1, 1), p);
+  return launch_ex(attn_rows_kernel<T, FP8, D, NB>, dim3(ctas), dim3(kRowsThreads), smem, s, pdl, dim3(1, 1, 1), p, k, v);
 }
 
 template <typename T, bool FP8, int D>
-cudaError_t attn_rows_blocks(const AttnDev& p, int blocks, int ctas, bool pdl, cudaStream_t s) {
+cudaError_t attn_rows_blocks(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, int blocks, int ctas, bool pdl, cudaStream_t s) {
   switch (blocks) {
-    case 1: return attn_rows_start<T, FP8, D, 1>(p, ctas, pdl, s);
-    case 2: return attn_rows_start<T, FP8, D, 2>(p, ctas, pdl, s);
-    default: return attn_rows_start<T, FP8, D, 4>(p, ctas, pdl, s);
+    case 1: return attn_rows_start<T, FP8, D, 1>(p, k, v, ctas, pdl, s);
+    case 2: return attn_rows_start<T, FP8, D, 2>(p, k, v, ctas, pdl, s);
+    default: return attn_rows_start<T, FP8, D, 4>(p, k, v, ctas, pdl, s);
   }
 }
 
 // blocks: 1, 2 or 4 blocks of eight rows per tile.
 template <typename T>
-cudaError_t attn_rows_dispatch(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s) {
-  if (p.c.head_dim == 128) return fp8 ? attn_rows_blocks<T, true, 128>(p, blocks, ctas, pdl, s) : attn_rows_blocks<T, false, 128>(p, blocks, ctas, pdl, s);
-  return fp8 ? attn_rows_blocks<T, true, 64>(p, blocks, ctas, pdl, s) : attn_rows_blocks<T, false, 64>(p, blocks, ctas, pdl, s);
+cudaError_t attn_rows_dispatch(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s) {
+  if (p.c.head_dim == 128) return fp8 ? attn_rows_blocks<T, true, 128>(p, k, v, blocks, ctas, pdl, s) : attn_rows_blocks<T, false, 128>(p, k, v, blocks, ctas, pdl, s);
+  return fp8 ? attn_rows_blocks<T, true, 64>(p, k, v, blocks, ctas, pdl, s) : attn_rows_blocks<T, false, 64>(p, k, v, blocks, ctas, pdl, s);
 }
 
 }  // namespace llg

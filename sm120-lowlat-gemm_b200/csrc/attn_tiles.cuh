@@ -122,14 +122,6 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// Box of a page: x = element, then slot, head, page.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int slot, int head, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(m), "r"(bar), "r"(x), "r"(slot), "r"(head), "r"(page)
-      : "memory");
-}
-
 // Ring of mbarrier phases: slot i of n, used round after round.
 struct Ring {
   int slot = 0;

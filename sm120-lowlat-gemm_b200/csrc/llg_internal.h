@@ -64,10 +64,10 @@ inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
 bool make_dense_map(CUtensorMap* m, const void* ptr, int64_t row_bytes, int64_t rows, int64_t ld_bytes, int box_bytes,
                     int box_rows, bool streamed);
 
-// Map over a paged cache tensor [pages, heads, slots, head_dim] (strides in bytes: page, head, slot): box = box_rows slots x
-// 64 16-bit elements with 128-byte swizzle, or x head_dim bytes without. False when the strides cannot be described.
+// Map over a paged cache tensor [pages, heads, slots, head_dim] (strides in bytes: page, head, slot): box = box_rows slots x at most
+// 128 bytes of a row, swizzled over the box's width (128 or 64 bytes) or not at all. False when the strides cannot be described.
 bool make_paged_map(CUtensorMap* m, const void* ptr, int head_dim, int elem_bytes, int slots, int heads, int pages, const int64_t stride[3],
-                    int box_rows);
+                    int box_rows, bool swizzle);
 
 // ---- skinny GEMV -------------------------------------------------------------------------------------------------
 struct SkinnyDev {
@@ -130,8 +130,8 @@ cudaError_t kv_append_launch(const llg_kv_append_args& a, unsigned* status, cuda
 cudaError_t kv_read_launch(const llg_kv_read_args& a, unsigned* status, cudaStream_t s);
 int64_t attn_workspace(const llg_attn_args& a);
 cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s);
-cudaError_t attn_rows_launch_bf16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
-cudaError_t attn_rows_launch_f16(const AttnDev& p, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_rows_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_rows_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_tiles_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
 // ctas: those of the kernel that left the partial results; tile_rows: rows of one of its tiles.

@@ -74,8 +74,9 @@ struct AttnDev {
   float scale_log2;       // softmax scale * log2(e); its magnitude in the tile kernel ...
   int negate;             // ... which turns the signs of q around for a negative scale
   int row_min, row_max;   // this launch serves sequences with row_min < new tokens * group <= row_max
+  int scale16;            // 16 scale bytes of a page from a multiple of 16 on lie together, 16-byte aligned
   int tok_tile;           // whole tokens per row tile
-  int box;                // tile kernel: rows of a TMA box (a divisor of 32 and of the page size), 0: no tensor maps
+  int box;                // rows of a TMA box (16, or a divisor of 32 and of the page size in the tile kernel), 0: no tensor maps
   float* part_o;          // [slots][rows per tile][head_dim]
   float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
   int4* split;            // [CTAs]: the item that starts, cut, at the end of a CTA's share: {CTAs, first token, kv head, rows};
