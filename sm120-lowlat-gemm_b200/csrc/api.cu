@@ -842,7 +842,9 @@ int llg_kv_read(const llg_kv_read_args* a, void* stream) {
 
 int64_t llg_paged_attention_ws(const llg_attn_args* a) {
   const int rc = check_attn(a);
-  return rc == LLG_OK ? attn_workspace(*a) : rc;
+  if (rc != LLG_OK) return rc;
+  const int64_t need = attn_workspace(*a);
+  return need >= 0 ? need : fail(LLG_E_INVALID, "paged_attention: too many key tiles in one call");
 }
 
 int llg_paged_attention(const llg_attn_args* a, void* stream) {
@@ -851,6 +853,7 @@ int llg_paged_attention(const llg_attn_args* a, void* stream) {
   if (a->kv.batch == 0 || a->kv.tokens == 0) return LLG_OK;
   if (!a->q || !a->out) return fail(LLG_E_INVALID, "paged_attention: q and out must be device pointers");
   const int64_t need = attn_workspace(*a);
+  if (need < 0) return fail(LLG_E_INVALID, "paged_attention: too many key tiles in one call");
   if (a->ws_bytes < need || !a->ws || !aligned(a->ws, 16))
     return fail(LLG_E_INVALID, "paged_attention: needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)need, (long long)a->ws_bytes);
   unsigned* st = status_word_device_ptr();

@@ -12,11 +12,13 @@ constexpr int kTileRows = 256;
 
 struct Part {  // one kernel's CTAs and scratch
   int ctas, rows, tok_tile;
-  int64_t split, part_ml, part_o;  // offsets
+  int row_max;     // query rows per kv head of the sequences it serves
+  int64_t split, first, part_ml, part_o;  // offsets
 };
 struct Plan {
   bool few, many;
   Part f, m;
+  int64_t units;  // no more key tiles than this
   int64_t bytes;
 };
 
@@ -26,7 +28,8 @@ void lay_out(Part* q, int64_t units, int ctas, int rows, int head_dim, int64_t* 
   q->ctas = (int)(units < ctas ? units : ctas);
   q->rows = rows;
   q->split = *at;
-  q->part_ml = q->split + pad((int64_t)q->ctas * 16);
+  q->first = q->split + pad((int64_t)q->ctas * 32);
+  q->part_ml = q->first + pad((int64_t)q->ctas * 4);
   q->part_o = q->part_ml + pad((int64_t)q->ctas * 2 * rows * 8);
   *at = q->part_o + pad((int64_t)q->ctas * 2 * rows * head_dim * 4);
 }
@@ -39,20 +42,25 @@ Plan plan_of(const llg_attn_args& a) {
   const int group = a.heads / c.kv_heads, sms = sm_count();
   const int64_t most = c.q_starts ? (int64_t)c.tokens * group : (int64_t)(c.tokens / c.batch) * group;
   const int64_t keys = (int64_t)c.table_width * c.page_size;
-  p.few = c.q_starts || most <= kRowsMax;
-  p.many = most > kRowsMax;
+  // With offsets the few-row kernel takes the sequences of one token (of a few, where the group is small), in tiles no wider than
+  // that: wider ones would hold registers that decoding sequences do not use. Without, tiles as wide as the rows.
+  const int64_t widest = c.q_starts ? (group <= 8 ? 8 : group <= 16 ? 16 : 32) : kRowsMax;
+  p.few = c.q_starts || most <= widest;
+  p.many = most > widest;
   if (p.few) {
-    const int64_t rows = most < kRowsMax ? most : kRowsMax;
+    const int64_t rows = most < widest ? most : widest;
     const int blocks = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.f.row_max = (int)widest;
     p.f.tok_tile = blocks * 8 / group;
-    const int64_t tiles = (c.tokens + p.f.tok_tile - 1) / p.f.tok_tile + c.batch;
-    lay_out(&p.f, tiles * c.kv_heads * ((keys + 63) / 64 + 1),
-            rows_ctas_per_sm(c.dtype == LLG_DT_E4M3, c.head_dim, blocks) * sms, blocks * 8, c.head_dim, &p.bytes);
+    p.units = (int64_t)c.batch * c.kv_heads * ((keys + 63) / 64 + 1);  // one tile per sequence
+    lay_out(&p.f, p.units, rows_ctas_per_sm(c.dtype == LLG_DT_E4M3, c.head_dim, blocks) * sms, blocks * 8, c.head_dim, &p.bytes);
   }
   if (p.many) {
     p.m.tok_tile = kTileRows / group;
     const int64_t tiles = (c.tokens + p.m.tok_tile - 1) / p.m.tok_tile + c.batch;
-    lay_out(&p.m, tiles * c.kv_heads * ((keys + 127) / 128 + 1), sms, kTileRows, c.head_dim, &p.bytes);
+    const int64_t units = tiles * c.kv_heads * ((keys + 127) / 128 + 1);
+    if (units > p.units) p.units = units;
+    lay_out(&p.m, units, sms, kTileRows, c.head_dim, &p.bytes);
   }
   return p;
 }
@@ -61,7 +69,8 @@ Plan plan_of(const llg_attn_args& a) {
 
 int64_t attn_workspace(const llg_attn_args& a) {
   if (a.kv.batch == 0 || a.kv.tokens == 0) return 0;
-  return plan_of(a).bytes;
+  const Plan p = plan_of(a);
+  return p.units < INT32_MAX / 2 ? p.bytes : -1;  // the kernels count key tiles in 32 bits
 }
 
 cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s) {
@@ -83,6 +92,7 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
   auto use = [&](const Part& q) {
     p.tok_tile = q.tok_tile;
     p.split = reinterpret_cast<int4*>(ws + q.split);
+    p.first = reinterpret_cast<int*>(ws + q.first);
     p.part_ml = reinterpret_cast<float*>(ws + q.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + q.part_o);
   };
@@ -95,7 +105,7 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
   };
   if (plan.many) {
     use(plan.m);
-    p.row_min = plan.few ? kRowsMax : 0;
+    p.row_min = plan.few ? plan.f.row_max : 0;
     p.row_max = INT32_MAX;
     // the tile kernel takes the maximum of unscaled scores: a positive scale (1e-30 for 0), the sign goes to q
     p.negate = scale_log2 < 0.f;
@@ -113,7 +123,7 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
   if (plan.few) {
     use(plan.f);
     p.row_min = 0;
-    p.row_max = kRowsMax;
+    p.row_max = plan.f.row_max;
     p.negate = 0;
     p.scale_log2 = scale_log2;
     p.box = p.c.page_size % 16 == 0 && maps(16, true) ? 16 : 0;  // a warp's 16 keys

@@ -1,6 +1,7 @@
 // Adds the partial results of items that several CTAs shared: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the order
-// of the CTAs. Bound by the latency of reading a few kilobytes back from L2; a row's parts are spread over the warps of a CTA
-// (a long sequence of few heads leaves one part per SM) and every warp keeps four of its parts in flight.
+// of the CTAs. Bound by the latency of reading a few kilobytes back from L2. The CTAs of the main kernel that shared an item are
+// also the indexes of those that add it up here, each its part of the rows: a long sequence of few heads, with a part from every
+// SM, so has all SMs at work, two parts have two. A CTA with fewer rows than warps puts several warps on a row.
 #include "paged_kv.cuh"
 
 namespace llg {
@@ -23,106 +24,133 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 
 constexpr int kWarps = 8;
 
-// blockIdx.x: the main kernel's CTA whose share ends inside an item. SPREAD warps work on one row, blockIdx.y counts groups of
-// kWarps / SPREAD rows.
-template <typename T, int D, int SPREAD>
+// Running sum of one row's parts, as one warp holds it: V values of head_dim per lane.
+template <int V>
+struct RowSum {
+  float top = -INFINITY, sum = 0.f, acc[V] = {};
+};
+
+// Parts share, share + spread, ... of the row: 32 of them at a time, one per lane, then one after the other.
+template <int V>
+__device__ __forceinline__ void add_parts(const AttnDev& p, RowSum<V>& s, int parts, int twice, int first, int tile_rows, int row, int share,
+                                          int spread, int lane) {
+  for (int i0 = share; i0 < parts; i0 += 32 * spread) {
+    const int i = i0 + lane * spread;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    int64_t at = 0;
+    if (i < parts) {
+      const int cta = i >> twice;
+      at = (int64_t)part_slot(first + cta, cta == 0) * tile_rows + row + (twice & i ? 128 : 0);
+      ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+    }
+    // the first sums are requested before their weights are known
+    const int n = min(32, (parts - i0 + spread - 1) / spread);
+    float x[4][V];
+    auto get = [&](int j, float (&v)[V]) {
+      const int64_t a = __shfl_sync(0xffffffffu, at, j);
+      const float* const src = p.part_o + a * (32 * V) + lane * V;
+      if constexpr (V == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) get(j, x[j]);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float now = fmaxf(s.top, mx);
+    const float keep = s.top == -INFINITY ? 0.f : exp2f(s.top - now);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - now);
+    s.top = now;
+    s.sum = s.sum * keep + w * ml.y;  // this lane's parts only
+#pragma unroll
+    for (int v = 0; v < V; ++v) s.acc[v] *= keep;
+    for (int j0 = 0; j0 < n; j0 += 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = __shfl_sync(0xffffffffu, w, j0 + j);
+        if (j0 + j < n && f != 0.f) {  // a part without keys has no sums
+#pragma unroll
+          for (int v = 0; v < V; ++v) s.acc[v] += f * x[j][v];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j0 + 4 + j < n) get(j0 + 4 + j, x[j]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, o);
+}
+
+template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_constant__ AttnDev p, int tile_rows) {
-  constexpr int V = D / 32;  // values per lane
+  constexpr int V = D / 32;
   __shared__ float part[kWarps][D + 2];
   pdl_trigger();
   pdl_wait();
-  int4 item = p.split[blockIdx.x];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.y & 1;  // which of the main CTA's two items
+  const int4 item = p.split[2 * blockIdx.x + e];
+  const int went_on = p.first[blockIdx.x];  // only looked at when an item went on
   if (item.x == 0) return;
-  const int twice = item.w >> 16;  // two parts per CTA
-  item.w &= 0xffff;
-  item.x <<= twice;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SPREAD;
-  const int row = blockIdx.y * (kWarps / SPREAD) + warp / SPREAD;
-  const bool live = row < item.w;
-  float top = -INFINITY, sum = 0.f, acc[V] = {};
-  if (live) {
-    // parts share, share + SPREAD, ...: 32 of them at a time, one per lane
-    for (int i0 = share; i0 < item.x; i0 += 32 * SPREAD) {
-      const int i = i0 + lane * SPREAD;
-      float2 ml = make_float2(-INFINITY, 0.f);
-      int64_t at = 0;
-      if (i < item.x) {
-        const int cta = i >> twice;
-        at = (int64_t)part_slot(blockIdx.x + cta, cta == 0) * tile_rows + row + (twice & i ? 128 : 0);
-        ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      }
-      float mx = ml.x;
+  {
+    const int twice = item.w >> 16, rows = item.w & 0xffff;
+    const int first = e == 0 ? went_on : blockIdx.x;
+    // this CTA's rows: worker, worker + workers, ...
+    const int each = gridDim.y >> 1, workers = item.x * each, worker = (blockIdx.x - first) * each + (blockIdx.y >> 1);
+    const int mine = worker < rows ? (rows - worker + workers - 1) / workers : 0;
+    const int spread = mine >= kWarps ? 1 : mine >= 4 ? 2 : mine >= 2 ? 4 : kWarps;  // warps per row
+    const int share = warp % spread;
+    for (int r0 = 0; r0 < mine; r0 += kWarps / spread) {
+      const int index = r0 + warp / spread;
+      const bool live = index < mine;
+      const int row = worker + index * workers;
+      RowSum<V> s;
+      if (live) add_parts<V>(p, s, item.x << twice, twice, first, tile_rows, row, share, spread, lane);
+      if (spread > 1) {
+        __syncthreads();
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float now = fmaxf(top, mx);
-      const float keep = top == -INFINITY ? 0.f : exp2f(top - now);
-      const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - now);
-      top = now;
-      sum = sum * keep + w * ml.y;  // this lane's parts only
+        for (int v = 0; v < V; ++v) part[warp][lane * V + v] = s.acc[v];
+        if (lane == 0) {
+          part[warp][D] = s.top;
+          part[warp][D + 1] = s.sum;
+        }
+        __syncthreads();
+        float all = -INFINITY;
+        for (int q = 0; q < spread; ++q) all = fmaxf(all, part[warp - share + q][D]);
+        s.top = all == -INFINITY ? 0.f : all;
+        s.sum = 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] *= keep;
-      const int n = min(32, (item.x - i0 + SPREAD - 1) / SPREAD);
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const float f = __shfl_sync(0xffffffffu, w, j);
-        const int64_t a = __shfl_sync(0xffffffffu, at, j);
-        if (f == 0.f) continue;  // a part without keys has no sums
-        const float* const src = p.part_o + a * D + lane * V;
-        if constexpr (V == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          acc[0] += f * x.x; acc[1] += f * x.y;
+        for (int v = 0; v < V; ++v) s.acc[v] = 0.f;
+        for (int q = 0; q < spread; ++q) {
+          const float* const from = part[warp - share + q];
+          const float f = exp2f(from[D] - s.top);
+          s.sum += f * from[D + 1];
+#pragma unroll
+          for (int v = 0; v < V; ++v) s.acc[v] += f * from[lane * V + v];
         }
       }
+      if (!live || share != 0) continue;
+      const float inv = s.sum > 0.f || s.sum != s.sum ? 1.f / s.sum : 0.f;
+      const int tok = row / p.group, head = item.z * p.group + row - tok * p.group;
+      const int64_t t = item.y + tok;
+      unsigned char* const dst = p.out + t * p.o_tok + head * p.o_head + 2 * V * lane;
+      if constexpr (V == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(s.acc[0] * inv, s.acc[1] * inv), pack2<T>(s.acc[2] * inv, s.acc[3] * inv));
+      else
+        *reinterpret_cast<uint32_t*>(dst) = pack2<T>(s.acc[0] * inv, s.acc[1] * inv);
+      if (p.lse && lane == 0)
+        p.lse[t * p.lse_tok + head] = s.sum > 0.f || s.sum != s.sum ? (s.top + log2f(s.sum)) * 0.693147180559945309f : -INFINITY;
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if constexpr (SPREAD > 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) part[warp][lane * V + v] = acc[v];
-    if (lane == 0) {
-      part[warp][D] = top;
-      part[warp][D + 1] = sum;
-    }
-    __syncthreads();
-    if (share != 0 || !live) return;
-    float all = top;
-#pragma unroll
-    for (int s = 1; s < SPREAD; ++s) all = fmaxf(all, part[warp + s][D]);
-    const float base = all == -INFINITY ? 0.f : all;
-    sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.f;
-#pragma unroll
-    for (int s = 0; s < SPREAD; ++s) {
-      const float f = exp2f(part[warp + s][D] - base);
-      sum += f * part[warp + s][D + 1];
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] += f * part[warp + s][lane * V + v];
-    }
-    top = base;
-  }
-  if (!live) return;
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  const int tok = row / p.group, head = item.z * p.group + row - tok * p.group;
-  const int64_t t = item.y + tok;
-  unsigned char* const dst = p.out + t * p.o_tok + head * p.o_head + 2 * V * lane;
-  if constexpr (V == 4)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack2<T>(acc[0] * inv, acc[1] * inv);
-  if (p.lse && lane == 0) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.693147180559945309f : -INFINITY;
 }
 
 template <typename T, int D>
 cudaError_t combine(const AttnDev& p, int ctas, int tile_rows, cudaStream_t s) {
-  const dim3 block(32 * kWarps), one(1, 1, 1);
-  // Few rows per item come with many parts (a long cache), many rows with two or three: one row per CTA or one per warp.
-  if (tile_rows <= 32) return launch_ex(attn_combine_kernel<T, D, kWarps>, dim3(ctas, tile_rows), block, 0, s, true, one, p, tile_rows);
-  return launch_ex(attn_combine_kernel<T, D, 1>, dim3(ctas, tile_rows / kWarps), block, 0, s, true, one, p, tile_rows);
+  // one CTA for each of the two items a CTA of the main kernel may share with others; of 256 rows, eight CTAs each, which makes
+  // two rows per warp of an item with two parts
+  return launch_ex(attn_combine_kernel<T, D>, dim3(ctas, tile_rows > 32 ? 16 : 2), dim3(32 * kWarps), 0, s, true, dim3(1, 1, 1), p, tile_rows);
 }
 
 }  // namespace

@@ -175,9 +175,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;
   constexpr int S = Cfg::kStages, CH = Cfg::kChunks, KS = D / 16, MB = D / 16;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ long long scratch[kRowsWarps + 4];
+  __shared__ int scratch[kRowsWarps + 2];
   __shared__ __align__(8) unsigned long long bars[kRowsWarps * S];
-  __shared__ unsigned char scales[FP8 ? kRowsWarps * S * 32 : 1];
+  __shared__ __align__(16) unsigned char scales[FP8 ? kRowsWarps * S * 32 : 1];
   __shared__ volatile uint32_t abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int quad = lane & 3, oct = lane >> 2;  // fragment coordinates
@@ -190,10 +190,14 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
     mbar_init(smem_u32(&bars[tid]), 32);
     mbar_fence_init();
   }
-  if (tid == 0) abort_word = 0u;
+  if (tid == 0) {
+    abort_word = 0u;
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
   pdl_trigger();
   pdl_wait();
-  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (tid == 0) clear_splits(p);
   Share share = find_share<kRowsKT, kRowsThreads>(p, scratch);
   const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing, bar = smem_u32(&bars[warp * S]);
   const uint32_t scale_at = smem_u32(scales) + warp * S * 32;
@@ -209,74 +213,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
     const int rows = g.toks * p.group;
     const int nb_used = (rows + 7) >> 3;
     const int pos0 = g.s.len - g.s.n + g.tok0;  // position of the tile's first token
-
-    // ---- queries: B fragments of K Q^T, row oct of each block
-    uint32_t qf[NB][KS][2];
-    float row_f[NB][2];                     // what turns a product of those rows into log2 units
-    int first_key[NB][2], last_key[NB][2];  // keys that rows 2 * quad, 2 * quad + 1 of a block see: [first, last]
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int row = nb * 8 + oct;
-      const bool ok = row < rows;
-      const int tok = row / p.group, hh = row - tok * p.group;
-      const unsigned char* src = p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        uint2 v = make_uint2(0u, 0u);
-        if (ok) {
-          if constexpr (FP8) {  // the order in which a thread holds a row of K: 16 * (quad + 4 i) + 4 j
-            const int i = ks >> 2, j = ks & 3;
-            v = *reinterpret_cast<const uint2*>(src + 2 * (16 * (quad + 4 * i) + 4 * j));
-          } else {
-            v.x = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad));
-            v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
-          }
-        }
-        qf[nb][ks][0] = v.x;
-        qf[nb][ks][1] = v.y;
-      }
-      float mine = p.scale_log2;              // of row oct
-      if constexpr (kToF16) {
-        float top = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
-        const float up = __uint_as_float((268u - e) << 23);  // 2^(14 - exponent of the row's largest value)
-        mine *= __uint_as_float((e - 14u) << 23);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
-            qf[nb][ks][h] = Mma<__half>::pack(f.x * up, f.y * up);
-          }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        row_f[nb][e] = __shfl_sync(0xffffffffu, mine, (2 * quad + e) * 4);
-        const int r = nb * 8 + 2 * quad + e;
-        const int pos = pos0 + r / p.group;
-        last_key[nb][e] = r < rows ? (p.causal ? min(pos, g.s.len - 1) : g.s.len - 1) : -1;
-        first_key[nb][e] = p.window > 0 ? pos - p.window + 1 : 0;
-      }
-    }
-
-    float o[NB][MB][4];
-    float m[NB][2], l[NB][2];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) o[nb][mb][0] = o[nb][mb][1] = o[nb][mb][2] = o[nb][mb][3] = 0.f;
-      m[nb][0] = m[nb][1] = -INFINITY;
-      l[nb][0] = l[nb][1] = 0.f;
-    }
 
     // ---- the warp's ring: tile t holds keys [64 t + 16 warp, + 16) of the segment
     const int nt = g.tile1 - g.tile0;
@@ -393,6 +329,74 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       issue(t);
     }
     locate(S - 1);
+
+    // ---- queries: B fragments of K Q^T, row oct of each block
+    uint32_t qf[NB][KS][2];
+    float row_f[NB][2];                     // what turns a product of those rows into log2 units
+    int first_key[NB][2], last_key[NB][2];  // keys that rows 2 * quad, 2 * quad + 1 of a block see: [first, last]
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = nb * 8 + oct;
+      const bool ok = row < rows;
+      const int tok = row / p.group, hh = row - tok * p.group;
+      const unsigned char* src = p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint2 v = make_uint2(0u, 0u);
+        if (ok) {
+          if constexpr (FP8) {  // the order in which a thread holds a row of K: 16 * (quad + 4 i) + 4 j
+            const int i = ks >> 2, j = ks & 3;
+            v = *reinterpret_cast<const uint2*>(src + 2 * (16 * (quad + 4 * i) + 4 * j));
+          } else {
+            v.x = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad));
+            v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
+          }
+        }
+        qf[nb][ks][0] = v.x;
+        qf[nb][ks][1] = v.y;
+      }
+      float mine = p.scale_log2;              // of row oct
+      if constexpr (kToF16) {
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
+        const float up = __uint_as_float((268u - e) << 23);  // 2^(14 - exponent of the row's largest value)
+        mine *= __uint_as_float((e - 14u) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&qf[nb][ks][h]));
+            qf[nb][ks][h] = Mma<__half>::pack(f.x * up, f.y * up);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        row_f[nb][e] = __shfl_sync(0xffffffffu, mine, (2 * quad + e) * 4);
+        const int r = nb * 8 + 2 * quad + e;
+        const int pos = pos0 + r / p.group;
+        last_key[nb][e] = r < rows ? (p.causal ? min(pos, g.s.len - 1) : g.s.len - 1) : -1;
+        first_key[nb][e] = p.window > 0 ? pos - p.window + 1 : 0;
+      }
+    }
+
+    float o[NB][MB][4];
+    float m[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[nb][mb][0] = o[nb][mb][1] = o[nb][mb][2] = o[nb][mb][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+    }
 
     for (int t = 0; t < nt; ++t) {
       const uint32_t kb = ring + get * Cfg::kStage, vb = kb + 16 * Cfg::kRowBytes, sb = scale_at + get * 32;
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * Cfg::kRows + row) * 2) = make_float2(top, sum);
       }
     }
-    if (g.starts && !g.whole && tid == 0) p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows);
+    if (!g.whole && tid == 0) note_split(p, g, rows);
     fence_async_shared();  // the next segment's TMA writes where the merge was
     __syncthreads();
     gathered = false;

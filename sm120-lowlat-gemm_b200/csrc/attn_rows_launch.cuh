@@ -8,7 +8,8 @@ namespace llg {
 template <typename T, bool FP8, int D, int NB>
 cudaError_t attn_rows_start(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool pdl, cudaStream_t s) {
   constexpr int smem = RowsCfg<T, FP8, D, NB>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<T, FP8, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, FP8, D, NB>), smem, done);
   if (e != cudaSuccess) return e;
   return launch_ex(attn_rows_kernel<T, FP8, D, NB>, dim3(ctas), dim3(kRowsThreads), smem, s, pdl, dim3(1, 1, 1), p, k, v);
 }

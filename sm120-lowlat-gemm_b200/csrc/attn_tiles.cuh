@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   using Cfg = TilesCfg<T, FP8, D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ long long scratch[kTilesThreads / 32 + 4];
+  __shared__ int scratch[kTilesThreads / 32 + 2];
   __shared__ uint32_t tmem_holder;
   __shared__ Segment segments[kSegRing];
   __shared__ volatile uint32_t abort_word, drain_word;
@@ -180,13 +180,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     }
     mbar_fence_init();
   }
+  if (tid == 32) {
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
   if (warp == 12) {
     tmem_alloc(smem_u32(&tmem_holder), 512);
     tmem_relinquish();
   }
   pdl_trigger();
   pdl_wait();
-  if (tid == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (tid == 0) clear_splits(p);
   tc_fence_before();
   Share share = find_share<kTilesKT, kTilesThreads>(p, scratch);  // synchronises the CTA
   __syncthreads();
@@ -378,18 +382,26 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int rows = g.toks * p.group;
       const int64_t first = g.s.t0 + g.tok0;
       constexpr int CH = D / 8;
-      const uint32_t flip = p.negate ? 0x80008000u : 0u;
+      // 32 (16) copies of 16 bytes per thread, all in flight at once; two rows' worth of index arithmetic per thread and step
 #pragma unroll 4
       for (int i = lt; i < kTilesRows * CH; i += 128) {
         const int row = i / CH, ch = i % CH;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) {
-          const int tok = row / p.group, hh = row - tok * p.group;
-          v = *reinterpret_cast<const uint4*>(p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16);
-          v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        const int tok = row / p.group, hh = row - tok * p.group;
+        const bool there = row < rows;
+        const unsigned char* const src = p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16;
+        cp_async16(base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4),
+                   there ? src : p.q, there ? 16u : 0u);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      if (p.negate) {  // a negative softmax scale: its sign goes to q, each thread turning what it copied
+        for (int i = lt; i < kTilesRows * CH; i += 128) {
+          const int row = i / CH, ch = i % CH;
+          const uint32_t at = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
+          const uint4 v = lds16(at);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ 0x80008000u), "r"(v.y ^ 0x80008000u),
+                       "r"(v.z ^ 0x80008000u), "r"(v.w ^ 0x80008000u) : "memory");
         }
-        const uint32_t dst = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
       }
       fence_async_shared();
       mbar_arrive(bar(BAR_Q_FULL));
@@ -410,11 +422,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           const Row row = next;
           next = locate(j + 1);
           copy16(row, false);
-          if (j == tile0) load_q(*seg);
+          if (keys && j == tile0 + 1) load_q(*seg);
           if (!keys) copy16(row, true);
           else if (j > tile0) copy16(held, true);
+          if (!keys && j == tile0) load_q(*seg);  // behind two tiles that travel meanwhile
           held = row;
         }
+        if (keys && tile1 - tile0 == 1) load_q(*seg);
         if (keys) copy16(held, true);
       } else {
         // the same sequence, every tile fetched three places ahead of its widening
@@ -433,9 +447,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           }
         };
         fetch(0);
-        load_q(*seg);
         fetch(1);
         if (n > 2) fetch(2);
+        load_q(*seg);
         for (int i = 0; i < n && ok; ++i) {
           widen();
           if (i + 3 < n) fetch(i + 3);
@@ -707,8 +721,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (!g.whole) *reinterpret_cast<float2*>(p.part_ml + slot_row * 2) = make_float2(done > 0 ? m : -INFINITY, sum);
         else if (p.lse) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (m + log2f(sum)) * 0.693147180559945309f : -INFINITY;
       }
-      if (tid == 0 && g.starts && !g.whole)
-        p.split[blockIdx.x] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows | (mode == MODE_KEYS ? 1 << 16 : 0));
+      if (tid == 0 && !g.whole) note_split(p, g, rows | (mode == MODE_KEYS ? 1 << 16 : 0));
       done_item();
     }
   }

@@ -8,7 +8,8 @@ namespace llg {
 template <typename T, bool FP8, int D>
 cudaError_t attn_tiles_start(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool pdl, cudaStream_t s) {
   constexpr int smem = TilesCfg<T, FP8, D>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<T, FP8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(attn_tiles_kernel<T, FP8, D>), smem, done);
   if (e != cudaSuccess) return e;
   return launch_ex(attn_tiles_kernel<T, FP8, D>, dim3(ctas), dim3(kTilesThreads), smem, s, pdl, dim3(1, 1, 1), p, k, v);
 }

@@ -79,8 +79,10 @@ struct AttnDev {
   int box;                // rows of a TMA box (16, or a divisor of 32 and of the page size in the tile kernel), 0: no tensor maps
   float* part_o;          // [slots][rows per tile][head_dim]
   float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
-  int4* split;            // [CTAs]: the item that starts, cut, at the end of a CTA's share: {CTAs, first token, kv head, rows};
-                          // 1 << 16 in the last: every CTA left two parts, the second 128 rows behind the first
+  int4* split;            // [CTAs][2]: the cut item that goes on at the beginning of a CTA's share, and the one that starts at its
+                          // end: {CTAs that share it (0: none), first token, kv head, rows}; 1 << 16 in the last: every CTA left
+                          // two parts, the second 128 rows behind the first
+  int* first;             // [CTAs]: the CTA in which the item that goes on started
 };
 
 // CTAs of the few-row kernel that fit an SM: four where a tile's key rows and accumulators are small (e4m3 rows, or head_dim 64,
@@ -110,10 +112,11 @@ __device__ __forceinline__ int token_tiles(const AttnDev& p, const SeqView& s) {
   return rows > p.row_min && rows <= p.row_max ? (s.n + p.tok_tile - 1) / p.tok_tile : 0;
 }
 
-// Key tiles of one kv head of a sequence, over all of its token tiles.
+// Key tiles of one kv head of a sequence, over all of its token tiles. (The host refuses calls whose key tiles might not fit 31
+// bits: 64-bit divisions in every CTA's start cost a microsecond.)
 template <int KT>
-__device__ __forceinline__ long long seq_units(const AttnDev& p, const SeqView& s) {
-  long long u = 0;
+__device__ __forceinline__ int seq_units(const AttnDev& p, const SeqView& s) {
+  int u = 0;
   const int nt = token_tiles(p, s);
   for (int r = 0; r < nt; ++r) {
     const int tf = r * p.tok_tile;
@@ -124,73 +127,88 @@ __device__ __forceinline__ long long seq_units(const AttnDev& p, const SeqView& 
 
 // A CTA's share of the key tiles and its place in the walk.
 struct Share {
-  long long u, end, per;  // next unit, end of the share, units per CTA
-  int seq;
-  long long off;          // units of `seq` (over all kv heads) before u
-  int known;              // sequence whose units of one kv head `per_head` holds
-  long long per_head;
+  int u, end, per;  // next unit, end of the share, units per CTA
+  int seq, off;     // units of `seq` (over all kv heads) before u
+  int known;        // sequence whose units of one kv head `per_head` holds
+  int per_head;
 };
 
-// Every thread of the CTA takes part. scratch: NT / 32 + 4 long longs of shared memory.
+// Every thread of the CTA takes part. scratch: NT / 32 + 2 ints of shared memory.
 template <int KT, int NT>
-__device__ __forceinline__ Share find_share(const AttnDev& p, long long* scratch) {
+__device__ __forceinline__ Share find_share(const AttnDev& p, int* scratch) {
+  constexpr int W = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long* part = scratch;             // NT / 32 warp sums
-  long long* found = scratch + NT / 32;  // {seq, units before the sequence}
-  long long mine = 0, first = 0;
+  int* const part = scratch;       // warp sums
+  int* const found = scratch + W;  // {seq, units before u}
+  // one prefix sum over the first NT sequences, and the total of all
+  int x = 0, rest = 0;
   for (int i = tid; i < p.c.batch; i += NT) {
-    const long long u = seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
-    if (i == tid) first = u;
-    mine += u;
+    const int u = seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
+    if (i == tid) x = u;
+    else rest += u;
   }
+  int inc = x;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) part[warp] = mine;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  long long total = 0;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) part[warp] = inc;
+  const int beyond = p.c.batch > NT ? __syncthreads_or(rest != 0) : (__syncthreads(), 0);
+  int before = 0, chunk = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) total += part[w];
-  __syncthreads();
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) before += part[w];
+    chunk += part[w];
+  }
+  int total = chunk;
+  if (beyond) {  // more sequences than threads
+    __syncthreads();
+    if (tid == 0) found[0] = 0;
+    __syncthreads();
+    atomicAdd(&found[0], rest);
+    __syncthreads();
+    total += found[0];
+  }
   Share sh;
-  sh.per = (total + gridDim.x - 1) / gridDim.x;
-  sh.u = sh.per * blockIdx.x;
+  sh.per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+  sh.u = sh.per * (int)blockIdx.x;
   sh.end = min(total, sh.u + sh.per);
-  sh.seq = 0;
-  sh.off = 0;
   sh.known = -1;
-  sh.per_head = 0;
+  sh.per_head = sh.seq = sh.off = 0;
   if (sh.u >= sh.end) return sh;
-  long long base = 0;
-  for (int c0 = 0; c0 < p.c.batch; c0 += NT) {
-    const int i = c0 + tid;
-    const long long x = i >= p.c.batch ? 0 : c0 == 0 ? first : seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
-    long long inc = x;
+  __syncthreads();
+  int base = 0;
+  for (int c0 = 0;; c0 += NT) {
+    const int lo = base + before + inc - x;
+    if (x > 0 && lo <= sh.u && sh.u < lo + x) {
+      found[0] = c0 + tid;
+      found[1] = sh.u - lo;
+    }
+    if (sh.u < base + chunk || c0 + NT >= p.c.batch) break;
+    // not among these: the next NT sequences
+    base += chunk;
+    const int i = c0 + NT + tid;
+    x = i < p.c.batch ? seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads : 0;
+    inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
+    __syncthreads();
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    long long before = base, chunk = 0;
+    before = chunk = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (w < warp) before += part[w];
       chunk += part[w];
     }
-    const long long lo = before + inc - x;
-    if (x > 0 && lo <= sh.u && sh.u < lo + x) {
-      found[0] = i;
-      found[1] = sh.u - lo;
-    }
-    __syncthreads();
-    if (found[0] >= 0) break;
-    base += chunk;
   }
-  sh.seq = (int)found[0];
-  sh.off = found[1];
   __syncthreads();
+  sh.seq = found[0];
+  sh.off = found[1];
   return sh;
 }
 
@@ -201,13 +219,13 @@ struct Segment {
   KeyRange keys;
   int tile0, tile1;            // key tiles, counted from key 0
   bool starts, whole;          // the segment begins its item / is all of it
-  int parts;                   // CTAs that share the item, when this segment begins it
+  int first, parts;            // the item's first CTA, and how many share it
 };
 
 template <int KT>
 __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segment& g) {
   if (sh.u >= sh.end) return false;
-  long long per_head;
+  int per_head;
   for (;;) {
     if (sh.seq >= p.c.batch) return false;
     g.s = seq_view(p.c, sh.seq);
@@ -221,8 +239,8 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
     sh.off = 0;
   }
   g.seq = sh.seq;
-  g.head = (int)(sh.off / per_head);
-  long long rem = sh.off - g.head * per_head;
+  g.head = sh.off / per_head;
+  int rem = sh.off - g.head * per_head;
   int units;
   for (int r = 0;; ++r) {
     g.tok0 = r * p.tok_tile;
@@ -232,13 +250,16 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
     if (rem < units) break;
     rem -= units;
   }
-  const long long left = sh.end - sh.u;
-  const int take = (int)min((long long)units - rem, left);
-  g.tile0 = g.keys.lo / KT + (int)rem;
+  const int take = min(units - rem, sh.end - sh.u);
+  g.tile0 = g.keys.lo / KT + rem;
   g.tile1 = g.tile0 + take;
   g.starts = rem == 0;
   g.whole = g.starts && take == units;
-  g.parts = g.starts ? (int)((sh.u + units - 1) / sh.per - blockIdx.x) + 1 : 0;
+  g.first = g.parts = 0;
+  if (!g.whole) {
+    g.first = (sh.u - rem) / sh.per;
+    g.parts = (sh.u - rem + units - 1) / sh.per - g.first + 1;
+  }
   sh.u += take;
   sh.off += take;
   if (sh.off == per_head * p.c.kv_heads) {
@@ -246,6 +267,15 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
     sh.off = 0;
   }
   return true;
+}
+
+// Notes a cut item for the kernel that adds its parts up. One thread.
+__device__ __forceinline__ void note_split(const AttnDev& p, const Segment& g, int rows) {
+  p.split[2 * blockIdx.x + (g.starts ? 1 : 0)] = make_int4(g.parts, g.s.t0 + g.tok0, g.head, rows);
+  if (!g.starts) p.first[blockIdx.x] = g.first;
+}
+__device__ __forceinline__ void clear_splits(const AttnDev& p) {
+  p.split[2 * blockIdx.x] = p.split[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
 }
 
 // A cut item's part of this CTA: slot 1 when the CTA begins the item (at the end of its share), else slot 0.

@@ -29,6 +29,11 @@ import torch
 
 from . import _ops  # noqa: F401  (registers torch.ops.lowlat_gemm)
 
+# resolved once: a call through the packet looks its overload up every time
+_append = torch.ops.lowlat_gemm.kv_append.default
+_read = torch.ops.lowlat_gemm.kv_read.default
+_attention = torch.ops.lowlat_gemm.paged_attention.default
+
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
               kv_lens: torch.Tensor, *, q_starts: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
@@ -40,7 +45,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     and its scale as 2**e. A power of two costs e4m3 no accuracy and makes value * scale exact in bf16 and fp32.
     head_dim: a multiple of 16 up to 256. The slots one call writes must be distinct: sequences may share the pages of a
     common prefix, not those they append to."""
-    torch.ops.lowlat_gemm.kv_append(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts)
+    _append(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts)
 
 
 def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, max_len: int, *,
@@ -54,7 +59,7 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tens
     shape = (kv_lens.shape[0], max_len, k_cache.shape[1], k_cache.shape[3])
     dtype = out_dtype or (torch.bfloat16 if e4m3 else k_cache.dtype)
     k, v = (torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
-    torch.ops.lowlat_gemm.kv_read(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens)
+    _read(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens)
     return k, v
 
 
@@ -75,6 +80,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    torch.ops.lowlat_gemm.paged_attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts,
-                                          q.shape[-1] ** -0.5 if scale is None else float(scale), causal, window)
+    _attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts,
+               q.shape[-1] ** -0.5 if scale is None else float(scale), causal, window)
     return (out, lse) if return_lse else out
