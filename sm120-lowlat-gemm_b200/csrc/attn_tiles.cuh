@@ -16,7 +16,13 @@
 // The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
 // Loaders: each of four warps fills a quarter of a tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
 // of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. 16-bit rows land in the swizzled
-// tile; e4m3 rows land in a staging ring and are widened into the tile with their power of two applied (exact).
+// tile; e4m3 rows land in a staging ring and are widened into the tile.
+// e4m3 caches are multiplied in f16 whatever q's type is: one conversion makes two values, exactly. The rows of a quarter tile (32
+// keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values (4 of 11 bits; a row
+// 2^-24 below the quarter's largest becomes 0); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
+// put the rest back where it costs nothing: score * (2^E, q's power) is the factor their multiply-add has anyway, and the
+// probability is 2^(s + F - m) with m the running maximum of s + F, so that P 2^-F V is what the product sums; the row sum takes
+// its quarters times 2^-F.
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
 // P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
@@ -35,6 +41,7 @@ constexpr int kTilesThreads = 512;
 
 template <typename T, bool FP8, int D>
 struct TilesCfg {
+  using Op = typename std::conditional<FP8, __half, T>::type;  // operand type of the products
   static constexpr int kHalf = 128 * 128;                 // 128 rows x 64 elements, one swizzle-atom column
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kHalf;           // a 128-row tile of Q, K or V
@@ -44,8 +51,10 @@ struct TilesCfg {
   static constexpr int kQ = 1024;                         // header before
   static constexpr int kRing = kQ + 2 * kTile;
   static constexpr int kStageAt = kRing + kSlots * kTile;
-  static constexpr int kScaleAt = kStageAt + kStageRing * kStage;  // [kStageRing][128] bytes
-  static constexpr int kSmem = kScaleAt + kStageRing * 128 + 1024;  // + alignment slack
+  static constexpr int kScaleAt = kStageAt + kStageRing * kStage;  // [kStageRing][128] f16: a staged row's factor
+  static constexpr int kRefAt = kScaleAt + kStageRing * 256;       // [8 key tiles][8] bytes: E and F of the quarters, biased by 127
+  static constexpr int kQFacAt = kRefAt + (FP8 ? 64 : 0);          // [2 items][256] floats: the power of two of a row of q
+  static constexpr int kSmem = kQFacAt + (FP8 ? 2048 : 0) + 1024;  // + alignment slack
 };
 
 // Shared-memory descriptor of V: rows of 64 elements (128 bytes, 128-byte swizzle) along K, 8 rows every 1024 bytes, the next
@@ -150,7 +159,9 @@ template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v) {
   using Cfg = TilesCfg<T, FP8, D>;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  using Op = typename Cfg::Op;
+  constexpr bool kBf16 = std::is_same<Op, __nv_bfloat16>::value;
+  constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
   __shared__ int scratch[kTilesThreads / 32 + 2];
   __shared__ uint32_t tmem_holder;
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     };
     // e4m3 rows: `stage` fetches the warp's quarter as it is, `widen` converts it into the ring
     constexpr int CH8 = D / 16, RP8 = 32 / CH8, IT8 = 32 / RP8;    // 16-byte pieces per row, rows per warp instruction, instructions
-    int staged = 0;
+    int staged = 0, tiles_in = 0;                                  // tiles_in: key tiles whose K has been staged
     Ring raw;
     auto stage = [&](const Row& r, bool is_v) {
       const int at = staged % 3;
@@ -322,7 +333,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(full);
       }
-      asm volatile("st.shared.u8 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 128 + lt), "r"(is_v ? r.v_sc : r.k_sc) : "memory");
+      // the row's factor relative to the quarter's largest, 2^-d as f16 (d <= 24)
+      const uint32_t b = is_v ? r.v_sc : r.k_sc, top = max(__reduce_max_sync(0xffffffffu, b), 27u);
+      const uint32_t d = top - b, half = d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 256 + lt * 2), "h"((uint16_t)half) : "memory");
+      if (!is_v) {
+        const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, r.v_sc), 27u);
+        if (lane == 0) {
+          const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + lw;
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
+        }
+        ++tiles_in;
+      }
       __syncwarp();
       ++staged;
     };
@@ -331,34 +354,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_CONVERT_WAIT);
       if (!ok) return;
       const uint32_t src = base + Cfg::kStageAt + raw.slot * Cfg::kStage + lw * (32 * D) + lane * 16;
-      const uint32_t scales = base + Cfg::kScaleAt + raw.slot * 128 + lw * 32;
+      const uint32_t scales = base + Cfg::kScaleAt + raw.slot * 256 + lw * 64;
       const uint32_t dst = base + Cfg::kRing + ring.slot * Cfg::kTile;
 #pragma unroll 4
       for (int i = 0; i < IT8; ++i) {
         const int q = i * RP8 + lane / CH8, ch = lane % CH8, row = lw * 32 + q;
         const uint4 v = lds16(src + i * 512);
         uint32_t b;
-        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(scales + q) : "memory");
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(b) : "r"(scales + q * 2) : "memory");
+        b |= b << 16;
+        const __half2 f = *reinterpret_cast<const __half2*>(&b);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Widen<T>::four(w[j], o[2 * j], o[2 * j + 1]);
-        if constexpr (kBf16) {
-          // 2^120 * 2^e in two factors, each a bf16: e up to 7 in the first
-          const int e = (int)b - 127;
-          const __nv_bfloat162 f0 = __float2bfloat162_rn(__uint_as_float((uint32_t)(min(e, 7) + 120 + 127) << 23));
+        for (int j = 0; j < 4; ++j) Widen<__half>::four(w[j], o[2 * j], o[2 * j + 1]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) *reinterpret_cast<__nv_bfloat162*>(&o[j]) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[j]), f0);
-          if (__any_sync(0xffffffffu, e > 7)) {
-            const __nv_bfloat162 f1 = __float2bfloat162_rn(__uint_as_float((uint32_t)(max(e - 7, 0) + 127) << 23));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) *reinterpret_cast<__nv_bfloat162*>(&o[j]) = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[j]), f1);
-          }
-        } else {
-          const __half2 f = __float2half2_rn(pow2_of(b));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) *reinterpret_cast<__half2*>(&o[j]) = __hmul2(*reinterpret_cast<__half2*>(&o[j]), f);
-        }
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<__half2*>(&o[j]) = __hmul2(*reinterpret_cast<__half2*>(&o[j]), f);
         const uint32_t at0 = dst + (ch >> 2) * Cfg::kHalf + row * 128;
         const int c0 = 2 * (ch & 3);
         // lanes of the two halves write alternate pieces first: eight lanes then fall on eight different bank groups
@@ -375,6 +386,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       ring.next(Cfg::kSlots);
       raw.next(3);
     };
+    int item_parity = 0;
     auto load_q = [&](const Segment& g) {
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
@@ -382,6 +394,38 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int rows = g.toks * p.group;
       const int64_t first = g.s.t0 + g.tok0;
       constexpr int CH = D / 8;
+      if constexpr (kToF16) {
+        const uint32_t flip = p.negate ? 0x80008000u : 0u;
+#pragma unroll 4
+        for (int i = lt; i < kTilesRows * CH; i += 128) {
+          const int row = i / CH, ch = i % CH;                     // CH neighbouring lanes hold a row
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row < rows) {
+            const int tok = row / p.group, hh = row - tok * p.group;
+            v = *reinterpret_cast<const uint4*>(p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16);
+          }
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[j]));
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+#pragma unroll
+          for (int o = CH / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
+          const float up = __uint_as_float((268u - e) << 23);      // 2^(14 - exponent of the row's largest value)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[j]));
+            w[j] = Mma<__half>::pack(f.x * up, f.y * up) ^ flip;
+          }
+          const uint32_t at = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          if (ch == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + Cfg::kQFacAt + item_parity * 1024 + row * 4), "r"((e - 14u) << 23) : "memory");
+        }
+        item_parity ^= 1;
+      } else {
       // 32 (16) copies of 16 bytes per thread, all in flight at once; two rows' worth of index arithmetic per thread and step
 #pragma unroll 4
       for (int i = lt; i < kTilesRows * CH; i += 128) {
@@ -402,6 +446,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ 0x80008000u), "r"(v.y ^ 0x80008000u),
                        "r"(v.z ^ 0x80008000u), "r"(v.w ^ 0x80008000u) : "memory");
         }
+      }
       }
       fence_async_shared();
       mbar_arrive(bar(BAR_Q_FULL));
@@ -588,11 +633,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + s * 128, tO = tmem + lanes + 256 + s * D;
     uint32_t s_phase = 0, pv_phase = 0;
-    const float c_log2 = p.scale_log2;
-    const uint64_t c2 = pack_f32x2(c_log2, c_log2);
+    int item_parity = 0, tile_base = 0;                            // e4m3: which q factors and which references are this item's
     while (const Segment* seg = next_item()) {
       const Segment& g = *seg;
       const int mode = tiles_mode(g, p.group);
+      const int my_parity = item_parity, my_base = tile_base - g.tile0;
+      item_parity ^= 1;
+      tile_base += g.tile1 - g.tile0;
       if (mode == MODE_ONE && s == 1) {
         done_item();
         continue;
@@ -606,7 +653,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       // rows of no token see everything: they keep no tile from the unmasked path, and nobody reads them
       const int last = !live ? INT_MAX : p.causal ? min(pos, g.s.len - 1) : g.s.len - 1;
       const int first = live && p.window > 0 ? pos - p.window + 1 : 0;
-      float m = -INFINITY;                                       // running maximum, times c_log2
+      float m = -INFINITY;                                       // running maximum of the scores in log2 units (+ F)
+      float c_row = p.scale_log2;
       uint64_t l2 = 0;                                           // two partial row sums
       int done = 0;                                              // key tiles of this stream behind us
       const int tile1 = g.tile1;
@@ -615,6 +663,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         s_phase ^= 1u;
         if (!ok) break;
         tc_fence_after();
+        // what turns a quarter's products into log2 units, and its F
+        float cq[4], fq[4];
+        uint32_t f_bytes = 0;
+        if constexpr (FP8) {
+          if (kToF16 && done == 0) {
+            float f;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(base + Cfg::kQFacAt + my_parity * 1024 + row * 4) : "memory");
+            c_row *= f;
+          }
+          const uint2 ref = lds8(base + Cfg::kRefAt + ((my_base + j) & 7) * 8);
+          f_bytes = ref.y;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            cq[q] = c_row * pow2_of((ref.x >> (8 * q)) & 0xffu);
+            fq[q] = __uint_as_float(0x4b000000u + ((ref.y >> (8 * q)) & 0xffu)) - 8388735.f;  // F: bits of 2^23 + byte, less 2^23 + 127
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            cq[q] = c_row;
+            fq[q] = 0.f;
+          }
+        }
         const int key0 = j * kTilesKT;
         // does any row of the warp see only a part of the tile?
         const bool edge = __any_sync(0xffffffffu, key0 + kTilesKT - 1 > last || key0 < first);
@@ -637,8 +708,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
 #pragma unroll
           for (int i = 2; i < 32; i += 2) part[q] = fmaxf(part[q], fmaxf(x[q][i], x[q][i + 1]));
         }
-        const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        const float top = mx * c_log2;
+        float top;
+        if constexpr (FP8) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) part[q] = fmaf(part[q], cq[q], fq[q]);
+          top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        } else {
+          top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c_row;
+        }
         const bool move = top > m + 8.f || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
           const float now = move ? top : m;
@@ -663,9 +740,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           m = now;
         }
         const float base_m = m == -INFINITY ? 0.f : m;
-        const uint64_t neg = pack_f32x2(-base_m, -base_m);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          const uint64_t c2 = pack_f32x2(cq[q], cq[q]), neg = pack_f32x2(fq[q] - base_m, fq[q] - base_m);
+          uint64_t quarter = 0;
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -673,8 +751,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             unpack_f32x2(fma_f32x2(pack_f32x2(x[q][2 * i], x[q][2 * i + 1]), c2, neg), a, b);
             a = exp2_fast(a);
             b = exp2_fast(b);
-            l2 = add_f32x2(l2, pack_f32x2(a, b));
-            w[i] = Mma<T>::pack(a, b);
+            if constexpr (FP8) quarter = add_f32x2(quarter, pack_f32x2(a, b));
+            else l2 = add_f32x2(l2, pack_f32x2(a, b));
+            w[i] = Mma<Op>::pack(a, b);
+          }
+          if constexpr (FP8) {
+            const float down = pow2_of(254u - ((f_bytes >> (8 * q)) & 0xffu));  // 2^-F
+            l2 = fma_f32x2(quarter, pack_f32x2(down, down), l2);
           }
           tmem_st16(tS + 16 * q, w);  // P lies over the first half of S, which this thread holds in registers
         }

@@ -78,7 +78,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind the last sequence are left as they were in `out`. An infinite or NaN key or value reaches every query of its
     sequence's call, also through weights of zero."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, q_starts,
                q.shape[-1] ** -0.5 if scale is None else float(scale), causal, window)
