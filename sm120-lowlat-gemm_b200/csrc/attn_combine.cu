@@ -32,15 +32,14 @@ struct RowSum {
 
 // Parts share, share + spread, ... of the row: 32 of them at a time, one per lane, then one after the other.
 template <int V>
-__device__ __forceinline__ void add_parts(const AttnDev& p, RowSum<V>& s, int parts, int twice, int first, int tile_rows, int row, int share,
+__device__ __forceinline__ void add_parts(const AttnDev& p, RowSum<V>& s, int parts, int first, int tile_rows, int row, int share,
                                           int spread, int lane) {
   for (int i0 = share; i0 < parts; i0 += 32 * spread) {
     const int i = i0 + lane * spread;
     float2 ml = make_float2(-INFINITY, 0.f);
     int64_t at = 0;
     if (i < parts) {
-      const int cta = i >> twice;
-      at = (int64_t)part_slot(first + cta, cta == 0) * tile_rows + row + (twice & i ? 128 : 0);
+      at = (int64_t)part_slot(first + i, i == 0) * tile_rows + row;
       ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
     }
     // the first sums are requested before their weights are known
@@ -95,7 +94,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
   const int went_on = p.first[blockIdx.x];  // only looked at when an item went on
   if (item.x == 0) return;
   {
-    const int twice = item.w >> 16, rows = item.w & 0xffff;
+    const int rows = item.w;
     const int first = e == 0 ? went_on : blockIdx.x;
     // this CTA's rows: worker, worker + workers, ...
     const int each = gridDim.y >> 1, workers = item.x * each, worker = (blockIdx.x - first) * each + (blockIdx.y >> 1);
@@ -107,7 +106,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
       const bool live = index < mine;
       const int row = worker + index * workers;
       RowSum<V> s;
-      if (live) add_parts<V>(p, s, item.x << twice, twice, first, tile_rows, row, share, spread, lane);
+      if (live) add_parts<V>(p, s, item.x, first, tile_rows, row, share, spread, lane);
       if (spread > 1) {
         __syncthreads();
 #pragma unroll
@@ -146,11 +145,71 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
   }
 }
 
+// Parts of the tile kernel, [slot][head_dim / 4][256 rows][4]: a warp takes 32 rows, one per lane, and eight values of each.
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const __grid_constant__ AttnDev p) {
+  constexpr int kRows = 256;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.y & 1;  // which of the main CTA's two items
+  const int4 item = p.split[2 * blockIdx.x + e];
+  const int went_on = p.first[blockIdx.x];
+  if (item.x == 0) return;
+  const int twice = item.w >> 16, rows = item.w & 0xffff, parts = item.x << twice;
+  const int first = e == 0 ? went_on : blockIdx.x;
+  const int each = gridDim.y >> 1, workers = item.x * each * kWarps;
+  const int worker = ((blockIdx.x - first) * each + (blockIdx.y >> 1)) * kWarps + warp;
+  const int units = (rows + 31) / 32 * (D / 8);
+  const float4* const o = reinterpret_cast<const float4*>(p.part_o);
+  for (int u = worker; u < units; u += workers) {
+    const int row = u / (D / 8) * 32 + lane, c = u % (D / 8);
+    const bool live = row < rows;
+    float top = -INFINITY, sum = 0.f, acc[8] = {};
+    for (int i0 = 0; i0 < parts; i0 += 4) {
+      float2 ml[4];
+      float4 x[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k, cta = i >> twice;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (i < parts && live) {
+          const int slot = part_slot(first + cta, cta == 0), r = row + (twice & i ? 128 : 0);
+          ml[k] = *reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot * kRows + r) * 2);
+          const float4* const src = o + ((int64_t)slot * (D / 4) + 2 * c) * kRows + r;
+          x[k][0] = src[0];
+          x[k][1] = src[kRows];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // no keys: the part has no sums
+        const float now = fmaxf(top, ml[k].x);
+        const float keep = top == -INFINITY ? 0.f : exp2f(top - now), w = exp2f(ml[k].x - now);
+        top = now;
+        sum = sum * keep + w * ml[k].y;
+        const float v[8] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w, x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[d] = acc[d] * keep + w * v[d];
+      }
+    }
+    if (!live) continue;
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int tok = row / p.group, head = item.z * p.group + row - tok * p.group;
+    const int64_t t = item.y + tok;
+    *reinterpret_cast<uint4*>(p.out + t * p.o_tok + head * p.o_head + 16 * c) =
+        make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv), pack2<T>(acc[4] * inv, acc[5] * inv),
+                   pack2<T>(acc[6] * inv, acc[7] * inv));
+    if (p.lse && c == 0) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+  }
+}
+
 template <typename T, int D>
 cudaError_t combine(const AttnDev& p, int ctas, int tile_rows, cudaStream_t s) {
-  // one CTA for each of the two items a CTA of the main kernel may share with others; of 256 rows, eight CTAs each, which makes
-  // two rows per warp of an item with two parts
-  return launch_ex(attn_combine_kernel<T, D>, dim3(ctas, tile_rows > 32 ? 16 : 2), dim3(32 * kWarps), 0, s, true, dim3(1, 1, 1), p, tile_rows);
+  // one CTA for each of the two items that a CTA of the main kernel may share with others, four where they have 256 rows
+  const dim3 block(32 * kWarps), one(1, 1, 1);
+  if (tile_rows > 32) return launch_ex(attn_combine_tiles_kernel<T, D>, dim3(ctas, 8), block, 0, s, true, one, p);
+  return launch_ex(attn_combine_kernel<T, D>, dim3(ctas, 2), block, 0, s, true, one, p, tile_rows);
 }
 
 }  // namespace

@@ -239,8 +239,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
     };
     if (one_page) {
       const int key0 = g.tile0 * kRowsKT + warp * 16;
-      block = key0 / c.page_size;
-      slot0 = key0 - block * c.page_size;
+      split_key(c, key0, block, slot0);
       enter(0);
     }
     auto locate = [&](int t) {
@@ -266,7 +265,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         const int key = key0 + my_row;
         row_off = -1;
         if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
-          const int b = key / c.page_size, slot = key - b * c.page_size;
+          int b, slot;
+          split_key(c, key, b, slot);
           const int q = page_of(c, g.seq, b);
           if (q >= 0) {
             row_off = is_v ? q * c.v_page + head * c.v_head + slot * c.v_slot : q * c.k_page + head * c.k_head + slot * c.k_slot;

@@ -7,16 +7,16 @@
 //   O += P V    tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (rows of head_dim: MN-major B)
 // Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). Warps 0-3 and 4-7: softmax of A and B; 8-11:
 // loaders; 12: MMA issue; 13:
-// the walk, published as segments in shared memory (14 and 15 fill the warpgroup: registers move between warpgroups, so that a
+// the walk, published as segments in shared memory; 14, 15: fetch e4m3 rows for the loaders to widen (or fill the warpgroup: registers move between warpgroups, so that a
 // row of 128 scores stays in the softmax threads). While one stream's softmax runs, the other stream's products do: per key tile and stream the tensor
 // core needs 2 x 128 x 128 x head_dim / 4096 cycles (1024 at head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the
 // two streams alternate between units that are equally busy.
 // Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
 // even key tiles, B the odd ones, and each leaves a partial result of its own.
 // The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
-// Loaders: each of four warps fills a quarter of a tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
-// of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. 16-bit rows land in the swizzled
-// tile; e4m3 rows land in a staging ring and are widened into the tile.
+// Loaders: each of four warps fills a quarter of a 16-bit tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
+// of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. e4m3 tiles come the same way, whole,
+// into a staging ring; the loaders widen them into the swizzled tile.
 // e4m3 caches are multiplied in f16 whatever q's type is: one conversion makes two values, exactly. The rows of a quarter tile (32
 // keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values (4 of 11 bits; a row
 // 2^-24 below the quarter's largest becomes 0); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
@@ -145,9 +145,8 @@ struct Ring {
 
 // Barriers in the header: word offsets of 8 bytes from the start of shared memory.
 enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24,
-             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29, BAR_RAW_FULL = 33 };
+             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29, BAR_RAW_FULL = 33, BAR_RAW_EMPTY = 37 };
 constexpr int kSegRing = 4;        // segments published ahead of the roles that work on them
-constexpr int kSegReaders = 13;    // warps that read a segment
 
 // How an item uses the two streams.
 enum : int { MODE_ROWS = 0, MODE_ONE = 1, MODE_KEYS = 2 };  // B: rows 128 and on / idle / odd key tiles
@@ -184,10 +183,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       mbar_init(bar(BAR_PV_DONE + s), 1);
     }
     mbar_init(bar(BAR_DONE), 1);
-    for (int i = 0; i < 4 * Cfg::kStageRing; ++i) mbar_init(bar(BAR_RAW_FULL + i), 1);
+    for (int i = 0; i < Cfg::kStageRing; ++i) {
+      mbar_init(bar(BAR_RAW_FULL + i), 32);
+      mbar_init(bar(BAR_RAW_EMPTY + i), 4);
+    }
     for (int i = 0; i < kSegRing; ++i) {
       mbar_init(bar(BAR_SEG_FULL + i), 1);
-      mbar_init(bar(BAR_SEG_EMPTY + i), kSegReaders);
+      mbar_init(bar(BAR_SEG_EMPTY + i), FP8 ? 15 : 13);  // the warps that read a segment
     }
     mbar_fence_init();
   }
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
 
   if (warp >= 8 && warp < 12) {
     // ================================================================================================ loaders
-    regs_down<64>();  // 512 threads start with 128 each: 2 x 200 (softmax) + 64 + 48 = 4 x 128
+    regs_down<64>();  // 512 threads start with 128 each: 2 x 200 (softmax) + 64 + 48, or 2 x 192 + 64 + 64 for e4m3 = 4 x 128
     const int lt = tid - 256, lw = warp - 8;                       // this warp fills rows 32 lw .. 32 lw + 31 of every tile
     Ring ring;
     uint32_t q_phase = 1;  // the first wait for an empty Q passes
@@ -242,7 +244,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     // A tile's row 32 lw + lane: its page (-1: no row, reads as zeros) and slot. The page table's entry is requested a tile ahead.
     struct Row {
       int pg, slot;
-      uint32_t k_sc, v_sc;
     };
     int entry = 0;
     auto in_use = [&](int j) {
@@ -250,22 +251,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       return j < tile1 && key >= key_lo && key < key_hi;
     };
     auto look_up = [&](int j) {
-      if (in_use(j)) entry = table_row[(j * kTilesKT + lt) / c.page_size];
+      int block, slot;
+      split_key(c, j * kTilesKT + lt, block, slot);
+      if (in_use(j)) entry = table_row[block];
     };
     auto locate = [&](int j) {
-      Row r{-1, 0, 0u, 0u};
+      Row r{-1, 0};
       const int pg = entry;
       look_up(j + 1);
       if (in_use(j)) {
-        r.slot = (j * kTilesKT + lt) % c.page_size;
+        int block;
+        split_key(c, j * kTilesKT + lt, block, r.slot);
         if ((unsigned)pg >= (unsigned)c.pages) {
           atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
         } else {
           r.pg = pg;
-          if constexpr (FP8) {
-            r.k_sc = c.ks[pg * c.ks_page + kv_head * c.ks_head + r.slot * c.ks_slot];
-            r.v_sc = c.vs[pg * c.vs_page + kv_head * c.vs_head + r.slot * c.vs_slot];
-          }
         }
       }
       return r;
@@ -307,50 +307,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       __syncwarp();
       ring.next(Cfg::kSlots);
     };
-    // e4m3 rows: `stage` fetches the warp's quarter as it is, `widen` converts it into the ring
+    // e4m3 rows: warps 14 and 15 fetch them as they are, `widen` converts the warp's quarter into the ring
     constexpr int CH8 = D / 16, RP8 = 32 / CH8, IT8 = 32 / RP8;    // 16-byte pieces per row, rows per warp instruction, instructions
-    int staged = 0, tiles_in = 0;                                  // tiles_in: key tiles whose K has been staged
     Ring raw;
-    auto stage = [&](const Row& r, bool is_v) {
-      const int at = staged % 3;
-      const uint32_t dst = base + Cfg::kStageAt + at * Cfg::kStage + lw * (32 * D), full = bar(BAR_RAW_FULL + 4 * at + lw);
-      if (by_tma(r)) {
-        if (lane == 0) mbar_expect_tx(full, 32 * D);
-        const int q = lane * box;
-        const int pg = __shfl_sync(0xffffffffu, r.pg, q & 31), slot = __shfl_sync(0xffffffffu, r.slot, q & 31);
-        if (q < 32) tma_load_4d(dst + q * D, is_v ? &map_v : &map_k, full, 0, slot, kv_head, pg);
-      } else {
-        const int64_t off = offset(r, is_v);
-        const unsigned char* const src = is_v ? c.v : c.k;
-#pragma unroll 4
-        for (int i = 0; i < IT8; ++i) {
-          const int64_t o = __shfl_sync(0xffffffffu, off, i * RP8 + lane / CH8);
-          cp_async16(dst + i * 512 + lane * 16, src + (o >= 0 ? o + (lane % CH8) * 16 : 0), o >= 0 ? 16u : 0u);
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_async_shared();  // a later TMA writes here
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full);
-      }
-      // the row's factor relative to the quarter's largest, 2^-d as f16 (d <= 24)
-      const uint32_t b = is_v ? r.v_sc : r.k_sc, top = max(__reduce_max_sync(0xffffffffu, b), 27u);
-      const uint32_t d = top - b, half = d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + at * 256 + lt * 2), "h"((uint16_t)half) : "memory");
-      if (!is_v) {
-        const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, r.v_sc), 27u);
-        if (lane == 0) {
-          const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + lw;
-          asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
-          asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
-        }
-        ++tiles_in;
-      }
-      __syncwarp();
-      ++staged;
-    };
     auto widen = [&]() {
-      wait(BAR_RAW_FULL + 4 * raw.slot + lw, raw.phase, ST_CONVERT_WAIT);
+      wait(BAR_RAW_FULL + raw.slot, raw.phase, ST_CONVERT_WAIT);
       wait(BAR_KV_EMPTY + ring.slot, ring.phase ^ 1u, ST_CONVERT_WAIT);
       if (!ok) return;
       const uint32_t src = base + Cfg::kStageAt + raw.slot * Cfg::kStage + lw * (32 * D) + lane * 16;
@@ -381,10 +342,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a1), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
       }
       fence_async_shared();
-      __syncwarp();  // and the stage may be fetched into again
-      if (lane == 0) mbar_arrive(bar(BAR_KV_FULL + ring.slot));
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(BAR_KV_FULL + ring.slot));
+        mbar_arrive(bar(BAR_RAW_EMPTY + raw.slot));
+      }
       ring.next(Cfg::kSlots);
-      raw.next(3);
+      raw.next(Cfg::kStageRing);
     };
     int item_parity = 0;
     auto load_q = [&](const Segment& g) {
@@ -394,59 +358,45 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int rows = g.toks * p.group;
       const int64_t first = g.s.t0 + g.tok0;
       constexpr int CH = D / 8;
-      if constexpr (kToF16) {
-        const uint32_t flip = p.negate ? 0x80008000u : 0u;
+      // 32 (16) copies of 16 bytes per thread, all in flight at once
+      const int ch = lt % CH;
+      int row = lt / CH, tok = row / p.group, hh = row - tok * p.group;
 #pragma unroll 4
-        for (int i = lt; i < kTilesRows * CH; i += 128) {
-          const int row = i / CH, ch = i % CH;                     // CH neighbouring lanes hold a row
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (row < rows) {
-            const int tok = row / p.group, hh = row - tok * p.group;
-            v = *reinterpret_cast<const uint4*>(p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16);
-          }
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          float top = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[j]));
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-#pragma unroll
-          for (int o = CH / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
-          const float up = __uint_as_float((268u - e) << 23);      // 2^(14 - exponent of the row's largest value)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[j]));
-            w[j] = Mma<__half>::pack(f.x * up, f.y * up) ^ flip;
-          }
-          const uint32_t at = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-          if (ch == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + Cfg::kQFacAt + item_parity * 1024 + row * 4), "r"((e - 14u) << 23) : "memory");
-        }
-        item_parity ^= 1;
-      } else {
-      // 32 (16) copies of 16 bytes per thread, all in flight at once; two rows' worth of index arithmetic per thread and step
-#pragma unroll 4
-      for (int i = lt; i < kTilesRows * CH; i += 128) {
-        const int row = i / CH, ch = i % CH;
-        const int tok = row / p.group, hh = row - tok * p.group;
+      for (int i = 0; i < kTilesRows * CH / 128; ++i) {
         const bool there = row < rows;
         const unsigned char* const src = p.q + (first + tok) * p.q_tok + (int64_t)(kv_head * p.group + hh) * p.q_head + ch * 16;
         cp_async16(base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4),
                    there ? src : p.q, there ? 16u : 0u);
+        row += 128 / CH;
+        for (hh += 128 / CH; hh >= p.group; hh -= p.group) ++tok;
       }
       cp_async_commit();
       cp_async_wait<0>();
-      if (p.negate) {  // a negative softmax scale: its sign goes to q, each thread turning what it copied
-        for (int i = lt; i < kTilesRows * CH; i += 128) {
-          const int row = i / CH, ch = i % CH;
-          const uint32_t at = base + Cfg::kQ + (row >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (row & 127) * 128 + (((ch & 7) ^ (row & 7)) << 4);
+      if (kToF16 || p.negate) {  // bf16 rows to f16 in place, and the sign of a negative softmax scale: each thread what it copied
+        const uint32_t flip = p.negate ? 0x80008000u : 0u;
+#pragma unroll 4
+        for (int r = lt / CH; r < kTilesRows; r += 128 / CH) {     // CH neighbouring lanes hold a row
+          const uint32_t at = base + Cfg::kQ + (r >> 7) * Cfg::kTile + (ch >> 3) * Cfg::kHalf + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4);
           const uint4 v = lds16(at);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ 0x80008000u), "r"(v.y ^ 0x80008000u),
-                       "r"(v.z ^ 0x80008000u), "r"(v.w ^ 0x80008000u) : "memory");
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          if constexpr (kToF16) {
+            // largest magnitude: bf16 bits without the sign are ordered like integers
+            uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+            for (int o = CH / 2; o >= 1; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 20u);
+            const float up = __uint_as_float((268u - e) << 23);    // 2^(14 - exponent of the row's largest value)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[j]));
+              w[j] = Mma<__half>::pack(f.x * up, f.y * up);
+            }
+            if (ch == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + Cfg::kQFacAt + item_parity * 1024 + r * 4), "r"((e - 14u) << 23) : "memory");
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0] ^ flip), "r"(w[1] ^ flip), "r"(w[2] ^ flip), "r"(w[3] ^ flip)
+                       : "memory");
         }
-      }
+        item_parity ^= 1;
       }
       fence_async_shared();
       mbar_arrive(bar(BAR_Q_FULL));
@@ -460,9 +410,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       table_row = c.table + (int64_t)seg->seq * c.table_stride;
       const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
       // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
-      look_up(tile0);
-      Row next = locate(tile0), held{};
       if constexpr (!FP8) {
+        look_up(tile0);
+        Row next = locate(tile0), held{};
         for (int j = tile0; j < tile1; ++j) {
           const Row row = next;
           next = locate(j + 1);
@@ -476,34 +426,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (keys && tile1 - tile0 == 1) load_q(*seg);
         if (keys) copy16(held, true);
       } else {
-        // the same sequence, every tile fetched three places ahead of its widening
-        const int n = 2 * (tile1 - tile0);
-        int at = tile0;
-        Row older{};  // rows whose V is still to come: `older` (when the streams take turns), then `held`
-        auto fetch = [&](int i) {
-          const bool is_k = keys ? (i == 0 || ((i & 1) && i < n - 1)) : (i & 1) == 0;
-          if (is_k) {
-            older = held;
-            held = next;
-            next = locate(++at);
-            stage(held, false);
-          } else {
-            stage(keys && i < n - 1 ? older : held, true);
-          }
-        };
-        fetch(0);
-        fetch(1);
-        if (n > 2) fetch(2);
         load_q(*seg);
-        for (int i = 0; i < n && ok; ++i) {
-          widen();
-          if (i + 3 < n) fetch(i + 3);
-        }
+        for (int n = 2 * (tile1 - tile0); n > 0 && ok; --n) widen();
       }
       done_item();
     }
   } else if (warp >= 12) {
-    regs_down<48>();
+    regs_down<FP8 ? 64 : 48>();
     if (warp == 12) {
     // ================================================================================================ MMA issue
     constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
@@ -624,10 +553,125 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       items.next(kSegRing);
       if (!more) break;
     }
+    } else if (FP8) {
+    // ================================================================================================ e4m3 fetch
+    // Tiles as they lie in the cache, in the order in which the loaders widen them - warp 14 those of K, warp 15 those of V - with
+    // what their rows' powers of two become: each row's factor relative to its quarter's largest, and the quarters' largest of K
+    // and V for the softmax. Lane l has row l of each quarter; the page table's entries are requested a tile ahead.
+    const bool is_v = warp == 15;
+    Ring raw;
+    int tiles_in = 0;            // key tiles fetched
+    while (const Segment* const seg = next_item()) {
+      const int tile0 = seg->tile0, tile1 = seg->tile1, key_lo = seg->keys.lo, key_hi = seg->keys.hi, kv_head = seg->head;
+      const int* const table_row = c.table + (int64_t)seg->seq * c.table_stride;
+      const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
+      const int n = 2 * (tile1 - tile0);
+      int j = tile0, entry[4];
+      auto look_up = [&]() {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = j * kTilesKT + 32 * q + lane;
+          int block, slot;
+          split_key(c, key, block, slot);
+          entry[q] = key >= key_lo && key < key_hi ? table_row[block] : INT_MIN;
+        }
+      };
+      look_up();
+      for (int i = 0; i < n && ok; ++i) {
+        const bool of_v = keys ? !(i == 0 || ((i & 1) && i < n - 1)) : (i & 1) != 0;
+        if (of_v != is_v) {      // the other warp's
+          raw.next(Cfg::kStageRing);
+          continue;
+        }
+        int pg[4], slot[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          int block;
+          split_key(c, j * kTilesKT + 32 * q + lane, block, slot[q]);
+          pg[q] = entry[q];
+        }
+        ++j;
+        if (j < tile1) look_up();
+        bool all = true;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if ((unsigned)pg[q] >= (unsigned)c.pages) {
+            if (pg[q] != INT_MIN) atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+            pg[q] = -1;
+            all = false;
+          }
+        }
+        all = __all_sync(0xffffffffu, all) && p.box > 0;
+        uint32_t sc[4], other[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          sc[q] = 0u;
+          if (pg[q] >= 0) {
+            const int64_t at_k = pg[q] * c.ks_page + kv_head * c.ks_head + slot[q] * c.ks_slot;
+            const int64_t at_v = pg[q] * c.vs_page + kv_head * c.vs_head + slot[q] * c.vs_slot;
+            sc[q] = is_v ? c.vs[at_v] : c.ks[at_k];
+            if (!is_v) other[q] = c.vs[at_v];
+          }
+        }
+        wait(BAR_RAW_EMPTY + raw.slot, raw.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
+        if (!ok) break;
+        const uint32_t dst = base + Cfg::kStageAt + raw.slot * Cfg::kStage, full = bar(BAR_RAW_FULL + raw.slot);
+        if (all) {
+          if (lane == 0) mbar_expect_tx_only(full, 128 * D);
+          __syncwarp();
+          const int at = lane * p.box;   // boxes of rows that share a page
+          int bp = 0, bs = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int x = __shfl_sync(0xffffffffu, pg[q], at & 31), y = __shfl_sync(0xffffffffu, slot[q], at & 31);
+            if ((at >> 5) == q) {
+              bp = x;
+              bs = y;
+            }
+          }
+          if (at < 128) tma_load_4d(dst + at * D, is_v ? &map_v : &map_k, full, 0, bs, kv_head, bp);
+        } else {
+          constexpr int CH = D / 16, RP = 32 / CH;
+          const unsigned char* const src = is_v ? c.v : c.k;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            int64_t off = -1;
+            if (pg[q] >= 0)
+              off = is_v ? pg[q] * c.v_page + kv_head * c.v_head + slot[q] * c.v_slot : pg[q] * c.k_page + kv_head * c.k_head + slot[q] * c.k_slot;
+#pragma unroll 2
+            for (int r = 0; r < CH; ++r) {
+              const int64_t o = __shfl_sync(0xffffffffu, off, r * RP + lane / CH);
+              cp_async16(dst + q * (32 * D) + r * 512 + lane * 16, src + (o >= 0 ? o + (lane % CH) * 16 : 0), o >= 0 ? 16u : 0u);
+            }
+          }
+          cp_async_commit();
+          cp_async_wait<0>();
+          fence_async_shared();  // a later TMA writes here
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t top = max(__reduce_max_sync(0xffffffffu, sc[q]), 27u);
+          const uint32_t d = top - sc[q], half = d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;  // 2^-d as f16
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + (32 * q + lane) * 2), "h"((uint16_t)half) : "memory");
+          if (!is_v) {
+            const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, other[q]), 27u);
+            if (lane == 0) {
+              const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + q;
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
+            }
+          }
+        }
+        if (!is_v) ++tiles_in;
+        mbar_arrive(full);
+        raw.next(Cfg::kStageRing);
+      }
+      done_item();
+    }
     }
   } else {
     // ================================================================================================ softmax
-    regs_up<200>();
+    regs_up<FP8 ? 192 : 200>();
     const int s = warp >> 2;                                   // stream
     const int row_in = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -775,7 +819,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int head = g.head * p.group + row - tok_row * p.group;
       const int64_t t = g.s.t0 + g.tok0 + tok_row;
       const float inv = g.whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
-      const int64_t slot_row = (int64_t)part_slot(blockIdx.x, g.starts) * kTilesRows + (mode == MODE_KEYS ? s * 128 + row_in : row);
+      const int slot = part_slot(blockIdx.x, g.starts), part_row = mode == MODE_KEYS ? s * 128 + row_in : row;
       if (done > 0) {
         wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);
         if (!ok) break;
@@ -793,15 +837,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
               dst[i] = make_uint4(Mma<T>::pack(x[8 * i] * inv, x[8 * i + 1] * inv), Mma<T>::pack(x[8 * i + 2] * inv, x[8 * i + 3] * inv),
                                   Mma<T>::pack(x[8 * i + 4] * inv, x[8 * i + 5] * inv), Mma<T>::pack(x[8 * i + 6] * inv, x[8 * i + 7] * inv));
           } else {
-            float4* const dst = reinterpret_cast<float4*>(p.part_o + slot_row * D + 32 * q);
+            // [slot][head_dim / 4][row][4]: a warp's rows lie side by side
+            float4* const dst = reinterpret_cast<float4*>(p.part_o) + ((int64_t)slot * (D / 4) + 8 * q) * kTilesRows + part_row;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 8; ++i) dst[i * kTilesRows] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
           }
         }
         tc_fence_before();
       }
       if (live) {
-        if (!g.whole) *reinterpret_cast<float2*>(p.part_ml + slot_row * 2) = make_float2(done > 0 ? m : -INFINITY, sum);
+        if (!g.whole) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * kTilesRows + part_row) * 2) = make_float2(done > 0 ? m : -INFINITY, sum);
         else if (p.lse) p.lse[t * p.lse_tok + head] = sum > 0.f || sum != sum ? (m + log2f(sum)) * 0.693147180559945309f : -INFINITY;
       }
       if (tid == 0 && !g.whole) note_split(p, g, rows | (mode == MODE_KEYS ? 1 << 16 : 0));

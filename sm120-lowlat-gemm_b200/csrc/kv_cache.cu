@@ -242,6 +242,7 @@ PagedKV paged_view(const llg_paged_kv& a, unsigned* status) {
   c.pages = a.pages; c.kv_heads = a.kv_heads; c.page_size = a.page_size; c.head_dim = a.head_dim;
   c.table_width = a.table_width; c.batch = a.batch; c.tokens = a.tokens;
   c.q_len = a.batch > 0 ? a.tokens / a.batch : 0;
+  c.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz(a.page_size) : -1;
   c.status = status;
   return c;
 }

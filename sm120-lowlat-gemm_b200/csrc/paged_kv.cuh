@@ -25,6 +25,7 @@ struct PagedKV {
   const int* lens;
   const int* starts;  // or null: every sequence has q_len new tokens
   int pages, kv_heads, page_size, head_dim, table_width, batch, tokens, q_len;
+  int page_shift;     // log2 of a page size that is a power of two, else -1
   unsigned* status;
 };
 
@@ -45,6 +46,17 @@ __device__ __forceinline__ SeqView seq_view(const PagedKV& c, int i) {
   const int64_t most = (int64_t)c.table_width * c.page_size;
   s.len = (int)min((int64_t)max(c.lens[i], 0), most);
   return s;
+}
+
+// Block (index into the page table's row) and slot of token j.
+__device__ __forceinline__ void split_key(const PagedKV& c, int j, int& block, int& slot) {
+  if (c.page_shift >= 0) {
+    block = j >> c.page_shift;
+    slot = j & (c.page_size - 1);
+  } else {
+    block = j / c.page_size;
+    slot = j - block * c.page_size;
+  }
 }
 
 // Page of token j, or -1 (recorded in the status word) when the table's entry names no page of the cache.
@@ -77,7 +89,7 @@ struct AttnDev {
   int scale16;            // 16 scale bytes of a page from a multiple of 16 on lie together, 16-byte aligned
   int tok_tile;           // whole tokens per row tile
   int box;                // rows of a TMA box (16, or a divisor of 32 and of the page size in the tile kernel), 0: no tensor maps
-  float* part_o;          // [slots][rows per tile][head_dim]
+  float* part_o;          // [slots][rows per tile][head_dim]; tile kernel: [slots][head_dim / 4][256 rows][4]
   float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
   int4* split;            // [CTAs][2]: the cut item that goes on at the beginning of a CTA's share, and the one that starts at its
                           // end: {CTAs that share it (0: none), first token, kv head, rows}; 1 << 16 in the last: every CTA left
