@@ -817,7 +817,7 @@ int llg_kv_append(const llg_kv_append_args* a, void* stream) {
   if (!aligned(a->k_in, 16) || !aligned(a->v_in, 16) || !strides16(a->k_in_stride, 2, es) || !strides16(a->v_in_stride, 2, es))
     return fail(LLG_E_INVALID, "kv_append: rows of k and v must be 16-byte aligned");
   if (a->kv.batch == 0 || a->kv.tokens == 0 || a->kv.pages == 0 || a->kv.table_width == 0) return LLG_OK;
-  if ((int64_t)a->kv.tokens * a->kv.kv_heads > INT32_MAX / 8) return fail(LLG_E_INVALID, "kv_append: too many rows in one call");
+  if ((int64_t)a->kv.kv_heads > INT32_MAX / 128) return fail(LLG_E_INVALID, "kv_append: kv_heads out of range");
   unsigned* st = status_word_device_ptr();
   if (!st) return fail(LLG_E_CUDA, "no device status word");
   return launched("kv_append", kv_append_launch(*a, st, static_cast<cudaStream_t>(stream)));
@@ -833,8 +833,8 @@ int llg_kv_read(const llg_kv_read_args* a, void* stream) {
   if (a->kv.batch == 0 || a->max_len == 0) return LLG_OK;
   if (!a->k_out || !a->v_out || !aligned(a->k_out, 16) || !aligned(a->v_out, 16)) return fail(LLG_E_INVALID, "kv_read: outputs must be 16-byte aligned");
   if (!a->kv.kv_lens || (a->kv.table_width > 0 && !a->kv.page_table)) return fail(LLG_E_INVALID, "kv_read: kv_lens and page_table must be device pointers");
-  if ((int64_t)a->kv.batch * a->max_len > INT32_MAX / 8 || (int64_t)a->kv.batch * a->max_len * a->kv.kv_heads > INT32_MAX)
-    return fail(LLG_E_INVALID, "kv_read: too many rows in one call");
+  if (a->kv.batch > 65535 || a->max_len > INT32_MAX / 2 || a->kv.kv_heads > INT32_MAX / 128)
+    return fail(LLG_E_INVALID, "kv_read: more than 65535 sequences, or max_len or kv_heads out of range");
   unsigned* st = status_word_device_ptr();
   if (!st) return fail(LLG_E_CUDA, "no device status word");
   return launched("kv_read", kv_read_launch(*a, st, static_cast<cudaStream_t>(stream)));

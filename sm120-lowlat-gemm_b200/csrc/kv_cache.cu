@@ -5,8 +5,9 @@
 // exact, so the one rounding is the conversion's. An infinity saturates to 448 * 2^119, a NaN stays one. A 16-bit cache is a copy.
 // Reading. value * 2^e, one rounding to the output type (none for bf16 and fp32: four significant bits fit).
 //
-// Both move bytes: 16-byte loads and 8- to 16-byte stores, a row per 8, 16 or 32 lanes, so that a token's heads - one
-// contiguous run of the qkv projection - are read by neighbouring lanes, and a row's maximum is a shuffle over its lanes.
+// Both move bytes. A CTA takes a few tokens: a thread per token finds its page and slot once, then the rows of all heads go
+// through, 8 values (append) or 16 stored bytes (read) per lane, a row on 8, 16 or 32 lanes so that a row's maximum is a shuffle,
+// several rows requested before the first is written.
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -62,74 +63,99 @@ __device__ __forceinline__ int row_exponent(float a) {
   return min(max(e, -100), 119);
 }
 
-// LPR lanes per row, 8 values per lane.
+// Where a token lies in the cache; pg < 0: nowhere.
+struct Place {
+  int pg, slot;
+};
+constexpr int kMaxTokens = 32;  // tokens per CTA at most
+
+// LPR lanes per row, 8 values per lane; tokens [blockIdx.x * per, + per).
 template <typename T, bool FP8, int LPR>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendDev p) {
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendDev p, int per) {
+  __shared__ Place where[kMaxTokens];
   pdl_trigger();
   pdl_wait();
   const PagedKV& c = p.c;
-  const int lane = threadIdx.x & 31, sub = lane % LPR;
-  const long long per_tok = 2ll * c.kv_heads;
-  const long long rows = per_tok * c.tokens;
-  const long long row0 = ((long long)blockIdx.x * kThreads + (threadIdx.x & ~31)) / LPR;  // the warp's first row
-  if (row0 >= rows) return;
-  const long long row = row0 + lane / LPR;
-  const bool there = row < rows;
-  const int t = (int)((there ? row : rows - 1) / per_tok);
-  int seq;
-  if (c.starts) {
-    // the rows of a warp belong to at most two tokens unless there are fewer than 32 / LPR rows per token
-    const int t_first = __shfl_sync(0xffffffffu, t, 0), t_last = __shfl_sync(0xffffffffu, t, 31);
-    seq = 0;
-    for (int x = t_first; x <= t_last; ++x) {
-      const int s = seq_of(c, x, lane);
-      if (x == t) seq = s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = threadIdx.x % LPR;
+  const int t0 = blockIdx.x * per, count = min(per, c.tokens - t0);
+  for (int i = warp; i < count; i += kThreads / 32) {  // a warp per token: its sequence by 32-way search
+    const int t = t0 + i;
+    const int seq = c.starts ? seq_of(c, t, lane) : t / c.q_len;
+    Place w{-1, 0};
+    if (lane == 0) {
+      if (seq < c.batch && (!c.starts || t >= c.starts[seq])) {  // seq == batch: behind the last sequence
+        const int end = c.starts ? min(c.starts[seq + 1], c.tokens) : (seq + 1) * c.q_len;
+        const int pos = c.lens[seq] - end + t;
+        if (pos >= 0) {
+          int block;
+          split_key(c, pos, block, w.slot);
+          if (block < c.table_width) w.pg = page_of(c, seq, block);
+        }
+      }
+      where[i] = w;
     }
-  } else {
-    seq = t / c.q_len;
   }
-  const int r = (int)((there ? row : rows - 1) - t * per_tok);
-  const bool is_v = r >= c.kv_heads;
-  const int head = is_v ? r - c.kv_heads : r;
-  bool ok = there && sub * 8 < c.head_dim && seq < c.batch;  // seq == batch: a token behind the last sequence
-  int pos = 0;
-  if (seq < c.batch) {
-    const int end = c.starts ? min(c.starts[seq + 1], c.tokens) : (seq + 1) * c.q_len;
-    pos = c.lens[seq] - end + t;
-    ok = ok && pos >= 0 && pos / c.page_size < c.table_width && (!c.starts || t >= c.starts[seq]);
-  } else {
-    ok = false;
-  }
-  int pg = -1;
-  if (ok) pg = page_of(c, seq, pos / c.page_size);
-  ok = ok && pg >= 0;
-  const int slot = pos % c.page_size;
-  const unsigned char* src = is_v ? p.v + t * p.v_tok + head * p.v_head : p.k + t * p.k_tok + head * p.k_head;
-  src += sub * 8 * sizeof(T);
-  unsigned char* const dst = is_v ? c.v + pg * c.v_page + head * c.v_head + slot * c.v_slot
-                                  : c.k + pg * c.k_page + head * c.k_head + slot * c.k_slot;
-  if constexpr (FP8) {
-    float f[8] = {};
-    if (ok) load8<T>(src, f);
-    float a = 0.f;
+  __syncthreads();
+  const int per_tok = 2 * c.kv_heads, rows = count * per_tok;
+  constexpr int kRowsPass = kThreads / LPR, kAhead = sizeof(T) == 4 ? 2 : 4;
+  const bool in_row = sub * 8 < c.head_dim;
+  for (int r0 = threadIdx.x / LPR; r0 - (int)(threadIdx.x / LPR) < rows; r0 += kRowsPass * kAhead) {
+    constexpr int W = sizeof(T) == 4 ? 2 : 1;
+    uint4 raw[kAhead][W];
+    Place at[kAhead];
+    int head[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = r0 + k * kRowsPass;
+      at[k] = Place{-1, 0};
+      head[k] = 0;
 #pragma unroll
-    for (int o = LPR / 2; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const int e = row_exponent(a);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (!ok) return;
-    uint2 q;
-    q.x = cvt_e4m3x2(f[0] * inv, f[1] * inv) | (cvt_e4m3x2(f[2] * inv, f[3] * inv) << 16);
-    q.y = cvt_e4m3x2(f[4] * inv, f[5] * inv) | (cvt_e4m3x2(f[6] * inv, f[7] * inv) << 16);
-    *reinterpret_cast<uint2*>(dst + sub * 8) = q;
-    if (sub == 0) {
-      unsigned char* const s = is_v ? c.vs + pg * c.vs_page + head * c.vs_head + slot * c.vs_slot
-                                    : c.ks + pg * c.ks_page + head * c.ks_head + slot * c.ks_slot;
-      *s = (unsigned char)(e + 127);
+      for (int w = 0; w < W; ++w) raw[k][w] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows) {
+        const int i = r / per_tok;
+        head[k] = r - i * per_tok;  // heads of K, then heads of V
+        at[k] = where[i];
+        if (at[k].pg >= 0 && in_row) {
+          const int64_t t = t0 + i;
+          const unsigned char* src = head[k] < c.kv_heads ? p.k + t * p.k_tok + head[k] * p.k_head
+                                                          : p.v + t * p.v_tok + (head[k] - c.kv_heads) * p.v_head;
+          src += sub * 8 * sizeof(T);
+#pragma unroll
+          for (int w = 0; w < W; ++w) raw[k][w] = *reinterpret_cast<const uint4*>(src + 16 * w);
+        }
+      }
     }
-  } else {
-    if (ok) *reinterpret_cast<uint4*>(dst + sub * 16) = *reinterpret_cast<const uint4*>(src);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const bool is_v = head[k] >= c.kv_heads;
+      const int h = is_v ? head[k] - c.kv_heads : head[k];
+      const bool ok = at[k].pg >= 0 && in_row;
+      unsigned char* const dst = is_v ? c.v + at[k].pg * c.v_page + h * c.v_head + at[k].slot * c.v_slot
+                                      : c.k + at[k].pg * c.k_page + h * c.k_head + at[k].slot * c.k_slot;
+      if constexpr (FP8) {
+        float f[8];
+        load8<T>(reinterpret_cast<const unsigned char*>(raw[k]), f);
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
+#pragma unroll
+        for (int o = LPR / 2; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const int e = row_exponent(a);
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (!ok) continue;
+        uint2 q;
+        q.x = cvt_e4m3x2(f[0] * inv, f[1] * inv) | (cvt_e4m3x2(f[2] * inv, f[3] * inv) << 16);
+        q.y = cvt_e4m3x2(f[4] * inv, f[5] * inv) | (cvt_e4m3x2(f[6] * inv, f[7] * inv) << 16);
+        *reinterpret_cast<uint2*>(dst + sub * 8) = q;
+        if (sub == 0) {
+          unsigned char* const s = is_v ? c.vs + at[k].pg * c.vs_page + h * c.vs_head + at[k].slot * c.vs_slot
+                                        : c.ks + at[k].pg * c.ks_page + h * c.ks_head + at[k].slot * c.ks_slot;
+          *s = (unsigned char)(e + 127);
+        }
+      } else {
+        if (ok) *reinterpret_cast<uint4*>(dst + sub * 16) = raw[k][0];
+      }
+    }
   }
 }
 
@@ -145,78 +171,121 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// LPR lanes per row, 8 values per lane; rows in the order of the output.
+// LPR lanes per row, 16 stored bytes per lane; tokens [blockIdx.x * per, + per) of sequence blockIdx.y; blockIdx.z: K or V. Rows go
+// through in the order of the output.
 template <typename T, bool FP8, int LPR>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadDev p) {
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadDev p, int per) {
+  __shared__ Place where[kMaxTokens];
   pdl_trigger();
   pdl_wait();
   const PagedKV& c = p.c;
+  const int seq = blockIdx.y, t0 = blockIdx.x * per, count = min(per, p.max_len - t0);
+  const bool is_v = blockIdx.z != 0;
   const int sub = threadIdx.x % LPR;
-  const long long rows = (long long)c.batch * p.max_len * c.kv_heads;
-  const long long row = ((long long)blockIdx.x * kThreads + threadIdx.x) / LPR;
-  if (row >= rows || sub * 8 >= c.head_dim) return;
-  const bool is_v = blockIdx.y != 0;
-  const int head = (int)(row % c.kv_heads);
-  const long long bt = row / c.kv_heads;
-  const int seq = (int)(bt / p.max_len), pos = (int)(bt - (long long)seq * p.max_len);
-  unsigned char* const dst = (is_v ? p.v : p.k) + (row * c.head_dim + sub * 8) * (int64_t)sizeof(T);
-  int pg = -1;
-  if (pos < c.lens[seq] && pos / c.page_size < c.table_width) pg = page_of(c, seq, pos / c.page_size);
-  const int slot = pos % c.page_size;
-  const unsigned char* const src = is_v ? c.v + pg * c.v_page + head * c.v_head + slot * c.v_slot
-                                        : c.k + pg * c.k_page + head * c.k_head + slot * c.k_slot;
-  if constexpr (FP8) {
-    float f[8] = {};
-    if (pg >= 0) {
-      const unsigned char* const s = is_v ? c.vs + pg * c.vs_page + head * c.vs_head + slot * c.vs_slot
-                                          : c.ks + pg * c.ks_page + head * c.ks_head + slot * c.ks_slot;
-      const uint2 q = *reinterpret_cast<const uint2*>(src + sub * 8);
-      const float up = __uint_as_float((uint32_t)*s << 23);
-      const float2 a = e4m3x2_to_f32(q.x & 0xffffu), b = e4m3x2_to_f32(q.x >> 16);
-      const float2 d = e4m3x2_to_f32(q.y & 0xffffu), e = e4m3x2_to_f32(q.y >> 16);
-      f[0] = a.x * up; f[1] = a.y * up; f[2] = b.x * up; f[3] = b.y * up;
-      f[4] = d.x * up; f[5] = d.y * up; f[6] = e.x * up; f[7] = e.y * up;
+  constexpr int kValues = FP8 ? 16 : 8;  // per lane
+  if (threadIdx.x < count) {
+    const int pos = t0 + threadIdx.x;
+    Place w{-1, 0};
+    if (pos < c.lens[seq]) {
+      int block;
+      split_key(c, pos, block, w.slot);
+      if (block < c.table_width) w.pg = page_of(c, seq, block);
     }
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<float4*>(dst + 16) = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      T o[8];
+    where[threadIdx.x] = w;
+  }
+  __syncthreads();
+  if (sub * kValues >= c.head_dim) return;
+  const unsigned char* const base = is_v ? c.v : c.k;
+  const unsigned char* const scales = is_v ? c.vs : c.ks;
+  const int64_t s_page = is_v ? c.v_page : c.k_page, s_head = is_v ? c.v_head : c.k_head, s_slot = is_v ? c.v_slot : c.k_slot;
+  const int64_t c_page = is_v ? c.vs_page : c.ks_page, c_head = is_v ? c.vs_head : c.ks_head, c_slot = is_v ? c.vs_slot : c.ks_slot;
+  unsigned char* const out = (is_v ? p.v : p.k) + ((int64_t)seq * p.max_len + t0) * c.kv_heads * c.head_dim * (int64_t)sizeof(T);
+  const int rows = count * c.kv_heads;
+  constexpr int kRowsPass = kThreads / LPR, kAhead = 4;
+  for (int r0 = threadIdx.x / LPR; r0 < rows; r0 += kRowsPass * kAhead) {
+    uint4 raw[kAhead];
+    uint32_t b[kAhead];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (std::is_same<T, __half>::value) o[i] = __float2half_rn(f[i]);
-        else o[i] = __float2bfloat16_rn(f[i]);
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = r0 + k * kRowsPass;
+      raw[k] = make_uint4(0u, 0u, 0u, 0u);
+      b[k] = 0u;
+      if (r < rows) {
+        const int i = r / c.kv_heads, head = r - i * c.kv_heads;
+        const Place w = where[i];
+        if (w.pg >= 0) {
+          raw[k] = *reinterpret_cast<const uint4*>(base + w.pg * s_page + head * s_head + w.slot * s_slot + sub * 16);
+          if constexpr (FP8) b[k] = scales[w.pg * c_page + head * c_head + w.slot * c_slot];
+        }
       }
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
     }
-  } else {
-    *reinterpret_cast<uint4*>(dst) = pg >= 0 ? *reinterpret_cast<const uint4*>(src + sub * 16) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = r0 + k * kRowsPass;
+      if (r >= rows) break;
+      unsigned char* const dst = out + ((int64_t)r * c.head_dim + sub * kValues) * (int64_t)sizeof(T);
+      if constexpr (FP8) {
+        const float up = __uint_as_float(b[k] << 23);
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = e4m3x2_to_f32(w[i] & 0xffffu), y = e4m3x2_to_f32(w[i] >> 16);
+          f[4 * i] = x.x * up; f[4 * i + 1] = x.y * up; f[4 * i + 2] = y.x * up; f[4 * i + 3] = y.y * up;
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        } else {
+          T o[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if constexpr (std::is_same<T, __half>::value) o[i] = __float2half_rn(f[i]);
+            else o[i] = __float2bfloat16_rn(f[i]);
+          }
+          reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(o)[0];
+          reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(o)[1];
+        }
+      } else {
+        *reinterpret_cast<uint4*>(dst) = raw[k];
+      }
+    }
   }
 }
 
-int lanes_of(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32; }
+int lanes_for(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32; }
+
+// Tokens per CTA: as many as keep four rows per lane group in flight, fewer while that leaves SMs without a CTA.
+int tokens_per_cta(long long tokens, int rows_per_token, int lpr) {
+  int per = 4 * (kThreads / lpr) / rows_per_token;
+  per = per < 1 ? 1 : per > kMaxTokens ? kMaxTokens : per;
+  while (per > 1 && (tokens + per - 1) / per < 2 * sm_count()) per /= 2;
+  return per;
+}
 
 template <typename T, bool FP8>
 cudaError_t append(const AppendDev& p, cudaStream_t s) {
-  const int lpr = lanes_of(p.c.head_dim);
-  const long long threads = 2ll * p.c.kv_heads * p.c.tokens * lpr;
-  const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads)), block(kThreads), one(1, 1, 1);
+  const int lpr = lanes_for(p.c.head_dim / 8);
+  const int per = tokens_per_cta(p.c.tokens, 2 * p.c.kv_heads, lpr);
+  const dim3 grid((unsigned)((p.c.tokens + per - 1) / per)), block(kThreads), one(1, 1, 1);
   switch (lpr) {
-    case 8: return launch_ex(kv_append_kernel<T, FP8, 8>, grid, block, 0, s, pdl_on(), one, p);
-    case 16: return launch_ex(kv_append_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p);
-    default: return launch_ex(kv_append_kernel<T, FP8, 32>, grid, block, 0, s, pdl_on(), one, p);
+    case 4: return launch_ex(kv_append_kernel<T, FP8, 4>, grid, block, 0, s, pdl_on(), one, p, per);
+    case 8: return launch_ex(kv_append_kernel<T, FP8, 8>, grid, block, 0, s, pdl_on(), one, p, per);
+    case 16: return launch_ex(kv_append_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p, per);
+    default: return launch_ex(kv_append_kernel<T, FP8, 32>, grid, block, 0, s, pdl_on(), one, p, per);
   }
 }
 
 template <typename T, bool FP8>
 cudaError_t read(const ReadDev& p, cudaStream_t s) {
-  const int lpr = lanes_of(p.c.head_dim);
-  const long long threads = (long long)p.c.batch * p.max_len * p.c.kv_heads * lpr;
-  const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads), 2), block(kThreads), one(1, 1, 1);
+  const int lpr = lanes_for(p.c.head_dim / (FP8 ? 16 : 8));
+  const int per = tokens_per_cta((long long)p.c.batch * p.max_len * 2, p.c.kv_heads, lpr);
+  const dim3 grid((unsigned)((p.max_len + per - 1) / per), (unsigned)p.c.batch, 2), block(kThreads), one(1, 1, 1);
   switch (lpr) {
-    case 8: return launch_ex(kv_read_kernel<T, FP8, 8>, grid, block, 0, s, pdl_on(), one, p);
-    case 16: return launch_ex(kv_read_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p);
-    default: return launch_ex(kv_read_kernel<T, FP8, 32>, grid, block, 0, s, pdl_on(), one, p);
+    case 4: return launch_ex(kv_read_kernel<T, FP8, 4>, grid, block, 0, s, pdl_on(), one, p, per);
+    case 8: return launch_ex(kv_read_kernel<T, FP8, 8>, grid, block, 0, s, pdl_on(), one, p, per);
+    case 16: return launch_ex(kv_read_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p, per);
+    default: return launch_ex(kv_read_kernel<T, FP8, 32>, grid, block, 0, s, pdl_on(), one, p, per);
   }
 }
 
