@@ -6,8 +6,8 @@
 // Reading. value * 2^e, one rounding to the output type (none for bf16 and fp32: four significant bits fit).
 //
 // Both move bytes. A CTA takes a few tokens: a thread per token finds its page and slot once, then the rows of all heads go
-// through, 8 values (append) or 16 stored bytes (read) per lane, a row on 8, 16 or 32 lanes so that a row's maximum is a shuffle,
-// several rows requested before the first is written.
+// through, 16 values (append: of K's row and of V's) or 16 stored bytes (read) per lane, a row on 4 to 32 lanes so that a row's
+// maximum is a shuffle, several rows requested before the first is written.
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -31,16 +31,16 @@ __device__ __forceinline__ int seq_of(const PagedKV& c, int t, int lane) {
   return lo;
 }
 
+// 16 values of type T held in raw words.
 template <typename T>
-__device__ __forceinline__ void load8(const unsigned char* p, float (&f)[8]) {
+__device__ __forceinline__ void as_floats(const uint4* raw, float (&f)[16]) {
+  const uint32_t* const w = reinterpret_cast<const uint32_t*>(raw);
   if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       float2 v;
       if constexpr (std::is_same<T, __half>::value) v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       else v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
@@ -69,7 +69,34 @@ struct Place {
 };
 constexpr int kMaxTokens = 32;  // tokens per CTA at most
 
-// LPR lanes per row, 8 values per lane; tokens [blockIdx.x * per, + per).
+// One row of K or V, 16 of its values per lane.
+template <typename T, bool FP8, int LPR>
+__device__ __forceinline__ void put_row(const uint4* raw, unsigned char* dst, unsigned char* scale, int sub, bool ok) {
+  if constexpr (FP8) {
+    float f[16];
+    as_floats<T>(raw, f);
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a = fmaxf(a, fabsf(f[i]));
+#pragma unroll
+    for (int o = LPR / 2; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const int e = row_exponent(a);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    if (!ok) return;
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = cvt_e4m3x2(f[4 * i] * inv, f[4 * i + 1] * inv) | (cvt_e4m3x2(f[4 * i + 2] * inv, f[4 * i + 3] * inv) << 16);
+    *reinterpret_cast<uint4*>(dst + sub * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+    if (sub == 0) *scale = (unsigned char)(e + 127);
+  } else {
+    if (!ok) return;
+    reinterpret_cast<uint4*>(dst + sub * 32)[0] = raw[0];
+    reinterpret_cast<uint4*>(dst + sub * 32)[1] = raw[1];
+  }
+}
+
+// LPR lanes per row; tokens [blockIdx.x * per, + per).
 template <typename T, bool FP8, int LPR>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendDev p, int per) {
   __shared__ Place where[kMaxTokens];
@@ -96,65 +123,45 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     }
   }
   __syncthreads();
-  const int per_tok = 2 * c.kv_heads, rows = count * per_tok;
-  constexpr int kRowsPass = kThreads / LPR, kAhead = sizeof(T) == 4 ? 2 : 4;
-  const bool in_row = sub * 8 < c.head_dim;
-  for (int r0 = threadIdx.x / LPR; r0 - (int)(threadIdx.x / LPR) < rows; r0 += kRowsPass * kAhead) {
-    constexpr int W = sizeof(T) == 4 ? 2 : 1;
-    uint4 raw[kAhead][W];
+  const int rows = count * c.kv_heads;
+  constexpr int kRowsPass = kThreads / LPR, kAhead = sizeof(T) == 4 ? 1 : 2, W = sizeof(T);  // 16-byte words per lane and row
+  const bool in_row = sub * 16 < c.head_dim;
+  const int mine = threadIdx.x / LPR;
+  for (int r0 = 0; r0 < rows; r0 += kRowsPass * kAhead) {  // the same for every lane: rows' maxima are shuffles
+    uint4 k[kAhead][W], v[kAhead][W];
     Place at[kAhead];
     int head[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int r = r0 + k * kRowsPass;
-      at[k] = Place{-1, 0};
-      head[k] = 0;
+    for (int a = 0; a < kAhead; ++a) {
+      const int r = r0 + a * kRowsPass + mine;
+      at[a] = Place{-1, 0};
+      head[a] = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) raw[k][w] = make_uint4(0u, 0u, 0u, 0u);
+      for (int w = 0; w < W; ++w) k[a][w] = v[a][w] = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows) {
-        const int i = r / per_tok;
-        head[k] = r - i * per_tok;  // heads of K, then heads of V
-        at[k] = where[i];
-        if (at[k].pg >= 0 && in_row) {
+        const int i = r / c.kv_heads;
+        head[a] = r - i * c.kv_heads;
+        at[a] = where[i];
+        if (at[a].pg >= 0 && in_row) {
           const int64_t t = t0 + i;
-          const unsigned char* src = head[k] < c.kv_heads ? p.k + t * p.k_tok + head[k] * p.k_head
-                                                          : p.v + t * p.v_tok + (head[k] - c.kv_heads) * p.v_head;
-          src += sub * 8 * sizeof(T);
+          const uint4* const ks = reinterpret_cast<const uint4*>(p.k + t * p.k_tok + head[a] * p.k_head) + sub * W;
+          const uint4* const vs = reinterpret_cast<const uint4*>(p.v + t * p.v_tok + head[a] * p.v_head) + sub * W;
 #pragma unroll
-          for (int w = 0; w < W; ++w) raw[k][w] = *reinterpret_cast<const uint4*>(src + 16 * w);
+          for (int w = 0; w < W; ++w) {
+            k[a][w] = ks[w];
+            v[a][w] = vs[w];
+          }
         }
       }
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const bool is_v = head[k] >= c.kv_heads;
-      const int h = is_v ? head[k] - c.kv_heads : head[k];
-      const bool ok = at[k].pg >= 0 && in_row;
-      unsigned char* const dst = is_v ? c.v + at[k].pg * c.v_page + h * c.v_head + at[k].slot * c.v_slot
-                                      : c.k + at[k].pg * c.k_page + h * c.k_head + at[k].slot * c.k_slot;
-      if constexpr (FP8) {
-        float f[8];
-        load8<T>(reinterpret_cast<const unsigned char*>(raw[k]), f);
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
-#pragma unroll
-        for (int o = LPR / 2; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const int e = row_exponent(a);
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        if (!ok) continue;
-        uint2 q;
-        q.x = cvt_e4m3x2(f[0] * inv, f[1] * inv) | (cvt_e4m3x2(f[2] * inv, f[3] * inv) << 16);
-        q.y = cvt_e4m3x2(f[4] * inv, f[5] * inv) | (cvt_e4m3x2(f[6] * inv, f[7] * inv) << 16);
-        *reinterpret_cast<uint2*>(dst + sub * 8) = q;
-        if (sub == 0) {
-          unsigned char* const s = is_v ? c.vs + at[k].pg * c.vs_page + h * c.vs_head + at[k].slot * c.vs_slot
-                                        : c.ks + at[k].pg * c.ks_page + h * c.ks_head + at[k].slot * c.ks_slot;
-          *s = (unsigned char)(e + 127);
-        }
-      } else {
-        if (ok) *reinterpret_cast<uint4*>(dst + sub * 16) = raw[k][0];
-      }
+    for (int a = 0; a < kAhead; ++a) {
+      const bool ok = at[a].pg >= 0 && in_row;
+      const int64_t pg = at[a].pg, slot = at[a].slot, h = head[a];
+      put_row<T, FP8, LPR>(k[a], c.k + pg * c.k_page + h * c.k_head + slot * c.k_slot,
+                           c.ks + (pg * c.ks_page + h * c.ks_head + slot * c.ks_slot), sub, ok);
+      put_row<T, FP8, LPR>(v[a], c.v + pg * c.v_page + h * c.v_head + slot * c.v_slot,
+                           c.vs + (pg * c.vs_page + h * c.vs_head + slot * c.vs_slot), sub, ok);
     }
   }
 }
@@ -255,9 +262,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
 
 int lanes_for(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32; }
 
-// Tokens per CTA: as many as keep four rows per lane group in flight, fewer while that leaves SMs without a CTA.
-int tokens_per_cta(long long tokens, int rows_per_token, int lpr) {
-  int per = 4 * (kThreads / lpr) / rows_per_token;
+// Tokens per CTA: as many as keep `ahead` rows per lane group in flight, fewer while that leaves SMs without a CTA.
+int tokens_per_cta(long long tokens, int heads, int lpr, int ahead) {
+  int per = ahead * (kThreads / lpr) / heads;
   per = per < 1 ? 1 : per > kMaxTokens ? kMaxTokens : per;
   while (per > 1 && (tokens + per - 1) / per < 2 * sm_count()) per /= 2;
   return per;
@@ -265,21 +272,20 @@ int tokens_per_cta(long long tokens, int rows_per_token, int lpr) {
 
 template <typename T, bool FP8>
 cudaError_t append(const AppendDev& p, cudaStream_t s) {
-  const int lpr = lanes_for(p.c.head_dim / 8);
-  const int per = tokens_per_cta(p.c.tokens, 2 * p.c.kv_heads, lpr);
+  const int lpr = lanes_for(p.c.head_dim / 16);
+  const int per = tokens_per_cta(p.c.tokens, p.c.kv_heads, lpr, sizeof(T) == 4 ? 1 : 2);
   const dim3 grid((unsigned)((p.c.tokens + per - 1) / per)), block(kThreads), one(1, 1, 1);
   switch (lpr) {
     case 4: return launch_ex(kv_append_kernel<T, FP8, 4>, grid, block, 0, s, pdl_on(), one, p, per);
     case 8: return launch_ex(kv_append_kernel<T, FP8, 8>, grid, block, 0, s, pdl_on(), one, p, per);
-    case 16: return launch_ex(kv_append_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p, per);
-    default: return launch_ex(kv_append_kernel<T, FP8, 32>, grid, block, 0, s, pdl_on(), one, p, per);
+    default: return launch_ex(kv_append_kernel<T, FP8, 16>, grid, block, 0, s, pdl_on(), one, p, per);
   }
 }
 
 template <typename T, bool FP8>
 cudaError_t read(const ReadDev& p, cudaStream_t s) {
   const int lpr = lanes_for(p.c.head_dim / (FP8 ? 16 : 8));
-  const int per = tokens_per_cta((long long)p.c.batch * p.max_len * 2, p.c.kv_heads, lpr);
+  const int per = tokens_per_cta((long long)p.c.batch * p.max_len * 2, p.c.kv_heads, lpr, 4);
   const dim3 grid((unsigned)((p.max_len + per - 1) / per), (unsigned)p.c.batch, 2), block(kThreads), one(1, 1, 1);
   switch (lpr) {
     case 4: return launch_ex(kv_read_kernel<T, FP8, 4>, grid, block, 0, s, pdl_on(), one, p, per);

@@ -137,7 +137,8 @@ def run_attention(a) -> None:
 
 def run_cache(a) -> None:
     kv, scales, table, lens, g = _paged(a)
-    k = torch.randn(a.batch * a.new, a.kv_heads, a.dim, generator=g, device=lens.device).to(torch.bfloat16)
+    qkv = torch.randn(a.batch * a.new, (a.heads + 2 * a.kv_heads) * a.dim, generator=g, device=lens.device).to(torch.bfloat16)
+    k = qkv[:, -a.kv_heads * a.dim:].view(-1, a.kv_heads, a.dim)  # as a projection leaves it: rows far apart
     for _ in range(a.calls):
         L.kv_append(k, k, *kv, table, lens, **scales)
         back, _ = L.kv_read(*kv, table, lens, a.kv, **scales)
