@@ -1,7 +1,9 @@
 """Tensor-parallel decode step over the GEMM library: one process per GPU, weights sharded Megatron-style.
 
-Per layer (hidden H, intermediate I; the attention itself is outside the GEMM path and is stood in for by a slice):
+Per layer (hidden H, intermediate I):
     qkv      [QKV/tp, H]   column-parallel (no communication)
+    attention over this rank's heads: with a DecodeCache the new tokens' keys and values go into the layer's paged cache and
+             paged_attention reads it; without one the attention is stood in for by a slice of the qkv projection
     o        [H, H/tp]     row-parallel    -> all-reduce(sum) of y[M, H]
     gate_up  [2*I/tp, H]   column-parallel, gate and up halves sharded separately so SiLU(gate)*up stays local
     down     [H, I/tp]     row-parallel    -> all-reduce(sum) of y[M, H]
@@ -60,6 +62,32 @@ def shard_gate_up(w: torch.Tensor, tp: int, rank: int) -> torch.Tensor:
     return torch.cat([w[rank * n:(rank + 1) * n], w[half + rank * n: half + (rank + 1) * n]], dim=0)
 
 
+class DecodeCache:
+    """Paged key/value caches of `layers` layers for `batch` sequences on this rank: one page table and one length vector serve
+    them all. dtype float8_e4m3fn (quantised rows with a power of two each) or the activations' 16-bit type. Sequences own
+    their pages from the start (max_len tokens each); kv_lens begins at 0, and every DecodeStep.run() with this cache adds its
+    tokens. Lengths live on the device, so a captured run appends on every replay; tokens beyond max_len are not stored."""
+
+    def __init__(self, layers: int, batch: int, max_len: int, kv_heads: int, device, head_dim: int = 128, page_size: int = 64,
+                 dtype: torch.dtype = FP8):
+        if dtype not in (FP8, torch.bfloat16, torch.float16):
+            raise ValueError(f"a cache holds float8_e4m3fn, bfloat16 or float16, not {dtype}")
+        if min(layers, batch, max_len, kv_heads, page_size) < 1:
+            raise ValueError("layers, batch, max_len, kv_heads and page_size must be at least 1")
+        per = -(-max_len // page_size)
+        self.batch, self.kv_heads, self.head_dim, self.dtype = batch, kv_heads, head_dim, dtype
+        self.page_table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
+        self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        shape = (batch * per, kv_heads, page_size, head_dim)
+        e4m3 = dtype == FP8
+        self.layers = []
+        for _ in range(layers):
+            k, v = (torch.zeros(shape, dtype=torch.uint8 if e4m3 else dtype, device=device).view(dtype) for _ in range(2))
+            scales = {n: torch.zeros(shape[:3], dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                      for n in ("k_scale", "v_scale")} if e4m3 else {}
+            self.layers.append(((k, v, self.page_table, self.kv_lens), scales))
+
+
 class DecodeLayer:
     """One rank's shard of one layer, with synthetic weights of the requested precision."""
 
@@ -79,7 +107,7 @@ class DecodeLayer:
 
 
 def _default_fns():
-    from . import api
+    import lowlat_gemm as api
     return api.gemm, api.quantize_fp8, api.quantize_nvfp4, api
 
 
@@ -91,11 +119,13 @@ class DecodeStep:
     sends the row-parallel projections through the push form - the GEMM's epilogue stores into every rank's buffer, one
     consumer kernel sums, adds the residual and quantizes for the next projection - and `push=False` through the pull
     form (separate all-reduce kernel, fused with the FP8 quantizer where `fuse_quant` allows, residual added by an
-    elementwise kernel). A single-rank comm (local=True) gives a one-GPU step the very same kernels."""
+    elementwise kernel). A single-rank comm (local=True) gives a one-GPU step the very same kernels.
+    cache: a DecodeCache of this rank's kv heads - (qkv - hidden) / 2 / head_dim / tp of them beside hidden / head_dim / tp query
+    heads - makes the step attend: the qkv projection's output is [query heads | key heads | value heads]."""
 
     def __init__(self, kind: str, layers: int, tp: int, rank: int, device, shape: LayerShape = LayerShape(), group=None,
                  gemm_fn=None, prefetch_bytes: int = 0, nvfp4_global: float = 64.0, comm=None, fuse_quant: bool = True,
-                 residual: bool = False, push: bool = False):
+                 residual: bool = False, push: bool = False, cache: DecodeCache | None = None):
         self.kind, self.tp, self.rank, self.group, self.device = kind, tp, rank, group, device
         self.shape = shape
         self.layers = [DecodeLayer(kind, shape, tp, rank, device, seed=i) for i in range(layers)]
@@ -113,6 +143,16 @@ class DecodeStep:
         self.push = bool(push and self.comm is not None)
         self.residual = residual
         self._ar_index = 0
+        self.cache = cache
+        if cache is not None:
+            kv = shape.qkv - shape.hidden
+            if kv <= 0 or kv % (2 * cache.head_dim * tp) or shape.hidden % (cache.head_dim * tp):
+                raise ValueError(f"qkv={shape.qkv}, hidden={shape.hidden} do not split into heads of {cache.head_dim} over tp={tp}")
+            if cache.kv_heads != kv // (2 * cache.head_dim * tp) or len(cache.layers) != layers:
+                raise ValueError(f"the cache holds {len(cache.layers)} layers of {cache.kv_heads} kv heads, the step has {layers} of "
+                                 f"{kv // (2 * cache.head_dim * tp)}")
+            if api is None:
+                raise ValueError("a cache needs the library's own entry points")
         self.fuse_quant = fuse_quant  # FP8 with `comm`: all-reduce and the next activation quantizer as one kernel
 
     def weight_bytes(self) -> int:
@@ -189,9 +229,22 @@ class DecodeStep:
             y = y + add
         return y, y
 
+    def _attend(self, qkv: torch.Tensor, layer: int) -> torch.Tensor:
+        """[M, QKV/tp] -> [M, hidden/tp]: this rank's heads' attention over the layer's cache, the new tokens appended first."""
+        dim, kv = self.cache.head_dim, self.cache.kv_heads * self.cache.head_dim
+        where, scales = self.cache.layers[layer]
+        q, k, v = (t.view(qkv.shape[0], -1, dim) for t in qkv.split([qkv.shape[1] - 2 * kv, kv, kv], dim=1))
+        self._api.kv_append(k, v, *where, **scales)
+        return self._api.paged_attention(q, *where, **scales).view(qkv.shape[0], -1)
+
     def run(self, x: torch.Tensor) -> torch.Tensor:
-        """x [M, hidden] replicated on every rank -> [M, hidden] replicated (after the last all-reduce)."""
+        """x [M, hidden] replicated on every rank -> [M, hidden] replicated (after the last all-reduce). With a cache, M is a
+        multiple of its batch: M / batch new tokens of every sequence, sequence by sequence."""
         self._ar_index = 0
+        if self.cache is not None:
+            if x.shape[0] % self.cache.batch:
+                raise ValueError(f"{x.shape[0]} rows are no multiple of the cache's {self.cache.batch} sequences")
+            self.cache.kv_lens.add_(x.shape[0] // self.cache.batch)
         order = self._order()
         nxt_w = {order[i]: self.layers[order[(i + 1) % len(order)][0]].w[order[(i + 1) % len(order)][1]][0]
                  for i in range(len(order))}
@@ -199,7 +252,10 @@ class DecodeStep:
         h_in, hidden = x, x
         for li, layer in enumerate(self.layers):
             qkv = self._project(h_in, *layer.w["qkv"], nxt_w[(li, "qkv")])
-            attn = qkv[:, :a_width]  # stand-in for this rank's attention heads' output
+            if self.cache is not None:
+                attn = self._attend(qkv, li)
+            else:
+                attn = qkv[:, :a_width]  # stand-in for this rank's attention heads' output
             if attn.data_ptr() % 16 or (attn.stride(0) * attn.element_size()) % 16:
                 attn = attn.contiguous()  # the GEMM takes strided rows as long as they stay 16-byte aligned
             o_in, hidden = self._row_parallel(attn, *layer.w["o"], nxt_w[(li, "o")], hidden, feeds_gemm=True)
