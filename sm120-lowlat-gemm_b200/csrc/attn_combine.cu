@@ -145,10 +145,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
   }
 }
 
-// Parts of the tile kernel, [slot][head_dim / 4][256 rows][4]: a warp takes 32 rows, one per lane, and eight values of each.
+// Parts of the tile kernel, [slot][head_dim / 4][256 rows][4]: a warp takes 32 rows, one per lane, and eight values of each. With
+// many parts (few rows of a long cache) the CTA's warps share that work, each every eighth part.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const __grid_constant__ AttnDev p) {
   constexpr int kRows = 256;
+  __shared__ float state[kWarps][10][32];
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -158,20 +160,31 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const _
   if (item.x == 0) return;
   const int twice = item.w >> 16, rows = item.w & 0xffff, parts = item.x << twice;
   const int first = e == 0 ? went_on : blockIdx.x;
-  const int each = gridDim.y >> 1, workers = item.x * each * kWarps;
-  const int worker = ((blockIdx.x - first) * each + (blockIdx.y >> 1)) * kWarps + warp;
+  const bool shared = parts > 2 * kWarps;  // by the whole CTA
+  const int each = gridDim.y >> 1, lanes = shared ? 1 : kWarps;
+  const int workers = item.x * each * lanes;
+  const int worker = ((blockIdx.x - first) * each + (blockIdx.y >> 1)) * lanes + (shared ? 0 : warp);
   const int units = (rows + 31) / 32 * (D / 8);
+  const int from = shared ? warp : 0, stride = shared ? kWarps : 1;
   const float4* const o = reinterpret_cast<const float4*>(p.part_o);
   for (int u = worker; u < units; u += workers) {
     const int row = u / (D / 8) * 32 + lane, c = u % (D / 8);
     const bool live = row < rows;
     float top = -INFINITY, sum = 0.f, acc[8] = {};
-    for (int i0 = 0; i0 < parts; i0 += 4) {
+    auto add = [&](float m, float l, const float (&v)[8]) {
+      const float now = fmaxf(top, m);
+      const float keep = top == -INFINITY ? 0.f : exp2f(top - now), w = exp2f(m - now);
+      top = now;
+      sum = sum * keep + w * l;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[d] = acc[d] * keep + w * v[d];
+    };
+    for (int i0 = from; i0 < parts; i0 += 4 * stride) {
       float2 ml[4];
       float4 x[4][2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i = i0 + k, cta = i >> twice;
+        const int i = i0 + k * stride, cta = i >> twice;
         ml[k] = make_float2(-INFINITY, 0.f);
         if (i < parts && live) {
           const int slot = part_slot(first + cta, cta == 0), r = row + (twice & i ? 128 : 0);
@@ -184,13 +197,24 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const _
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (ml[k].x == -INFINITY) continue;  // no keys: the part has no sums
-        const float now = fmaxf(top, ml[k].x);
-        const float keep = top == -INFINITY ? 0.f : exp2f(top - now), w = exp2f(ml[k].x - now);
-        top = now;
-        sum = sum * keep + w * ml[k].y;
         const float v[8] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w, x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
+        add(ml[k].x, ml[k].y, v);
+      }
+    }
+    if (shared) {
+      __syncthreads();  // the state of the unit before has been read
+      state[warp][8][lane] = top;
+      state[warp][9][lane] = sum;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) acc[d] = acc[d] * keep + w * v[d];
+      for (int d = 0; d < 8; ++d) state[warp][d][lane] = acc[d];
+      __syncthreads();
+      if (warp != 0) continue;
+      for (int w = 1; w < kWarps; ++w) {
+        if (state[w][8][lane] == -INFINITY) continue;
+        float v[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) v[d] = state[w][d][lane];
+        add(state[w][8][lane], state[w][9][lane], v);
       }
     }
     if (!live) continue;

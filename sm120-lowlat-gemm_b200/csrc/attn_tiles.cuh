@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       raw.next(Cfg::kStageRing);
     };
     int item_parity = 0;
-    auto load_q = [&](const Segment& g) {
+    auto q_free = [&]() { return mbar_try(bar(BAR_Q_EMPTY), q_phase); };
+    auto start_q = [&](const Segment& g) {  // copies under way
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
       if (!ok) return;
@@ -371,6 +372,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         for (hh += 128 / CH; hh >= p.group; hh -= p.group) ++tok;
       }
       cp_async_commit();
+    };
+    auto finish_q = [&]() {                 // copies there, and in the form the products take
+      if (!ok) return;
+      constexpr int CH = D / 8;
+      const int ch = lt % CH;
       cp_async_wait<0>();
       if (kToF16 || p.negate) {  // bf16 rows to f16 in place, and the sign of a negative softmax scale: each thread what it copied
         const uint32_t flip = p.negate ? 0x80008000u : 0u;
@@ -409,6 +415,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       kv_head = seg->head;
       table_row = c.table + (int64_t)seg->seq * c.table_stride;
       const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
+      // queries first when their place is free already (the first item), else behind the first tiles
+      const bool early = __all_sync(0xffffffffu, q_free());
+      if (early) start_q(*seg);
+      auto load_q = [&]() {
+        if (!early) start_q(*seg);
+        finish_q();
+      };
       // order in which the MMA warp takes them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... when the streams take turns
       if constexpr (!FP8) {
         look_up(tile0);
@@ -417,16 +430,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           const Row row = next;
           next = locate(j + 1);
           copy16(row, false);
-          if (keys && j == tile0 + 1) load_q(*seg);
+          if (keys && j == tile0 + 1) load_q();
           if (!keys) copy16(row, true);
           else if (j > tile0) copy16(held, true);
-          if (!keys && j == tile0) load_q(*seg);  // behind two tiles that travel meanwhile
+          if (!keys && j == tile0) load_q();  // behind two tiles that travel meanwhile
           held = row;
         }
-        if (keys && tile1 - tile0 == 1) load_q(*seg);
+        if (keys && tile1 - tile0 == 1) load_q();
         if (keys) copy16(held, true);
       } else {
-        load_q(*seg);
+        load_q();
         for (int n = 2 * (tile1 - tile0); n > 0 && ok; --n) widen();
       }
       done_item();
@@ -557,7 +570,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     // ================================================================================================ e4m3 fetch
     // Tiles as they lie in the cache, in the order in which the loaders widen them - warp 14 those of K, warp 15 those of V - with
     // what their rows' powers of two become: each row's factor relative to its quarter's largest, and the quarters' largest of K
-    // and V for the softmax. Lane l has row l of each quarter; the page table's entries are requested a tile ahead.
+    // and V for the softmax. Where scale bytes lie row by row and all of a tile's rows exist, a lane has the four rows from 4 * lane
+    // on - one page table entry, requested a tile ahead, and one word of scales; else it has row `lane` of each quarter.
     const bool is_v = warp == 15;
     Ring raw;
     int tiles_in = 0;            // key tiles fetched
@@ -566,33 +580,75 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int* const table_row = c.table + (int64_t)seg->seq * c.table_stride;
       const bool keys = tiles_mode(*seg, p.group) == MODE_KEYS;
       const int n = 2 * (tile1 - tile0);
-      int j = tile0, entry[4];
-      auto look_up = [&]() {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int key = j * kTilesKT + 32 * q + lane;
-          int block, slot;
-          split_key(c, key, block, slot);
-          entry[q] = key >= key_lo && key < key_hi ? table_row[block] : INT_MIN;
-        }
+      int j = tile0, entry = INT_MIN;
+      const unsigned char *const ks = c.ks + kv_head * c.ks_head, *const vs = c.vs + kv_head * c.vs_head;
+      const bool words = p.scale16 && p.box > 0;
+      auto whole = [&](int t) { return words && t * kTilesKT >= key_lo && (t + 1) * kTilesKT <= key_hi; };
+      auto look_up = [&](int t) {
+        int block, slot;
+        split_key(c, t * kTilesKT + 4 * lane, block, slot);
+        if (t < tile1 && whole(t)) entry = table_row[block];
       };
-      look_up();
+      look_up(j);
       for (int i = 0; i < n && ok; ++i) {
         const bool of_v = keys ? !(i == 0 || ((i & 1) && i < n - 1)) : (i & 1) != 0;
         if (of_v != is_v) {      // the other warp's
           raw.next(Cfg::kStageRing);
           continue;
         }
+        const int tile = j++, fast_pg = entry;
+        look_up(j);
+        if (whole(tile) && __all_sync(0xffffffffu, (unsigned)fast_pg < (unsigned)c.pages)) {
+          int block, slot;
+          split_key(c, tile * kTilesKT + 4 * lane, block, slot);
+          const uint32_t sv = *reinterpret_cast<const uint32_t*>(vs + fast_pg * c.vs_page + slot);
+          const uint32_t sc = is_v ? sv : *reinterpret_cast<const uint32_t*>(ks + fast_pg * c.ks_page + slot);
+          wait(BAR_RAW_EMPTY + raw.slot, raw.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);
+          if (!ok) break;
+          const uint32_t dst = base + Cfg::kStageAt + raw.slot * Cfg::kStage, full = bar(BAR_RAW_FULL + raw.slot);
+          if (lane == 0) mbar_expect_tx_only(full, 128 * D);
+          __syncwarp();
+          const int at = lane * p.box;   // boxes of rows that share a page
+          const int bp = __shfl_sync(0xffffffffu, fast_pg, (at >> 2) & 31), bs = __shfl_sync(0xffffffffu, slot, (at >> 2) & 31);
+          if (at < 128) tma_load_4d(dst + at * D, is_v ? &map_v : &map_k, full, 0, bs, kv_head, bp);
+          // largest of the quarter's bytes: of the word's four, then of the quarter's eight lanes
+          auto quarter_top = [&](uint32_t w) {
+            w = __vmaxu4(w, w >> 16);
+            w = max(w & 0xffu, (w >> 8) & 0xffu);
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, d));
+            return max(w, 27u);
+          };
+          const uint32_t top = quarter_top(sc);
+          uint32_t half[2] = {0u, 0u};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t d = top - ((sc >> (8 * r)) & 0xffu);
+            half[r >> 1] |= (d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u) << (16 * (r & 1));  // 2^-d as f16
+          }
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + lane * 8), "r"(half[0]), "r"(half[1]) : "memory");
+          if (!is_v) {
+            const uint32_t v_top = quarter_top(sv);
+            if ((lane & 7) == 0) {
+              const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + (lane >> 3);
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
+            }
+            ++tiles_in;
+          }
+          mbar_arrive(full);
+          raw.next(Cfg::kStageRing);
+          continue;
+        }
         int pg[4], slot[4];
+        bool all = true;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          const int key = tile * kTilesKT + 32 * q + lane;
           int block;
-          split_key(c, j * kTilesKT + 32 * q + lane, block, slot[q]);
-          pg[q] = entry[q];
+          split_key(c, key, block, slot[q]);
+          pg[q] = key >= key_lo && key < key_hi ? table_row[block] : INT_MIN;
         }
-        ++j;
-        if (j < tile1) look_up();
-        bool all = true;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if ((unsigned)pg[q] >= (unsigned)c.pages) {
@@ -607,10 +663,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         for (int q = 0; q < 4; ++q) {
           sc[q] = 0u;
           if (pg[q] >= 0) {
-            const int64_t at_k = pg[q] * c.ks_page + kv_head * c.ks_head + slot[q] * c.ks_slot;
-            const int64_t at_v = pg[q] * c.vs_page + kv_head * c.vs_head + slot[q] * c.vs_slot;
-            sc[q] = is_v ? c.vs[at_v] : c.ks[at_k];
-            if (!is_v) other[q] = c.vs[at_v];
+            const uint32_t of_values = vs[pg[q] * c.vs_page + slot[q] * c.vs_slot];
+            sc[q] = is_v ? of_values : ks[pg[q] * c.ks_page + slot[q] * c.ks_slot];
+            other[q] = of_values;
           }
         }
         wait(BAR_RAW_EMPTY + raw.slot, raw.phase ^ 1u, ST_PRODUCER_EMPTY_WAIT);

@@ -124,17 +124,29 @@ __device__ __forceinline__ int token_tiles(const AttnDev& p, const SeqView& s) {
   return rows > p.row_min && rows <= p.row_max ? (s.n + p.tok_tile - 1) / p.tok_tile : 0;
 }
 
-// Key tiles of one kv head of a sequence, over all of its token tiles. (The host refuses calls whose key tiles might not fit 31
-// bits: 64-bit divisions in every CTA's start cost a microsecond.)
+// Key tiles of token tile r.
+template <int KT>
+__device__ __forceinline__ int tile_units(const AttnDev& p, const SeqView& s, int r) {
+  const int tf = r * p.tok_tile;
+  return key_tiles<KT>(key_range(p, s, tf, min(p.tok_tile, s.n - tf)));
+}
+
+// Key tiles of one kv head of a sequence, over all of its token tiles, by one thread or by a warp. (The host refuses calls whose
+// key tiles might not fit 31 bits: 64-bit divisions in every CTA's start cost a microsecond.)
 template <int KT>
 __device__ __forceinline__ int seq_units(const AttnDev& p, const SeqView& s) {
   int u = 0;
   const int nt = token_tiles(p, s);
-  for (int r = 0; r < nt; ++r) {
-    const int tf = r * p.tok_tile;
-    u += key_tiles<KT>(key_range(p, s, tf, min(p.tok_tile, s.n - tf)));
-  }
+  for (int r = 0; r < nt; ++r) u += tile_units<KT>(p, s, r);
   return u;
+}
+template <int KT>
+__device__ __forceinline__ int seq_units_warp(const AttnDev& p, const SeqView& s) {
+  const int nt = token_tiles(p, s);
+  if (nt <= 1) return nt == 0 ? 0 : tile_units<KT>(p, s, 0);
+  int u = 0;
+  for (int r = threadIdx.x & 31; r < nt; r += 32) u += tile_units<KT>(p, s, r);
+  return __reduce_add_sync(0xffffffffu, u);
 }
 
 // A CTA's share of the key tiles and its place in the walk.
@@ -145,7 +157,8 @@ struct Share {
   int per_head;
 };
 
-// Every thread of the CTA takes part. scratch: NT / 32 + 2 ints of shared memory.
+// Every thread of the CTA takes part. scratch: NT / 32 + 2 ints of shared memory. Up to NT / 32 sequences are counted by a warp each
+// (a prompt chunk has many tiles), more by a thread each.
 template <int KT, int NT>
 __device__ __forceinline__ Share find_share(const AttnDev& p, int* scratch) {
   constexpr int W = NT / 32;
@@ -154,10 +167,20 @@ __device__ __forceinline__ Share find_share(const AttnDev& p, int* scratch) {
   int* const found = scratch + W;  // {seq, units before u}
   // one prefix sum over the first NT sequences, and the total of all
   int x = 0, rest = 0;
-  for (int i = tid; i < p.c.batch; i += NT) {
-    const int u = seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
-    if (i == tid) x = u;
-    else rest += u;
+  if (p.c.batch <= W) {
+    if (warp < p.c.batch) {
+      const int u = seq_units_warp<KT>(p, seq_view(p.c, warp)) * p.c.kv_heads;
+      if (lane == 0) part[warp] = u;
+    }
+    __syncthreads();
+    if (tid < p.c.batch) x = part[tid];
+    __syncthreads();
+  } else {
+    for (int i = tid; i < p.c.batch; i += NT) {
+      const int u = seq_units<KT>(p, seq_view(p.c, i)) * p.c.kv_heads;
+      if (i == tid) x = u;
+      else rest += u;
+    }
   }
   int inc = x;
 #pragma unroll
@@ -234,6 +257,7 @@ struct Segment {
   int first, parts;            // the item's first CTA, and how many share it
 };
 
+// Whole warps take part.
 template <int KT>
 __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segment& g) {
   if (sh.u >= sh.end) return false;
@@ -242,7 +266,7 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
     if (sh.seq >= p.c.batch) return false;
     g.s = seq_view(p.c, sh.seq);
     if (sh.known != sh.seq) {
-      sh.per_head = seq_units<KT>(p, g.s);
+      sh.per_head = seq_units_warp<KT>(p, g.s);
       sh.known = sh.seq;
     }
     per_head = sh.per_head;
@@ -253,15 +277,32 @@ __device__ __forceinline__ bool next_segment(const AttnDev& p, Share& sh, Segmen
   g.seq = sh.seq;
   g.head = sh.off / per_head;
   int rem = sh.off - g.head * per_head;
-  int units;
-  for (int r = 0;; ++r) {
-    g.tok0 = r * p.tok_tile;
-    g.toks = min(p.tok_tile, g.s.n - g.tok0);
-    g.keys = key_range(p, g.s, g.tok0, g.toks);
-    units = key_tiles<KT>(g.keys);
-    if (rem < units) break;
-    rem -= units;
+  int tile = 0;
+  const int nt = token_tiles(p, g.s);
+  if (nt > 1) {  // 32 token tiles at a time
+    const int lane = threadIdx.x & 31;
+    for (int r0 = 0;; r0 += 32) {
+      const int x = r0 + lane < nt ? tile_units<KT>(p, g.s, r0 + lane) : 0;
+      int inc = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, rem < inc);
+      if (hit != 0u || r0 + 32 >= nt) {
+        const int at = hit ? __ffs(hit) - 1 : min(31, nt - 1 - r0);
+        rem -= __shfl_sync(0xffffffffu, inc - x, at);
+        tile = r0 + at;
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, inc, 31);
+    }
   }
+  g.tok0 = tile * p.tok_tile;
+  g.toks = min(p.tok_tile, g.s.n - g.tok0);
+  g.keys = key_range(p, g.s, g.tok0, g.toks);
+  const int units = key_tiles<KT>(g.keys);
   const int take = min(units - rem, sh.end - sh.u);
   g.tile0 = g.keys.lo / KT + rem;
   g.tile1 = g.tile0 + take;
