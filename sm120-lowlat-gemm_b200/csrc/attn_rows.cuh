@@ -2,7 +2,8 @@
 //
 //   s = scale * q . k,  m = max s,  l = sum exp(s - m),  o = sum exp(s - m) v / l       one pass, running m, l and o
 //
-// Key tiles of 64 tokens; each of the CTA's four warps owns 16 of them with its own ring of stages, softmax state and
+// Key tiles of 64 tokens (128: e4m3, up to 8 rows, which halves what is spent per key beside the products); each of the CTA's four
+// warps owns 16 (32) of them with its own ring of stages, softmax state and
 // accumulators, so nothing between the loads and the last merge synchronises more than a warp. Sixteen rows that are all there and
 // share a page come by TMA, swizzled; others are gathered with cp.async, zeros for the missing. The products are taken
 // transposed, S^T[16 keys x rows] = K Q^T and O^T[head_dim x rows] = V^T P^T, so that the rows - 8 for a group of eight heads
@@ -27,7 +28,6 @@
 
 namespace llg {
 
-constexpr int kRowsKT = 64;       // keys per unit, 16 per warp
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = 32 * kRowsWarps;
 
@@ -148,9 +148,12 @@ struct RowsCfg {
   static constexpr int kChunks = kRowBytes / 16;      // 16-byte pieces per row
   static constexpr int kParts = kRowBytes > 128 ? 2 : 1;            // a row lies in pieces of at most 128 bytes ...
   static constexpr int kPitch = kRowBytes / kParts;                 // ... of this size, 16 rows of a piece together
-  static constexpr int kStage = 2 * 16 * kRowBytes;   // per warp: K, V
+  static constexpr int kSub = FP8 && NB == 1 ? 2 : 1; // groups of 16 keys per warp and tile
+  static constexpr int kKeys = 16 * kSub * kRowsWarps;
+  static constexpr int kGroup = 2 * 16 * kRowBytes;   // bytes of a group: K, V
+  static constexpr int kStage = kSub * kGroup;        // per warp
   static constexpr int kStages = [] {
-    const int n = (226 * 1024 / kCtas - 4096) / kRowsWarps / (kStage + 32);
+    const int n = (226 * 1024 / kCtas - 4096) / kRowsWarps / (kStage + 32 * kSub);
     return n > 8 ? 8 : n;
   }();
   static constexpr int kRing = kStages * kStage;      // per warp
@@ -173,11 +176,12 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   using Cfg = RowsCfg<T, FP8, D, NB>;
   using Op = typename Cfg::Op;
   constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;
+  constexpr int KT = Cfg::kKeys, SUB = Cfg::kSub;
   constexpr int S = Cfg::kStages, CH = Cfg::kChunks, KS = D / 16, MB = D / 16;
   extern __shared__ unsigned char smem_raw[];
   __shared__ int scratch[kRowsWarps + 2];
   __shared__ __align__(8) unsigned long long bars[kRowsWarps * S];
-  __shared__ __align__(16) unsigned char scales[FP8 ? kRowsWarps * S * 32 : 1];
+  __shared__ __align__(16) unsigned char scales[FP8 ? kRowsWarps * S * 32 * Cfg::kSub : 1];
   __shared__ volatile uint32_t abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int quad = lane & 3, oct = lane >> 2;  // fragment coordinates
@@ -198,9 +202,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   pdl_trigger();
   pdl_wait();
   if (tid == 0) clear_splits(p);
-  Share share = find_share<kRowsKT, kRowsThreads>(p, scratch);
+  Share share = find_share<KT, kRowsThreads>(p, scratch);
   const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing, bar = smem_u32(&bars[warp * S]);
-  const uint32_t scale_at = smem_u32(scales) + warp * S * 32;
+  const uint32_t scale_at = smem_u32(scales) + warp * S * 32 * SUB;
   int put = 0, get = 0;         // stages filled next / read next
   uint32_t get_phase = 0;
   bool gathered = false;        // copies of cp.async went into the ring since the last proxy fence
@@ -209,119 +213,110 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   const bool one_page = c.page_size % 16 == 0;  // 16 keys from a multiple of 16 on share a page
 
   Segment g;
-  while (next_segment<kRowsKT>(p, share, g)) {
+  while (next_segment<KT>(p, share, g)) {
     const int rows = g.toks * p.group;
     const int nb_used = (rows + 7) >> 3;
     const int pos0 = g.s.len - g.s.n + g.tok0;  // position of the tile's first token
 
-    // ---- the warp's ring: tile t holds keys [64 t + 16 warp, + 16) of the segment
+    // ---- the warp's ring: tile t holds the warp's groups of 16 keys, from key_of(t) on
     const int nt = g.tile1 - g.tile0;
     const int head = g.head;
     const int* const table_row = c.table + (int64_t)g.seq * c.table_stride;
     // keys that every row of the tile sees: tiles inside need no mask
     const int all_hi = p.causal ? min(pos0, g.s.len - 1) : g.s.len - 1;
     const int all_lo = p.window > 0 ? pos0 + g.toks - p.window : 0;
-    // The tile located last. One page (16 keys from a multiple of 16 on): its page (-1: none), first slot, rows [row_lo, row_hi)
-    // that exist; the page table's entry is requested a tile ahead. Else: row_off, lanes 0-15 of K's row, 16-31 of V's, -1: none.
-    int pg = -1, at = 0, row_lo = 0, row_hi = 0;
-    int64_t row_off = -1;
-    int block = 0, slot0 = 0, entry = INT_MIN;
-    uint32_t pend = 0;         // scale byte of the lane's row
-    const bool is_v = lane >= 16;
-    const int my_row = lane & 15;
-    const unsigned char* const sc_base = FP8 ? (is_v ? c.vs + head * c.vs_head + my_row * c.vs_slot : c.ks + head * c.ks_head + my_row * c.ks_slot) : nullptr;
-    auto scale_byte = [&]() -> uint32_t {  // of the lane's row of the page located last
-      return sc_base[pg * (is_v ? c.vs_page : c.ks_page) + at * (is_v ? c.vs_slot : c.ks_slot)];
+    auto key_of = [&](int t) { return (g.tile0 + t) * KT + warp * (16 * SUB); };
+    // The tile located last, where 16 keys from a multiple of 16 on share a page: the lane's group (lane % SUB), its page (-1: none)
+    // and first slot; the page table's entry is requested a tile ahead.
+    const int sub = lane % SUB;
+    int pg = -1, at = 0, entry = INT_MIN;
+    auto enter = [&](int t) {
+      const int k0 = key_of(t) + 16 * sub;
+      int block, slot;
+      split_key(c, k0, block, slot);
+      entry = t < nt && k0 < g.keys.hi && k0 + 16 > g.keys.lo ? table_row[block] : INT_MIN;
     };
-    auto enter = [&](int t) {  // requests the entry of tile t's page
-      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
-      entry = t < nt && key0 < g.keys.hi && key0 + 16 > g.keys.lo ? table_row[block] : INT_MIN;
-    };
-    if (one_page) {
-      const int key0 = g.tile0 * kRowsKT + warp * 16;
-      split_key(c, key0, block, slot0);
-      enter(0);
-    }
     auto locate = [&](int t) {
-      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
-      if (one_page) {
-        pg = entry;
-        at = slot0;
-        slot0 += kRowsKT;
-        while (slot0 >= c.page_size) {
-          slot0 -= c.page_size;
-          ++block;
-        }
-        enter(t + 1);
-        row_lo = g.keys.lo - key0;
-        row_hi = g.keys.hi - key0;
-        if ((unsigned)pg >= (unsigned)c.pages) {
-          if (pg != INT_MIN) atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
-          pg = -1;
-        } else if constexpr (FP8) {
-          if (!p.scale16) pend = scale_byte();
-        }
-      } else {
-        const int key = key0 + my_row;
-        row_off = -1;
-        if (t < nt && key >= g.keys.lo && key < g.keys.hi) {
-          int b, slot;
-          split_key(c, key, b, slot);
-          const int q = page_of(c, g.seq, b);
-          if (q >= 0) {
-            row_off = is_v ? q * c.v_page + head * c.v_head + slot * c.v_slot : q * c.k_page + head * c.k_head + slot * c.k_slot;
-            if constexpr (FP8)
-              pend = is_v ? c.vs[q * c.vs_page + head * c.vs_head + slot * c.vs_slot] : c.ks[q * c.ks_page + head * c.ks_head + slot * c.ks_slot];
-          }
-        }
+      if (!one_page) return;
+      int block;
+      split_key(c, key_of(t) + 16 * sub, block, at);
+      pg = entry;
+      enter(t + 1);
+      if ((unsigned)pg >= (unsigned)c.pages) {
+        if (pg != INT_MIN) atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
+        pg = -1;
       }
     };
+    if (one_page) enter(0);
+    const bool by_tma = one_page && p.box != 0;
     auto issue = [&](int t) {  // starts the copies of tile t, located by the call before, into stage `put`
       if (t >= nt) return;
-      const uint32_t dst = ring + put * Cfg::kStage, full = bar + 8u * put;
-      bool there = true;       // the lane's row
-      if (one_page && p.box && pg >= 0 && row_lo <= 0 && row_hi >= 16) {
+      const uint32_t dst = ring + put * Cfg::kStage, full = bar + 8u * put, sdst = scale_at + put * 32 * SUB;
+      const int k0 = key_of(t);
+      if (by_tma && k0 >= g.keys.lo && k0 + 16 * SUB <= g.keys.hi && __all_sync(0xffffffffu, pg >= 0)) {
         if (gathered) {
           fence_async_shared();
           __syncwarp();
           gathered = false;
         }
-        if (lane == 0) {
-          mbar_expect_tx(full, Cfg::kStage);
+        if (FP8 && !p.scale16) {  // scale bytes that do not lie together: one per lane
+          for (int q = 0; q < SUB; ++q) {
+            const int64_t x = __shfl_sync(0xffffffffu, pg, q), y = __shfl_sync(0xffffffffu, at, q) + (lane & 15);
+            const uint32_t v = lane < 16 ? c.ks[x * c.ks_page + head * c.ks_head + y * c.ks_slot] : c.vs[x * c.vs_page + head * c.vs_head + y * c.vs_slot];
+            asm volatile("st.shared.u8 [%0], %1;" ::"r"(sdst + q * 32 + lane), "r"(v) : "memory");
+          }
+        }
+        if (lane < SUB) {
+          mbar_expect_tx(full, Cfg::kGroup);
 #pragma unroll
           for (int h = 0; h < Cfg::kParts; ++h) {
-            tma_load_4d(dst + h * 2048, &map_k, full, h * 64, at, head, pg);
-            tma_load_4d(dst + 16 * Cfg::kRowBytes + h * 2048, &map_v, full, h * 64, at, head, pg);
+            tma_load_4d(dst + sub * Cfg::kGroup + h * 2048, &map_k, full, h * 64, at, head, pg);
+            tma_load_4d(dst + sub * Cfg::kGroup + 16 * Cfg::kRowBytes + h * 2048, &map_v, full, h * 64, at, head, pg);
           }
-        } else if (FP8 && p.scale16 && lane <= 2) {  // the 16 scale bytes of K (lane 1) and V (lane 2)
-          cp_async16(scale_at + put * 32 + (lane - 1) * 16, lane == 1 ? c.ks + pg * c.ks_page + head * c.ks_head + at : c.vs + pg * c.vs_page + head * c.vs_head + at, 16u);
+        } else if (FP8 && p.scale16 && lane < 3 * SUB) {  // a group's 16 scale bytes of K, of V
+          const bool is_v = lane >= 2 * SUB;
+          cp_async16(sdst + sub * 32 + (is_v ? 16 : 0), is_v ? c.vs + pg * c.vs_page + head * c.vs_head + at : c.ks + pg * c.ks_page + head * c.ks_head + at, 16u);
           cp_async_arrive_noinc(full);
         } else {
           mbar_arrive(full);
         }
-        if (FP8 && p.scale16) {
-          put = put + 1 == S ? 0 : put + 1;
-          return;
-        }
       } else {
-        if (one_page) {
-          row_off = -1;
-          if (FP8 && pg >= 0 && p.scale16) pend = scale_byte();
-          if (pg >= 0 && my_row >= row_lo && my_row < row_hi)
-            row_off = is_v ? pg * c.v_page + head * c.v_head + (at + my_row) * c.v_slot : pg * c.k_page + head * c.k_head + (at + my_row) * c.k_slot;
-        }
-        there = row_off >= 0;
+        // row by row, zeros for rows that are not there; lanes 0-15: rows of K, 16-31: of V
+        const bool is_v = lane >= 16;
+#pragma unroll 1
+        for (int q = 0; q < SUB; ++q) {
+          const int key = k0 + 16 * q + (lane & 15);
+          int64_t page = -1, slot = 0;
+          if (one_page) {
+            const int x = __shfl_sync(0xffffffffu, pg, q), y = __shfl_sync(0xffffffffu, at, q);
+            if (key >= g.keys.lo && key < g.keys.hi) page = x;
+            slot = y + (lane & 15);
+          } else if (key >= g.keys.lo && key < g.keys.hi) {
+            int block, y;
+            split_key(c, key, block, y);
+            page = page_of(c, g.seq, block);
+            slot = y;
+          }
+          int64_t off = -1;
+          uint32_t scale = 0u;
+          if (page >= 0) {
+            off = is_v ? page * c.v_page + head * c.v_head + slot * c.v_slot : page * c.k_page + head * c.k_head + slot * c.k_slot;
+            if constexpr (FP8)
+              scale = is_v ? c.vs[page * c.vs_page + head * c.vs_head + slot * c.vs_slot] : c.ks[page * c.ks_page + head * c.ks_head + slot * c.ks_slot];
+          }
 #pragma unroll 2
-        for (int i = 0; i < CH / 2; ++i) {
-          const int row = lane / CH + i * (32 / CH), ch = lane % CH;
-          const int64_t ko = __shfl_sync(0xffffffffu, row_off, row), vo = __shfl_sync(0xffffffffu, row_off, 16 + row);
-          cp_async16(dst + rows_at<Cfg>(row, ch), c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
-          cp_async16(dst + 16 * Cfg::kRowBytes + rows_at<Cfg>(row, ch), c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+          for (int i = 0; i < CH / 2; ++i) {
+            const int row = lane / CH + i * (32 / CH), ch = lane % CH;
+            const int64_t ko = __shfl_sync(0xffffffffu, off, row), vo = __shfl_sync(0xffffffffu, off, 16 + row);
+            const uint32_t to = dst + q * Cfg::kGroup + rows_at<Cfg>(row, ch);
+            cp_async16(to, c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16u : 0u);
+            cp_async16(to + 16 * Cfg::kRowBytes, c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16u : 0u);
+          }
+          if constexpr (FP8) asm volatile("st.shared.u8 [%0], %1;" ::"r"(sdst + q * 32 + lane), "r"(scale) : "memory");
         }
         cp_async_arrive_noinc(full);
         gathered = true;
       }
-      if constexpr (FP8) asm volatile("st.shared.u8 [%0], %1;" ::"r"(scale_at + put * 32 + lane), "r"(there ? pend : 0u) : "memory");
       put = put + 1 == S ? 0 : put + 1;
     };
     for (int t = 0; t < S - 1; ++t) {
@@ -399,7 +394,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
     }
 
     for (int t = 0; t < nt; ++t) {
-      const uint32_t kb = ring + get * Cfg::kStage, vb = kb + 16 * Cfg::kRowBytes, sb = scale_at + get * 32;
+      const uint32_t stage = ring + get * Cfg::kStage, sb = scale_at + get * 32 * SUB;
       if (ok_all && !mbar_wait(bar + 8u * get, get_phase, &abort_word)) {
         ok_all = false;
         atomicCAS(c.status, 0u, (unsigned)ST_CONVERT_WAIT);
@@ -412,72 +407,83 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       issue(t + S - 1);  // into the stage that the warp finished reading one tile ago
 
       // ---- S^T = K Q^T: thread holds keys oct, oct + 8 of rows 2 * quad, 2 * quad + 1 of each block
-      float s[NB][4];
+      float s[SUB][NB][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-      if constexpr (FP8) {
+      for (int u = 0; u < SUB; ++u) {
+        const uint32_t kb = stage + u * Cfg::kGroup;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const int ch = quad + 4 * i;
-          const uint4 r0 = lds16(kb + rows_at<Cfg>(krow, ch)), r1 = lds16(kb + rows_at<Cfg>(krow + 8, ch));
-          const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+        for (int nb = 0; nb < NB; ++nb) s[u][nb][0] = s[u][nb][1] = s[u][nb][2] = s[u][nb][3] = 0.f;
+        if constexpr (FP8) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int i = 0; i < D / 64; ++i) {
+            const int ch = quad + 4 * i;
+            const uint4 r0 = lds16(kb + rows_at<Cfg>(krow, ch)), r1 = lds16(kb + rows_at<Cfg>(krow + 8, ch));
+            const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t a[4];
+              Widen<Op>::four(w0[j], a[0], a[2]);
+              Widen<Op>::four(w1[j], a[1], a[3]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                if (nb < nb_used) Mma<Op>::run(s[u][nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
             uint32_t a[4];
-            Widen<Op>::four(w0[j], a[0], a[2]);
-            Widen<Op>::four(w1[j], a[1], a[3]);
+            const int row = lane & 15, ch = 2 * ks + (lane >> 4);
+            ldsm_x4(kb + rows_at<Cfg>(row, ch), a);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (nb < nb_used) Mma<Op>::run(s[nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
+              if (nb < nb_used) Mma<Op>::run(s[u][nb], a, qf[nb][ks][0], qf[nb][ks][1]);
           }
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t a[4];
-          const int row = lane & 15, ch = 2 * ks + (lane >> 4);
-          ldsm_x4(kb + rows_at<Cfg>(row, ch), a);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            if (nb < nb_used) Mma<Op>::run(s[nb], a, qf[nb][ks][0], qf[nb][ks][1]);
         }
       }
 
       // ---- softmax
-      const int key0 = (g.tile0 + t) * kRowsKT + warp * 16;
-      const bool inner = key0 >= all_lo && key0 + 15 <= all_hi;
-      float kf[2] = {1.f, 1.f}, vf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};  // keys krow, krow + 8: 2^e of K, 2^e and e of V
-      if constexpr (FP8) {
-        const uint32_t at = sb + krow;
+      const int key0 = key_of(t);
+      const bool inner = key0 >= all_lo && key0 + 16 * SUB - 1 <= all_hi;
+      float kf[SUB][2], vf[SUB][2], ve[SUB][2];  // keys krow, krow + 8 of a group: 2^e of K, 2^e and e of V
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          uint32_t bk, bv;
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk) : "r"(at + 8 * e) : "memory");
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv) : "r"(at + 16 + 8 * e) : "memory");
-          kf[e] = pow2_of(bk);
-          vf[e] = pow2_of(bv);
-          ve[e] = __uint_as_float(0x4b000000u + max(bv, 27u)) - 8388735.f;  // e, not below -100: bits of 2^23 + b, less 2^23 + 127
+          kf[u][e] = vf[u][e] = 1.f;
+          ve[u][e] = 0.f;
+          if constexpr (FP8) {
+            uint32_t bk, bv;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk) : "r"(sb + 32 * u + krow + 8 * e) : "memory");
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv) : "r"(sb + 32 * u + 16 + krow + 8 * e) : "memory");
+            kf[u][e] = pow2_of(bk);
+            vf[u][e] = pow2_of(bv);
+            ve[u][e] = __uint_as_float(0x4b000000u + max(bv, 27u)) - 8388735.f;  // e, not below -100: bits of 2^23 + b, less 2^23 + 127
+          }
         }
-      }
-      uint32_t pf[NB][2];
+      uint32_t pf[SUB][NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         if (nb >= nb_used) continue;
-        float x[4];
+        float x[SUB][4];
         bool more = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = s[nb][e] * (row_f[nb][e & 1] * kf[e >> 1]);
-          if (!inner) {
-            const int key = key0 + krow + (e >> 1) * 8;
-            if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[e] = -INFINITY;
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[u][e] = s[u][nb][e] * (row_f[nb][e & 1] * kf[u][e >> 1]);
+            if (!inner) {
+              const int key = key0 + 16 * u + krow + (e >> 1) * 8;
+              if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[u][e] = -INFINITY;
+            }
+            more |= x[u][e] + ve[u][e >> 1] > m[nb][e & 1] + 8.f;
           }
-          more |= x[e] + ve[e >> 1] > m[nb][e & 1] + 8.f;
-        }
         if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[e] + ve[0], x[e + 2] + ve[1]);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) mx = fmaxf(mx, fmaxf(x[u][e] + ve[u][0], x[u][e + 2] + ve[u][1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -492,54 +498,61 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
             }
           }
         }
-        float pr[4];
+        const float base[2] = {m[nb][0] == -INFINITY ? 0.f : m[nb][0], m[nb][1] == -INFINITY ? 0.f : m[nb][1]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float mm = m[nb][e & 1];
-          pr[e] = exp2_fast(x[e] - (mm == -INFINITY ? 0.f : mm));
-          l[nb][e & 1] += pr[e];
+        for (int u = 0; u < SUB; ++u) {
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pr[e] = exp2_fast(x[u][e] - base[e & 1]);
+            l[nb][e & 1] += pr[e];
+          }
+          pf[u][nb][0] = transpose8x8(Mma<Op>::pack(pr[0] * vf[u][0], pr[1] * vf[u][0]));
+          pf[u][nb][1] = transpose8x8(Mma<Op>::pack(pr[2] * vf[u][1], pr[3] * vf[u][1]));
         }
-        pf[nb][0] = transpose8x8(Mma<Op>::pack(pr[0] * vf[0], pr[1] * vf[0]));
-        pf[nb][1] = transpose8x8(Mma<Op>::pack(pr[2] * vf[1], pr[3] * vf[1]));
       }
 
       // ---- O^T += V^T P^T
-      if constexpr (FP8) {
-        constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (of head_dim: 16 * krow + ..., or 8 * oct + ...)
-        uint32_t w[4][W];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = ((r & 1) ? vrow1 : vrow0) + (r >> 1) * 8;
-          if constexpr (D == 128) {
-            const uint4 v = lds16(vb + rows_at<Cfg>(row, krow));
-            w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
-          } else {
-            const uint2 v = lds8(vb + rows_at<Cfg>(row, oct >> 1) + (oct & 1) * 8);
-            w[r][0] = v.x; w[r][1] = v.y;
+      for (int u = 0; u < SUB; ++u) {
+        const uint32_t vb = stage + u * Cfg::kGroup + 16 * Cfg::kRowBytes;
+        if constexpr (FP8) {
+          constexpr int W = D / 32;  // 4-byte words of a row that a thread holds (of head_dim: 16 * krow + ..., or 8 * oct + ...)
+          uint32_t w[4][W];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = ((r & 1) ? vrow1 : vrow0) + (r >> 1) * 8;
+            if constexpr (D == 128) {
+              const uint4 v = lds16(vb + rows_at<Cfg>(row, krow));
+              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+            } else {
+              const uint2 v = lds8(vb + rows_at<Cfg>(row, oct >> 1) + (oct & 1) * 8);
+              w[r][0] = v.x; w[r][1] = v.y;
+            }
           }
-        }
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          uint32_t lo[4], hi[4];
-          Widen<Op>::cross(w[0][j], w[1][j], lo);
-          Widen<Op>::cross(w[2][j], w[3][j], hi);
+          for (int j = 0; j < W; ++j) {
+            uint32_t lo[4], hi[4];
+            Widen<Op>::cross(w[0][j], w[1][j], lo);
+            Widen<Op>::cross(w[2][j], w[3][j], hi);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                if (nb < nb_used) Mma<Op>::run(o[nb][2 * j + h], a, pf[u][nb][0], pf[u][nb][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            uint32_t a[4];
+            const int row = (lane & 7) + ((lane >> 4) << 3), ch = 2 * mb + ((lane >> 3) & 1);
+            ldsm_x4_t(vb + rows_at<Cfg>(row, ch), a);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (nb < nb_used) Mma<Op>::run(o[nb][2 * j + h], a, pf[nb][0], pf[nb][1]);
+              if (nb < nb_used) Mma<Op>::run(o[nb][mb], a, pf[u][nb][0], pf[u][nb][1]);
           }
-        }
-      } else {
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          uint32_t a[4];
-          const int row = (lane & 7) + ((lane >> 4) << 3), ch = 2 * mb + ((lane >> 3) & 1);
-          ldsm_x4_t(vb + rows_at<Cfg>(row, ch), a);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            if (nb < nb_used) Mma<Op>::run(o[nb][mb], a, pf[nb][0], pf[nb][1]);
         }
       }
       __syncwarp();          // every lane has read the stage before the next issue overwrites it

@@ -97,10 +97,10 @@ struct AttnDev {
   int* first;             // [CTAs]: the CTA in which the item that goes on started
 };
 
-// CTAs of the few-row kernel that fit an SM: four where a tile's key rows and accumulators are small (e4m3 rows, or head_dim 64,
-// with 8 rows), which hides the chain from a load to the next product better than longer rings; three and two otherwise.
+// CTAs of the few-row kernel that fit an SM: as many as its registers and rings of two to three tiles let in, which hides the chain
+// from a load to the next product better than longer rings (e4m3, head_dim 128, 8 rows: three).
 __host__ __device__ constexpr int rows_ctas_per_sm(bool fp8, int head_dim, int blocks) {
-  return fp8 || head_dim == 64 ? (blocks == 1 ? 4 : blocks == 2 ? 3 : 2) : 2;
+  return blocks == 4 ? 2 : blocks == 2 ? (fp8 || head_dim == 64 ? 3 : 2) : fp8 ? 3 : head_dim == 64 ? 4 : 2;
 }
 
 // Keys [lo, hi) that any row of token tile [tf, tf + cnt) sees.
