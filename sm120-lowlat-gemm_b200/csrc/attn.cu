@@ -121,12 +121,11 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     int box = 32;
     while (p.c.page_size % box) box /= 2;
     p.box = box >= 8 && maps(box, !fp8) ? box : 0;
-    cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s)
+    const cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s)
                         : attn_tiles_launch_bf16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s);
     if (e != cudaSuccess) return e;
-    e = attn_combine_launch(p, f16, plan.m.ctas, kTileRows, s);
-    if (e != cudaSuccess) return e;
   }
+  const AttnDev many = p;
   if (plan.few) {
     use(plan.f);
     p.row_min = 0;
@@ -135,13 +134,12 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     p.scale_log2 = scale_log2;
     p.box = p.c.page_size % 16 == 0 && maps(16, true) ? 16 : 0;  // a warp's 16 keys
     const int blocks = plan.f.rows / 8;
-    cudaError_t e = f16 ? attn_rows_launch_f16(p, mk, mv, fp8, blocks, plan.f.ctas, pdl_on(), s)
-                        : attn_rows_launch_bf16(p, mk, mv, fp8, blocks, plan.f.ctas, pdl_on(), s);
-    if (e != cudaSuccess) return e;
-    e = attn_combine_launch(p, f16, plan.f.ctas, plan.f.rows, s);
+    const bool early = plan.many || pdl_on();  // behind the tile kernel the launch overlaps its end; the kernel waits for it
+    const cudaError_t e = f16 ? attn_rows_launch_f16(p, mk, mv, fp8, blocks, plan.f.ctas, early, s)
+                        : attn_rows_launch_bf16(p, mk, mv, fp8, blocks, plan.f.ctas, early, s);
     if (e != cudaSuccess) return e;
   }
-  return cudaSuccess;
+  return attn_combine_launch(plan.many ? many : p, p, f16, plan.many ? plan.m.ctas : 0, plan.few ? plan.f.ctas : 0, plan.few ? plan.f.rows : 0, s);
 }
 
 }  // namespace llg

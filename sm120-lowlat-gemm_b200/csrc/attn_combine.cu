@@ -82,22 +82,19 @@ __device__ __forceinline__ void add_parts(const AttnDev& p, RowSum<V>& s, int pa
   for (int o = 16; o >= 1; o >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, o);
 }
 
+// One CTA for each of the two items that CTA `cta` of the few-row kernel may share with others.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_constant__ AttnDev p, int tile_rows) {
+__device__ __forceinline__ void combine_rows(const AttnDev& p, int cta, int e, int tile_rows, float (*part)[D + 2]) {
   constexpr int V = D / 32;
-  __shared__ float part[kWarps][D + 2];
-  pdl_trigger();
-  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int e = blockIdx.y & 1;  // which of the main CTA's two items
-  const int4 item = p.split[2 * blockIdx.x + e];
-  const int went_on = p.first[blockIdx.x];  // only looked at when an item went on
+  const int4 item = p.split[2 * cta + e];
+  const int went_on = p.first[cta];  // only looked at when an item went on
   if (item.x == 0) return;
   {
     const int rows = item.w;
-    const int first = e == 0 ? went_on : blockIdx.x;
+    const int first = e == 0 ? went_on : cta;
     // this CTA's rows: worker, worker + workers, ...
-    const int each = gridDim.y >> 1, workers = item.x * each, worker = (blockIdx.x - first) * each + (blockIdx.y >> 1);
+    const int workers = item.x, worker = cta - first;
     const int mine = worker < rows ? (rows - worker + workers - 1) / workers : 0;
     const int spread = mine >= kWarps ? 1 : mine >= 4 ? 2 : mine >= 2 ? 4 : kWarps;  // warps per row
     const int share = warp % spread;
@@ -146,24 +143,22 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_
 }
 
 // Parts of the tile kernel, [slot][head_dim / 4][256 rows][4]: a warp takes 32 rows, one per lane, and eight values of each. With
-// many parts (few rows of a long cache) the CTA's warps share that work, each every eighth part.
+// many parts (few rows of a long cache) the CTA's warps share that work, each every eighth part. kTileShare CTAs for each of the
+// two items that CTA `cta` of the tile kernel may share with others; this is number `nth`.
+constexpr int kTileShare = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const __grid_constant__ AttnDev p) {
+__device__ __forceinline__ void combine_tiles(const AttnDev& p, int cta, int e, int nth, float (*state)[10][32]) {
   constexpr int kRows = 256;
-  __shared__ float state[kWarps][10][32];
-  pdl_trigger();
-  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int e = blockIdx.y & 1;  // which of the main CTA's two items
-  const int4 item = p.split[2 * blockIdx.x + e];
-  const int went_on = p.first[blockIdx.x];
+  const int4 item = p.split[2 * cta + e];
+  const int went_on = p.first[cta];
   if (item.x == 0) return;
   const int twice = item.w >> 16, rows = item.w & 0xffff, parts = item.x << twice;
-  const int first = e == 0 ? went_on : blockIdx.x;
+  const int first = e == 0 ? went_on : cta;
   const bool shared = parts > 2 * kWarps;  // by the whole CTA
-  const int each = gridDim.y >> 1, lanes = shared ? 1 : kWarps;
-  const int workers = item.x * each * lanes;
-  const int worker = ((blockIdx.x - first) * each + (blockIdx.y >> 1)) * lanes + (shared ? 0 : warp);
+  const int lanes = shared ? 1 : kWarps;
+  const int workers = item.x * kTileShare * lanes;
+  const int worker = ((cta - first) * kTileShare + nth) * lanes + (shared ? 0 : warp);
   const int units = (rows + 31) / 32 * (D / 8);
   const int from = shared ? warp : 0, stride = shared ? kWarps : 1;
   const float4* const o = reinterpret_cast<const float4*>(p.part_o);
@@ -184,10 +179,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const _
       float4 x[4][2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i = i0 + k * stride, cta = i >> twice;
+        const int i = i0 + k * stride, of = i >> twice;
         ml[k] = make_float2(-INFINITY, 0.f);
         if (i < parts && live) {
-          const int slot = part_slot(first + cta, cta == 0), r = row + (twice & i ? 128 : 0);
+          const int slot = part_slot(first + of, of == 0), r = row + (twice & i ? 128 : 0);
           ml[k] = *reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot * kRows + r) * 2);
           const float4* const src = o + ((int64_t)slot * (D / 4) + 2 * c) * kRows + r;
           x[k][0] = src[0];
@@ -228,20 +223,34 @@ __global__ void __launch_bounds__(32 * kWarps) attn_combine_tiles_kernel(const _
   }
 }
 
+// Both kernels' items in one launch: first those of the tile kernel's CTAs, then those of the few-row kernel's.
 template <typename T, int D>
-cudaError_t combine(const AttnDev& p, int ctas, int tile_rows, cudaStream_t s) {
-  // one CTA for each of the two items that a CTA of the main kernel may share with others, four where they have 256 rows
-  const dim3 block(32 * kWarps), one(1, 1, 1);
-  if (tile_rows > 32) return launch_ex(attn_combine_tiles_kernel<T, D>, dim3(ctas, 8), block, 0, s, true, one, p);
-  return launch_ex(attn_combine_kernel<T, D>, dim3(ctas, 2), block, 0, s, true, one, p, tile_rows);
+__global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_constant__ AttnDev many, const __grid_constant__ AttnDev few,
+                                                                   int many_blocks, int few_rows) {
+  __shared__ union {
+    float part[kWarps][D + 2];
+    float state[kWarps][10][32];
+  } sh;
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x;
+  if (b < many_blocks) combine_tiles<T, D>(many, b / (2 * kTileShare), b & 1, (b >> 1) % kTileShare, sh.state);
+  else combine_rows<T, D>(few, (b - many_blocks) >> 1, (b - many_blocks) & 1, few_rows, sh.part);
+}
+
+template <typename T, int D>
+cudaError_t combine(const AttnDev& many, const AttnDev& few, int many_ctas, int few_ctas, int few_rows, cudaStream_t s) {
+  const int many_blocks = many_ctas * 2 * kTileShare;
+  return launch_ex(attn_combine_kernel<T, D>, dim3(many_blocks + 2 * few_ctas), dim3(32 * kWarps), 0, s, true, dim3(1, 1, 1), many, few,
+                   many_blocks, few_rows);
 }
 
 }  // namespace
 
-cudaError_t attn_combine_launch(const AttnDev& p, bool f16, int ctas, int tile_rows, cudaStream_t s) {
-  if (p.c.head_dim == 128)
-    return f16 ? combine<__half, 128>(p, ctas, tile_rows, s) : combine<__nv_bfloat16, 128>(p, ctas, tile_rows, s);
-  return f16 ? combine<__half, 64>(p, ctas, tile_rows, s) : combine<__nv_bfloat16, 64>(p, ctas, tile_rows, s);
+cudaError_t attn_combine_launch(const AttnDev& many, const AttnDev& few, bool f16, int many_ctas, int few_ctas, int few_rows, cudaStream_t s) {
+  if (many.c.head_dim == 128)
+    return f16 ? combine<__half, 128>(many, few, many_ctas, few_ctas, few_rows, s) : combine<__nv_bfloat16, 128>(many, few, many_ctas, few_ctas, few_rows, s);
+  return f16 ? combine<__half, 64>(many, few, many_ctas, few_ctas, few_rows, s) : combine<__nv_bfloat16, 64>(many, few, many_ctas, few_ctas, few_rows, s);
 }
 
 }  // namespace llg

@@ -148,8 +148,9 @@ cudaError_t attn_rows_launch_bf16(const AttnDev& p, const CUtensorMap& k, const 
 cudaError_t attn_rows_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_tiles_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
-// ctas: those of the kernel that left the partial results; tile_rows: rows of one of its tiles.
-cudaError_t attn_combine_launch(const AttnDev& p, bool f16, int ctas, int tile_rows, cudaStream_t s);
+// Adds up what the tile kernel's `many_ctas` and the few-row kernel's `few_ctas` CTAs (tiles of few_rows rows) left; 0 for a kernel
+// that did not run, whose descriptor is then only the other's.
+cudaError_t attn_combine_launch(const AttnDev& many, const AttnDev& few, bool f16, int many_ctas, int few_ctas, int few_rows, cudaStream_t s);
 
 // ---- block-scale layouts (relayout.cu) ---------------------------------------------------------------------------
 // Row-major [rows, cols] bytes (row pitch ld) <-> tiles of 128 rows x 4 columns, 512 bytes each, padded to whole tiles.
