@@ -88,7 +88,7 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
   p.lse_tok = a.lse_stride;
   p.group = a.heads / a.kv.kv_heads;
   p.causal = a.causal != 0;
-  p.window = a.window;
+  p.window = a.window < (1 << 30) ? a.window : 1 << 30;  // no cache is longer, and positions less this stay in 32 bits
   const bool fp8 = a.kv.dtype == LLG_DT_E4M3, f16 = a.q_dtype == LLG_DT_F16;
   const float scale_log2 = a.scale * 1.44269504088896341f;
   unsigned char* const ws = static_cast<unsigned char*>(a.ws);

@@ -191,7 +191,7 @@ __device__ __forceinline__ void combine_tiles(const AttnDev& p, int cta, int e, 
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (ml[k].x == -INFINITY) continue;  // no keys: the part has no sums
+        if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // no keys: the part has no sums (without a maximum but with a sum: NaN)
         const float v[8] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w, x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
         add(ml[k].x, ml[k].y, v);
       }
@@ -205,7 +205,7 @@ __device__ __forceinline__ void combine_tiles(const AttnDev& p, int cta, int e, 
       __syncthreads();
       if (warp != 0) continue;
       for (int w = 1; w < kWarps; ++w) {
-        if (state[w][8][lane] == -INFINITY) continue;
+        if (state[w][8][lane] == -INFINITY && state[w][9][lane] == 0.f) continue;
         float v[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) v[d] = state[w][d][lane];

@@ -3,19 +3,19 @@
 //   s = scale * q . k,  m = max s,  l = sum exp(s - m),  o = sum exp(s - m) v / l       one pass, running m, l and o
 //
 // Key tiles of 64 tokens (128: e4m3, up to 8 rows, which halves what is spent per key beside the products); each of the CTA's four
-// warps owns 16 (32) of them with its own ring of stages, softmax state and
-// accumulators, so nothing between the loads and the last merge synchronises more than a warp. Sixteen rows that are all there and
-// share a page come by TMA, swizzled; others are gathered with cp.async, zeros for the missing. The products are taken
-// transposed, S^T[16 keys x rows] = K Q^T and O^T[head_dim x rows] = V^T P^T, so that the rows - 8 for a group of eight heads
-// and one token - are the narrow side (8) of mma.m16n8k16 and no row of the tensor-core tile is padding.
+// warps owns 16 (32) of them with its own ring of stages, softmax state and accumulators, so nothing between the loads and the last
+// merge synchronises more than a warp. Sixteen rows that are all there and share a page come by TMA, swizzled; others are gathered
+// with cp.async, zeros for the missing. The products are taken transposed, S^T[16 keys x rows] = K Q^T and
+// O^T[head_dim x rows] = V^T P^T, so that the rows - 8 for a group of eight heads and one token - are the narrow side (8) of
+// mma.m16n8k16 and no row of the tensor-core tile is padding.
 //   16-bit cache: K by ldmatrix, V by ldmatrix.trans.
 //   e4m3 cache: 16-byte reads of a row give a thread 16 neighbouring values; the order of head_dim inside a product is free, so
 //     they serve four consecutive k steps of K Q^T (Q is read in the same order) and eight row blocks of V^T without any
 //     transposition, and so are the orders of the keys and of head_dim's blocks among the lanes, which keep the reads of the
-//     TMA's swizzle free of bank conflicts. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's type is: a bf16 row of
-//     q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less lose bits). The scores
-//     take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the running maximum is that of
-//     s + e, so p 2^e <= 2^8 and keeps f16's 11 bits where it matters.
+//     TMA's swizzle free of bank conflicts. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's
+//     type is: a bf16 row of q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less
+//     lose bits). The scores take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the
+//     running maximum is that of s + e, so p 2^e <= 2^8 and keeps f16's 11 bits where it matters.
 // P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
 // The running maximum moves only when a score exceeds it by more than 2^8: p <= 256 then, and the shuffles and the rescaling of
 // O are skipped for almost every tile.
@@ -104,39 +104,24 @@ struct Mma<__half> {
   }
 };
 
-// Two e4m3 bytes of `w` (picked by the byte-permutation selectors of w and v) as a pair of 16-bit operands.
-// bf16: value * 2^-120.  f16: the value.
-template <typename T>
-struct Widen;
-template <>
-struct Widen<__nv_bfloat16> {
-  // bytes 1 and 3 of `w` -> bf16 pair
-  static __device__ __forceinline__ uint32_t odd(uint32_t w) { return ((w & 0x7f007f00u) >> 4) | (w & 0x80008000u); }
-  static __device__ __forceinline__ void four(uint32_t w, uint32_t& lo, uint32_t& hi) {  // bytes 0,1 -> lo; 2,3 -> hi
-    lo = odd(__byte_perm(w, 0u, 0x1404));
-    hi = odd(__byte_perm(w, 0u, 0x3424));
-  }
-};
-template <>
-struct Widen<__half> {
-  static __device__ __forceinline__ uint32_t pair(uint32_t v) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
-    return r;
-  }
-  static __device__ __forceinline__ void four(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = pair(w & 0xffffu);
-    hi = pair(w >> 16);
-  }
-  // (a.b0, b.b0) (a.b1, b.b1) (a.b2, b.b2) (a.b3, b.b3)
-  static __device__ __forceinline__ void cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
-    const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
-    o[0] = pair(x & 0xffffu);
-    o[1] = pair(x >> 16);
-    o[2] = pair(y & 0xffffu);
-    o[3] = pair(y >> 16);
-  }
-};
+// e4m3 bytes as pairs of f16, which holds every one of their values.
+__device__ __forceinline__ uint32_t widen2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+  return r;
+}
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  lo = widen2(w & 0xffffu);
+  hi = widen2(w >> 16);
+}
+// (a.b0, b.b0) (a.b1, b.b1) (a.b2, b.b2) (a.b3, b.b3)
+__device__ __forceinline__ void widen_cross(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
+  const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
+  o[0] = widen2(x & 0xffffu);
+  o[1] = widen2(x >> 16);
+  o[2] = widen2(y & 0xffffu);
+  o[3] = widen2(y >> 16);
+}
 
 __device__ __forceinline__ float pow2_of(uint32_t biased) { return __uint_as_float(biased << 23); }
 
@@ -422,8 +407,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t a[4];
-              Widen<Op>::four(w0[j], a[0], a[2]);
-              Widen<Op>::four(w1[j], a[1], a[3]);
+              widen4(w0[j], a[0], a[2]);
+              widen4(w1[j], a[1], a[3]);
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
                 if (nb < nb_used) Mma<Op>::run(s[u][nb], a, qf[nb][4 * i + j][0], qf[nb][4 * i + j][1]);
@@ -533,8 +518,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             uint32_t lo[4], hi[4];
-            Widen<Op>::cross(w[0][j], w[1][j], lo);
-            Widen<Op>::cross(w[2][j], w[3][j], hi);
+            widen_cross(w[0][j], w[1][j], lo);
+            widen_cross(w[2][j], w[3][j], hi);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};

@@ -5,12 +5,11 @@
 //   S = Q K^T   tcgen05.mma 128 x 128, both operands in shared memory (K-major, 128-byte swizzle)
 //   P           softmax in registers, one thread per row: no shuffles; P goes back over S in tensor memory, 16 bit
 //   O += P V    tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (rows of head_dim: MN-major B)
-// Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). Warps 0-3 and 4-7: softmax of A and B; 8-11:
-// loaders; 12: MMA issue; 13:
-// the walk, published as segments in shared memory; 14, 15: fetch e4m3 rows for the loaders to widen (or fill the warpgroup: registers move between warpgroups, so that a
-// row of 128 scores stays in the softmax threads). While one stream's softmax runs, the other stream's products do: per key tile and stream the tensor
-// core needs 2 x 128 x 128 x head_dim / 4096 cycles (1024 at head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the
-// two streams alternate between units that are equally busy.
+// Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). Warps 0-3 and 4-7: softmax of A and B; 8-11: loaders;
+// 12: MMA issue; 13: the walk, published as segments in shared memory; 14, 15: fetch e4m3 rows for the loaders to widen, or fill the
+// warpgroup: registers move between warpgroups, so that a row of 128 scores stays in the softmax threads. While one stream's softmax
+// runs, the other stream's products do: per key tile and stream the tensor core needs 2 x 128 x 128 x head_dim / 4096 cycles (1024 at
+// head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the two streams alternate between units that are equally busy.
 // Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
 // even key tiles, B the odd ones, and each leaves a partial result of its own.
 // The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Widen<__half>::four(w[j], o[2 * j], o[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) widen4(w[j], o[2 * j], o[2 * j + 1]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) *reinterpret_cast<__half2*>(&o[j]) = __hmul2(*reinterpret_cast<__half2*>(&o[j]), f);
         const uint32_t at0 = dst + (ch >> 2) * Cfg::kHalf + row * 128;
@@ -775,7 +774,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           f_bytes = ref.y;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            cq[q] = c_row * pow2_of((ref.x >> (8 * q)) & 0xffu);
+            // not 0, which would make NaN of a masked column's -inf (a row of zeros against rows of zeros: 2^-121 * 2^-100)
+            cq[q] = fmaxf(c_row * pow2_of((ref.x >> (8 * q)) & 0xffu), 1.17549435e-38f);
             fq[q] = __uint_as_float(0x4b000000u + ((ref.y >> (8 * q)) & 0xffu)) - 8388735.f;  // F: bits of 2^23 + byte, less 2^23 + 127
           }
         } else {

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     if (lane == 0) {
       if (seq < c.batch && (!c.starts || t >= c.starts[seq])) {  // seq == batch: behind the last sequence
         const int end = c.starts ? min(c.starts[seq + 1], c.tokens) : (seq + 1) * c.q_len;
-        const int pos = c.lens[seq] - end + t;
+        const int pos = max(c.lens[seq], 0) - end + t;
         if (pos >= 0) {
           int block;
           split_key(c, pos, block, w.slot);

@@ -94,7 +94,7 @@ def reference(q, kc, vc, ks, vs, table, lens, starts, scale, causal, window):
         # products and sums over keys 2^-24 each), and the error of a score - a dot product of dim fp32 products and sums,
         # 2^-24 each of sum |q||k| - which moves a weight by twice its size; exp2 adds 2^-21
         mass = torch.einsum("thj,jhd->thd", w, v.abs())
-        score = (torch.einsum("thd,jhd->thj", qq.abs(), k.abs()) * scale).amax(-1, keepdim=True) if length else torch.zeros_like(top)
+        score = (torch.einsum("thd,jhd->thj", qq.abs(), k.abs()) * abs(scale)).amax(-1, keepdim=True) if length else torch.zeros_like(top)
         delta = score * (dim + 4) * 2.0 ** -24 + 2.0 ** -21
         tol[t0:t1] = half * o[t0:t1].abs() + mass * (half + 2 * delta + length * 2.0 ** -24) + torch.finfo(q.dtype).tiny
     return o, lse, tol
@@ -228,6 +228,114 @@ def test_smallest_and_largest_row_scales():
     q = torch.randn(1, 8, 128, generator=g).to(BF).cuda()
     out = L.paged_attention(q, kc, vc, table, torch.tensor([200], dtype=torch.int32, device="cuda"), k_scale=ks, v_scale=vs)
     want, _, tol = reference(q, kc, vc, ks, vs, table, [200], [0, 1], 128 ** -0.5, True, 0)
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales_that_are_not_positive(scale, ct):
+    for news, lens in (([1, 1], [70, 500]), ([90, 2], [300, 150])):
+        check(news, lens, 8, 1, 128, 16, BF, E4M3 if ct == "e4m3" else BF, scale=scale)
+        check(news, lens, 8, 2, 64, 16, HF, E4M3 if ct == "e4m3" else HF, scale=scale)
+
+
+@pytest.mark.parametrize("loud", [0.0, 1e-30, 1e-12])
+def test_queries_of_zeros_and_near_them(loud):
+    """The factors of a bf16 row of q and of a quarter tile without rows are tiny together; masked keys stay masked."""
+    for news, lens in (([1, 1], [70, 500]), ([90, 2], [301, 150]), ([40], [3001])):
+        for ct in (BF, E4M3):
+            check(news, lens, 8, 1, 128, 16, BF, ct, loud=loud)
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+@pytest.mark.parametrize("page", [8, 24, 40, 96])
+def test_chunks_over_pages_of_any_size(page, ct):
+    """Boxes of 8 and 32 rows, and pages that no box fits."""
+    check([70, 1], [300, 90], 8, 2, 128, page, BF, E4M3 if ct == "e4m3" else BF, seed=page)
+    check([33], [1500], 4, 1, 64, page, HF, E4M3 if ct == "e4m3" else HF, seed=page)
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+def test_rows_between_the_kernels(ct):
+    """9 to 32 query rows per kv head, uniform and ragged, and groups of 32."""
+    for new in (2, 3, 4, 5):
+        check([new] * 3, [30, 300, 1000], 8, 1, 128, 16, BF, E4M3 if ct == "e4m3" else BF, seed=new)
+        check([new] * 3, [30, 300, 1000], 8, 1, 64, 16, HF, E4M3 if ct == "e4m3" else HF, ragged=True, seed=new)
+    check([1, 5, 40], [100, 300, 90], 32, 1, 128, 16, BF, E4M3 if ct == "e4m3" else BF)
+    check([2, 3], [100, 300], 48, 2, 128, 16, BF, E4M3 if ct == "e4m3" else BF)
+
+
+def test_more_sequences_than_threads():
+    news = [(i % 3) if i % 97 else 45 for i in range(700)]
+    check(news, [n + (31 * i) % 157 for i, n in enumerate(news)], 8, 1, 64, 16, BF, BF)
+
+
+def test_windows_wider_than_any_cache():
+    for news, lens in (([5], [2]), ([90], [20]), ([1, 60], [300, 400])):
+        for window in (2 ** 31 - 1, 2 ** 30, 2 ** 30 - 1):
+            check(news, lens, 8, 1, 128, 16, BF, BF, window=window, width=32)
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+@pytest.mark.parametrize("news,lens", [([1], [20000]), ([2, 70], [900, 9000]), ([40], [9000]), ([300, 1], [700, 40])])
+def test_a_nan_query_stays_a_nan_and_alone(news, lens, ct):
+    """Also where several CTAs share its sequence and no part has a maximum."""
+    ct = E4M3 if ct == "e4m3" else BF
+    table, pages = pages_for(lens, 16, 11)
+    kc, vc, ks, vs = make_cache(pages, 1, 16, 128, ct, 12)
+    g = torch.Generator().manual_seed(13)
+    q = torch.randn(sum(news), 4, 128, generator=g).to(BF).cuda()
+    starts = torch.tensor([sum(news[:i]) for i in range(len(news) + 1)], dtype=torch.int32, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want, wl = L.paged_attention(q, kc, vc, table, ln, q_starts=starts, k_scale=ks, v_scale=vs, return_lse=True)
+    bad = q.clone()
+    bad[-1, 2, 5] = math.nan
+    got, gl = L.paged_attention(bad, kc, vc, table, ln, q_starts=starts, k_scale=ks, v_scale=vs, return_lse=True)
+    assert bool(got[-1, 2].isnan().all()) and bool(gl[-1, 2].isnan())
+    want[-1, 2], wl[-1, 2] = got[-1, 2], gl[-1, 2]
+    assert torch.equal(want.view(torch.int16), got.view(torch.int16)) and torch.equal(wl.view(torch.int32), gl.view(torch.int32))
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+@pytest.mark.parametrize("news,lens", [([1, 1], [70, 500]), ([90, 2], [300, 150])])
+def test_keys_and_values_in_one_allocation(news, lens, ct):
+    """Strided views of one tensor, scale rows that are not contiguous, and a strided output: the same results."""
+    ct = E4M3 if ct == "e4m3" else BF
+    table, pages = pages_for(lens, 16, 21)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, 128, ct, 22)
+    both = torch.stack([kc.view(torch.uint8), vc.view(torch.uint8)], 1)
+    kv = [both[:, i].view(ct) for i in range(2)]
+    scales = [None, None]
+    if ks is not None:
+        s = torch.stack([ks.view(torch.uint8), vs.view(torch.uint8)], 3)
+        scales = [s[..., i].view(E8M0) for i in range(2)]
+    g = torch.Generator().manual_seed(23)
+    q = torch.randn(sum(news), 8, 128, generator=g).to(BF).cuda()
+    starts = torch.tensor([sum(news[:i]) for i in range(len(news) + 1)], dtype=torch.int32, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = L.paged_attention(q, kc, vc, table, ln, q_starts=starts, k_scale=ks, v_scale=vs)
+    wide = torch.full((sum(news), 10, 128), 7.0, dtype=BF, device="cuda")
+    L.paged_attention(q, *kv, table, ln, q_starts=starts, k_scale=scales[0], v_scale=scales[1], out=wide[:, 1:9])
+    assert torch.equal(wide[:, 1:9], want) and bool((wide[:, ::9] == 7.0).all())
+
+
+@pytest.mark.parametrize("qt", [BF, HF])
+@pytest.mark.parametrize("new", [1, 70])
+def test_row_scales_far_apart(new, qt):
+    """Neighbouring rows whose powers of two differ by up to 2^16: the tile kernel keeps a row's value times 2^-d, d up to 16 below
+    the quarter's largest, in f16, whose smallest step is 2^-24 - an error of 2^-25 of the quarter's power of two per element."""
+    table, pages = pages_for([700], 16, 31)
+    kc, vc, ks, vs = make_cache(pages, 1, 16, 128, E4M3, 32)
+    g = torch.Generator().manual_seed(33)
+    for s in (ks, vs):
+        s.view(torch.uint8).copy_(torch.randint(108, 125, s.shape, generator=g).to(torch.uint8))
+    q = torch.randn(new, 4, 128, generator=g).to(qt).cuda()
+    out = L.paged_attention(q, kc, vc, table, torch.tensor([700], dtype=torch.int32, device="cuda"), k_scale=ks, v_scale=vs)
+    want, _, tol = reference(q, kc, vc, ks, vs, table, [700], [0, new], 128 ** -0.5, True, 0)
+    # 2^-3 is the largest power (byte 124): a score is off by sum|q| 2^-28 / sqrt(128), which moves a weight by twice that; V by 2^-28
+    shift = q.double().abs().sum(-1, keepdim=True) * 2.0 ** -28 / 128 ** 0.5
+    v = rows_of(vc, vs, table, 0, 700).abs().amax()
+    tol = tol + 2 * shift * v + 2.0 ** -28
     assert bool(((out.double() - want).abs() <= tol).all())
 
 
