@@ -195,6 +195,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   bool gathered = false;        // copies of cp.async went into the ring since the last proxy fence
   bool ok_all = true;
   const PagedKV& c = p.c;
+  // row / group for rows of a tile: exact while row * group < 2^16
+  const uint32_t group_inv = (65535u + p.group) / p.group;
+  auto token_of = [&](int row) { return (int)((uint32_t)row * group_inv >> 16); };
   const bool one_page = c.page_size % 16 == 0;  // 16 keys from a multiple of 16 on share a page
 
   Segment g;
@@ -211,28 +214,61 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
     const int all_hi = p.causal ? min(pos0, g.s.len - 1) : g.s.len - 1;
     const int all_lo = p.window > 0 ? pos0 + g.toks - p.window : 0;
     auto key_of = [&](int t) { return (g.tile0 + t) * KT + warp * (16 * SUB); };
-    // The tile located last, where 16 keys from a multiple of 16 on share a page: the lane's group (lane % SUB), its page (-1: none)
-    // and first slot; the page table's entry is requested a tile ahead.
-    const int sub = lane % SUB;
-    int pg = -1, at = 0, entry = INT_MIN;
-    auto enter = [&](int t) {
-      const int k0 = key_of(t) + 16 * sub;
+    // Where 16 keys from a multiple of 16 on share a page: page table entries of the warp's next 32 groups, one per lane, and of the
+    // 32 behind them, on their way. A request per tile would make a chain of them: filling a ring of seven stages took 3 us.
+    constexpr int kLook = 32 / SUB;             // tiles
+    auto look_up = [&](int t0) {
+      const int t = t0 + lane / SUB, k0 = key_of(t) + 16 * (lane % SUB);
       int block, slot;
       split_key(c, k0, block, slot);
-      entry = t < nt && k0 < g.keys.hi && k0 + 16 > g.keys.lo ? table_row[block] : INT_MIN;
+      return t < nt && k0 < g.keys.hi && k0 + 16 > g.keys.lo ? table_row[block] : INT_MIN;
     };
+    int entries = INT_MIN, ahead = INT_MIN;
+    if (one_page) {
+      entries = look_up(0);
+      ahead = look_up(kLook);
+    }
+    // the tile located last: the lane's group (lane % SUB), its page (-1: none) and first slot; tiles are located in order
+    const int sub = lane % SUB;
+    int pg = -1, at = 0;
     auto locate = [&](int t) {
       if (!one_page) return;
+      if (t % kLook == 0 && t > 0) {
+        entries = ahead;
+        ahead = look_up(t + kLook);
+      }
       int block;
       split_key(c, key_of(t) + 16 * sub, block, at);
-      pg = entry;
-      enter(t + 1);
+      pg = __shfl_sync(0xffffffffu, entries, t % kLook * SUB + sub);
       if ((unsigned)pg >= (unsigned)c.pages) {
         if (pg != INT_MIN) atomicCAS(c.status, 0u, (unsigned)ST_BAD_PAGE);
         pg = -1;
       }
     };
-    if (one_page) enter(0);
+
+    // ---- queries: B fragments of K Q^T, row oct of each block; requested before the ring is filled
+    uint32_t qf[NB][KS][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = nb * 8 + oct;
+      const int tok = token_of(row), hh = row - tok * p.group;
+      const unsigned char* src = p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint2 v = make_uint2(0u, 0u);
+        if (row < rows) {
+          if constexpr (FP8) {  // the order in which a thread holds a row of K: 16 * (quad + 4 i) + 4 j
+            const int i = ks >> 2, j = ks & 3;
+            v = *reinterpret_cast<const uint2*>(src + 2 * (16 * (quad + 4 * i) + 4 * j));
+          } else {
+            v.x = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad));
+            v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
+          }
+        }
+        qf[nb][ks][0] = v.x;
+        qf[nb][ks][1] = v.y;
+      }
+    }
     const bool by_tma = one_page && p.box != 0;
     auto issue = [&](int t) {  // starts the copies of tile t, located by the call before, into stage `put`
       if (t >= nt) return;
@@ -304,37 +340,18 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       }
       put = put + 1 == S ? 0 : put + 1;
     };
+#pragma unroll 1
     for (int t = 0; t < S - 1; ++t) {
       locate(t);
       issue(t);
     }
     locate(S - 1);
 
-    // ---- queries: B fragments of K Q^T, row oct of each block
-    uint32_t qf[NB][KS][2];
+    // ---- what the rows see, and bf16 queries to f16
     float row_f[NB][2];                     // what turns a product of those rows into log2 units
     int first_key[NB][2], last_key[NB][2];  // keys that rows 2 * quad, 2 * quad + 1 of a block see: [first, last]
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int row = nb * 8 + oct;
-      const bool ok = row < rows;
-      const int tok = row / p.group, hh = row - tok * p.group;
-      const unsigned char* src = p.q + (int64_t)(g.s.t0 + g.tok0 + tok) * p.q_tok + (int64_t)(g.head * p.group + hh) * p.q_head;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        uint2 v = make_uint2(0u, 0u);
-        if (ok) {
-          if constexpr (FP8) {  // the order in which a thread holds a row of K: 16 * (quad + 4 i) + 4 j
-            const int i = ks >> 2, j = ks & 3;
-            v = *reinterpret_cast<const uint2*>(src + 2 * (16 * (quad + 4 * i) + 4 * j));
-          } else {
-            v.x = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad));
-            v.y = *reinterpret_cast<const uint32_t*>(src + 2 * (16 * ks + 2 * quad + 8));
-          }
-        }
-        qf[nb][ks][0] = v.x;
-        qf[nb][ks][1] = v.y;
-      }
       float mine = p.scale_log2;              // of row oct
       if constexpr (kToF16) {
         float top = 0.f;
@@ -362,7 +379,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       for (int e = 0; e < 2; ++e) {
         row_f[nb][e] = __shfl_sync(0xffffffffu, mine, (2 * quad + e) * 4);
         const int r = nb * 8 + 2 * quad + e;
-        const int pos = pos0 + r / p.group;
+        const int pos = pos0 + token_of(r);
         last_key[nb][e] = r < rows ? (p.causal ? min(pos, g.s.len - 1) : g.s.len - 1) : -1;
         first_key[nb][e] = p.window > 0 ? pos - p.window + 1 : 0;
       }
@@ -590,7 +607,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       }
       if (g.whole) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int tok = row / p.group, head = g.head * p.group + row - tok * p.group;
+        const int tok = token_of(row), head = g.head * p.group + row - tok * p.group;
         const int64_t t = g.s.t0 + g.tok0 + tok;
         *reinterpret_cast<uint2*>(p.out + t * p.o_tok + head * p.o_head + 2 * d) =
             make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));

@@ -638,3 +638,33 @@ def test_refusals():
         rd(kc, kc, table, ln, -1)
     refused("must both be bfloat16", att, q, kc.float(), kc.float(), table, ln)
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("ct", [BF, E4M3])
+def test_offsets_beyond_32_bits(ct):
+    """Pages more than 4 GiB into the cache: the same bits as from a small one."""
+    heads, page, dim = 2, 64, 128
+    row = dim * ct.itemsize
+    pages = (5 << 30) // (heads * page * row)
+    far = torch.tensor([[pages - 1, pages - 5, pages - 2], [pages - 4, 1, pages - 3]], dtype=torch.int32, device="cuda")
+    near = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([150, 131], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(41)
+    kv = torch.randn(2 * 131, 2 * heads, dim, generator=g).to(BF).cuda()
+    q = torch.randn(2 * 131, 8, dim, generator=g).to(BF).cuda()
+    results = []
+    for table, n in ((near, 6), (far, pages)):
+        kc, vc = (torch.zeros if n == 6 else torch.empty)((2, n, heads, page, dim), dtype=ct, device="cuda").unbind(0)
+        scales = {}
+        if ct == E4M3:
+            ks, vs = torch.empty(2, n, heads, page, dtype=torch.uint8, device="cuda").view(E8M0).unbind(0)
+            scales = dict(k_scale=ks, v_scale=vs)
+        first = torch.full((2,), 19, dtype=torch.int32, device="cuda")  # then 131 new ones reach lengths of 150 and 131
+        L.kv_append(kv[:38, :heads], kv[:38, heads:], kc, vc, table, first, **scales)
+        L.kv_append(kv[:, :heads], kv[:, heads:], kc, vc, table, lens, **scales)
+        results.append([L.paged_attention(q, kc, vc, table, lens, **scales), L.paged_attention(q[:2], kc, vc, table, lens, **scales),
+                        *L.kv_read(kc, vc, table, lens, 150, **scales)])
+        del kc, vc, scales
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert N.device_status() == 0
