@@ -52,7 +52,7 @@ Plan plan_of(const llg_attn_args& a) {
   p.many = most > widest;
   if (p.few) {
     const int64_t rows = most < widest ? most : widest;
-    const int blocks = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    const int blocks = (int)(rows + 7) / 8;
     p.f.row_max = (int)widest;
     p.f.tok_tile = blocks * 8 / group;
     p.units = (int64_t)c.batch * c.kv_heads * ((keys + 63) / 64 + 1);  // one tile per sequence

@@ -225,7 +225,7 @@ __device__ __forceinline__ void combine_tiles(const AttnDev& p, int cta, int e, 
 
 // Both kernels' items in one launch: first those of the tile kernel's CTAs, then those of the few-row kernel's.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kWarps) attn_combine_kernel(const __grid_constant__ AttnDev many, const __grid_constant__ AttnDev few,
+__global__ void __launch_bounds__(32 * kWarps, 4) attn_combine_kernel(const __grid_constant__ AttnDev many, const __grid_constant__ AttnDev few,
                                                                    int many_blocks, int few_rows) {
   __shared__ union {
     float part[kWarps][D + 2];

@@ -19,11 +19,12 @@ cudaError_t attn_rows_blocks(const AttnDev& p, const CUtensorMap& k, const CUten
   switch (blocks) {
     case 1: return attn_rows_start<T, FP8, D, 1>(p, k, v, ctas, pdl, s);
     case 2: return attn_rows_start<T, FP8, D, 2>(p, k, v, ctas, pdl, s);
+    case 3: return attn_rows_start<T, FP8, D, 3>(p, k, v, ctas, pdl, s);
     default: return attn_rows_start<T, FP8, D, 4>(p, k, v, ctas, pdl, s);
   }
 }
 
-// blocks: 1, 2 or 4 blocks of eight rows per tile.
+// blocks: 1 to 4 blocks of eight rows per tile.
 template <typename T>
 cudaError_t attn_rows_dispatch(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s) {
   if (p.c.head_dim == 128) return fp8 ? attn_rows_blocks<T, true, 128>(p, k, v, blocks, ctas, pdl, s) : attn_rows_blocks<T, false, 128>(p, k, v, blocks, ctas, pdl, s);
