@@ -310,7 +310,7 @@ typedef struct llg_kv_append_args {
 LLG_API int llg_kv_append(const llg_kv_append_args* args, void* stream);
 
 /* Reads the first max_len tokens of every sequence back: k_out and v_out [batch, max_len, kv_heads, head_dim], contiguous,
- * zero behind kv_lens[i]. kv.q_starts and kv.tokens are not used. out_dtype: the cache's for BF16 / F16; BF16, F16 or F32 for E4M3. */
+ * zero behind kv_lens[i]; at most 65535 sequences. kv.q_starts and kv.tokens are not used. out_dtype: the cache's for BF16 / F16; BF16, F16 or F32 for E4M3. */
 typedef struct llg_kv_read_args {
   llg_paged_kv kv;
   void* k_out; void* v_out;
@@ -324,8 +324,10 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * sees key j when j <= position (causal) and j > position - window (window > 0); scores are scale * q . k, o = softmax v,
  * lse = log of the sum of exp(scores) (natural, fp32). A query that sees no key gives o = 0 and lse = -inf.
  * head_dim 64 or 128; q and out in the cache's 16-bit type, or either 16-bit type over E4M3; heads / kv_heads <= 32.
- * With F16 queries an E4M3 value is used as F16 (its row's power of two applied). ws: llg_paged_attention_ws() bytes of
- * scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
+ * An E4M3 value is multiplied as F16 whatever q's type is, its row's power of two kept apart where one kv head has few query rows
+ * and relative to the largest of 32 neighbouring rows where it has many: rows 2^-15 below that largest then lose bits, rows 2^-24
+ * below count as zeros. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits. ws:
+ * llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
 typedef struct llg_attn_args {
   llg_paged_kv kv;
   const void* q; int64_t q_stride[2];            /* token, head; elements, multiples of 16 bytes */
@@ -338,8 +340,10 @@ typedef struct llg_attn_args {
 } llg_attn_args;
 
 LLG_API int llg_paged_attention(const llg_attn_args* args, void* stream);
-/* Bytes of scratch llg_paged_attention needs for these arguments on the current device (ws itself is not looked at); at most
- * a few megabytes per device, whatever the lengths are. Negative: LLG_E_*. */
+/* Bytes of scratch llg_paged_attention needs for these arguments on the current device (ws itself is not looked at): two partial
+ * results per CTA, whatever the lengths are - up to 39 MB on 148 SMs where a kv head has many query rows, 10 MB where it has few.
+ * Negative: LLG_E_*, also for calls of more key tiles (of 64 tokens, table_width * page_size of them per sequence and kv head) than
+ * 31 bits count. */
 LLG_API int64_t llg_paged_attention_ws(const llg_attn_args* args);
 
 /* sizeof of llg_paged_kv, llg_kv_append_args, llg_kv_read_args, llg_attn_args as this library was compiled. */

@@ -13,6 +13,9 @@ Two engines behind one call: a CUDA-core streaming GEMV for W16A16 with at most 
 and a TMA-fed tcgen05 tensor-core kernel with tensor-memory accumulators for every precision and any M. A plan per
 (precision, N, K) picks engine and tiling per M. All compute runs in libllg_core.so (hand-written CUDA, C ABI in
 include/llg_core.h); nothing falls back to the CPU or to a vendor GEMM.
+
+Between the projections: kv_append, kv_read and paged_attention serve a paged key/value cache (bf16, f16, or e4m3 with a power
+of two per row) and the attention over it; see lowlat_gemm.attention.
 """
 
 from .api import (_FP4_KINDS, _workspace, _ws, gemm, kind_of, pdl_enabled, quantize_fp8, quantize_int8,  # noqa: F401

@@ -57,7 +57,8 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tens
         raise ValueError(f"lowlat_gemm: max_len must not be negative, got {max_len}")
     e4m3 = k_cache.dtype == torch.float8_e4m3fn
     dtype = out_dtype or (torch.bfloat16 if e4m3 else k_cache.dtype)
-    k, v = torch.empty((2, kv_lens.shape[0], max_len, k_cache.shape[1], k_cache.shape[3]), dtype=dtype, device=k_cache.device).unbind(0)
+    k = k_cache.new_empty((kv_lens.shape[0], max_len, k_cache.shape[1], k_cache.shape[3]), dtype=dtype)
+    v = torch.empty_like(k)
     _read(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens)
     return k, v
 
