@@ -6,8 +6,6 @@
 namespace llg {
 namespace {
 
-// Sequences with more query rows (new tokens * heads per kv head) than this go to the tile kernel.
-constexpr int kRowsMax = 32;
 constexpr int kTileRows = 256;
 
 struct Part {  // one kernel's CTAs and scratch
@@ -42,13 +40,14 @@ Plan plan_of(const llg_attn_args& a) {
   const int group = a.heads / c.kv_heads, sms = sm_count();
   const int64_t most = c.q_starts ? (int64_t)c.tokens * group : (int64_t)(c.tokens / c.batch) * group;
   const int64_t keys = (int64_t)c.table_width * c.page_size;
-  // With offsets the few-row kernel takes the sequences of one token (of a few, where the group is small), in tiles no wider than
-  // that: wider ones would hold registers that decoding sequences do not use. Without, tiles as wide as the rows.
-  // 17 to 32 rows of a 16-bit cache with head_dim 128 fill the few-row kernel's registers and run faster as tiles (16 sequences of
-  // 1.2k to 2.5k keys, 32 rows: 78 us against 49); narrower or e4m3 rows do not (39.5 against 40.5; 45 against 63).
-  const int64_t fit = c.head_dim == 128 && c.dtype != LLG_DT_E4M3 && group <= 16 ? 16 : kRowsMax;
-  const int64_t widest = c.q_starts ? (group <= 8 ? 8 : group <= 16 ? 16 : 32) : fit;
-  p.few = c.q_starts || most <= widest;
+  // Rows per kv head that the few-row kernel takes. 25 to 32 rows of head_dim 128 fill its registers and run faster as tiles, fewer
+  // and narrower ones do not (16 sequences of 1.2k to 2.5k keys, few-row kernel against tiles, us: 32 rows of 128 16-bit values 76
+  // and 50.5, e4m3 78 and 69; 24 rows 44 and 50.5, 46 and 69; 32 rows of 64 values 38 and 41, 42 and 51).
+  const int64_t fit = c.head_dim == 128 ? 24 : 32;
+  // With offsets it takes the sequences of one token (of a few, where the group is small), in tiles no wider than that: wider ones
+  // would hold registers that decoding sequences do not use. Without, tiles as wide as the rows.
+  const int64_t widest = c.q_starts ? (group <= 8 ? 8 : group <= 16 ? 16 : fit) : fit;
+  p.few = group <= widest && (c.q_starts || most <= widest);
   p.many = most > widest;
   if (p.few) {
     const int64_t rows = most < widest ? most : widest;

@@ -1,7 +1,8 @@
 // Adds the partial results of items that several CTAs shared: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the order
 // of the CTAs. Bound by the latency of reading a few kilobytes back from L2. The CTAs of the main kernel that shared an item are
 // also the indexes of those that add it up here, each its part of the rows: a long sequence of few heads, with a part from every
-// SM, so has all SMs at work, two parts have two. A CTA with fewer rows than warps puts several warps on a row.
+// SM, so has all SMs at work, two parts have two. A CTA with fewer rows than warps puts several warps on a row. One launch serves both
+// kernels (two cost a ragged batch 2.5 us), in 64 registers: four CTAs per SM took 1.5 us less than three behind 296 CTAs.
 #include "paged_kv.cuh"
 
 namespace llg {

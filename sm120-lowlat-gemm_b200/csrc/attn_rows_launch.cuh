@@ -20,7 +20,7 @@ cudaError_t attn_rows_blocks(const AttnDev& p, const CUtensorMap& k, const CUten
     case 1: return attn_rows_start<T, FP8, D, 1>(p, k, v, ctas, pdl, s);
     case 2: return attn_rows_start<T, FP8, D, 2>(p, k, v, ctas, pdl, s);
     case 3: return attn_rows_start<T, FP8, D, 3>(p, k, v, ctas, pdl, s);
-    default: return attn_rows_start<T, FP8, D, 4>(p, k, v, ctas, pdl, s);
+    default: return attn_rows_start<T, FP8, D, D == 64 ? 4 : 3>(p, k, v, ctas, pdl, s);  // head_dim 128 has no more than 24 rows here
   }
 }
 

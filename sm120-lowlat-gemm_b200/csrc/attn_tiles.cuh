@@ -24,6 +24,8 @@
 // its quarters times 2^-F.
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
+// Measured, 64 heads over 8, head_dim 128: 2048 tokens behind 14k keys, bf16, 944 to 960 us (1.08 PFLOP/s, at the power cap); 512 behind
+// 8192, e4m3, 179 us (0.79 PFLOP/s: the loaders' conversions and their shared-memory traffic).
 // P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
 #pragma once
 
