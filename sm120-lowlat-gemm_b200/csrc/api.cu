@@ -118,7 +118,7 @@ bool make_sf_map(CUtensorMap* m, const void* ptr, int64_t row_bytes, int64_t row
 }  // namespace
 
 bool make_paged_map(CUtensorMap* m, const void* ptr, int head_dim, int elem_bytes, int slots, int heads, int pages, const int64_t stride[3],
-                    int box_rows, bool swizzle) {
+                    int box_rows, bool swizzle, int box_heads) {
   auto fn = encode_fn();
   if (!fn) return false;
   for (int i = 0; i < 3; ++i)
@@ -127,7 +127,7 @@ bool make_paged_map(CUtensorMap* m, const void* ptr, int head_dim, int elem_byte
   const int width = head_dim * elem_bytes > 128 ? 128 : head_dim * elem_bytes;  // bytes
   cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)slots, (cuuint64_t)heads, (cuuint64_t)pages};
   cuuint64_t strides[3] = {(cuuint64_t)stride[2], (cuuint64_t)stride[1], (cuuint64_t)stride[0]};
-  cuuint32_t box[4] = {(cuuint32_t)(width / elem_bytes), (cuuint32_t)box_rows, 1u, 1u};
+  cuuint32_t box[4] = {(cuuint32_t)(width / elem_bytes), (cuuint32_t)box_rows, (cuuint32_t)box_heads, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUresult r = fn(m, wide ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides,
                         box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

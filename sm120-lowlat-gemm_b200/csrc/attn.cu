@@ -120,8 +120,12 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     int box = 32;
     while (p.c.page_size % box) box /= 2;
     p.box = box >= 8 && maps(box, !fp8) ? box : 0;
-    const cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s)
-                        : attn_tiles_launch_bf16(p, mk, mv, fp8, plan.m.ctas, pdl_on(), s);
+    // queries: a stream's 128 rows are a box of whole tokens where the group divides them
+    CUtensorMap mq{};
+    const int64_t qs[3] = {p.q_tok * a.kv.tokens, p.q_tok, p.q_head};
+    p.q_box = 128 % p.group == 0 && make_paged_map(&mq, a.q, p.c.head_dim, 2, a.heads, a.kv.tokens, 1, qs, p.group, true, 128 / p.group);
+    const cudaError_t e = f16 ? attn_tiles_launch_f16(p, mk, mv, mq, fp8, plan.m.ctas, pdl_on(), s)
+                              : attn_tiles_launch_bf16(p, mk, mv, mq, fp8, plan.m.ctas, pdl_on(), s);
     if (e != cudaSuccess) return e;
   }
   const AttnDev many = p;
@@ -135,7 +139,7 @@ cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s
     const int blocks = plan.f.rows / 8;
     const bool early = plan.many || pdl_on();  // behind the tile kernel the launch overlaps its end; the kernel waits for it
     const cudaError_t e = f16 ? attn_rows_launch_f16(p, mk, mv, fp8, blocks, plan.f.ctas, early, s)
-                        : attn_rows_launch_bf16(p, mk, mv, fp8, blocks, plan.f.ctas, early, s);
+                              : attn_rows_launch_bf16(p, mk, mv, fp8, blocks, plan.f.ctas, early, s);
     if (e != cudaSuccess) return e;
   }
   return attn_combine_launch(plan.many ? many : p, p, f16, plan.many ? plan.m.ctas : 0, plan.few ? plan.f.ctas : 0, plan.few ? plan.f.rows : 0, s);

@@ -15,7 +15,9 @@
 // The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
 // Loaders: each of four warps fills a quarter of a 16-bit tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
 // of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. e4m3 tiles come the same way, whole,
-// into a staging ring; the loaders widen them into the swizzled tile.
+// into a staging ring; the loaders widen them into the swizzled tile. Queries: a stream's rows are one box of whole tokens where the
+// group is a power of two (a ragged windowed batch 73.9 us with 32 cp.async per thread and item instead, 70.8 so);
+// other groups are gathered.
 // e4m3 caches are multiplied in f16 whatever q's type is: one conversion makes two values, exactly. The rows of a quarter tile (32
 // keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values (4 of 11 bits; a row
 // 2^-24 below the quarter's largest becomes 0); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
@@ -24,8 +26,8 @@
 // its quarters times 2^-F.
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
-// Measured, 64 heads over 8, head_dim 128: 2048 tokens behind 14k keys, bf16, 944 to 960 us (1.08 PFLOP/s, at the power cap); 512 behind
-// 8192, e4m3, 179 us (0.79 PFLOP/s: the loaders' conversions and their shared-memory traffic).
+// Measured, 64 heads over 8, head_dim 128: 2048 tokens behind 14k keys, bf16, 937 us (1.10 PFLOP/s, at the power cap); 512 behind
+// 8192, e4m3, 176 us (0.81 PFLOP/s: the loaders' conversions and their shared-memory traffic).
 // P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
 #pragma once
 
@@ -146,7 +148,7 @@ struct Ring {
 
 // Barriers in the header: word offsets of 8 bytes from the start of shared memory.
 enum : int { BAR_KV_FULL = 0, BAR_KV_EMPTY = 8, BAR_Q_FULL = 16, BAR_Q_EMPTY = 17, BAR_S_FULL = 18, BAR_P_FULL = 20, BAR_PV_DONE = 22, BAR_DONE = 24,
-             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29, BAR_RAW_FULL = 33, BAR_RAW_EMPTY = 37 };
+             BAR_SEG_FULL = 25, BAR_SEG_EMPTY = 29, BAR_RAW_FULL = 33, BAR_RAW_EMPTY = 37, BAR_Q_RAW = 41 };
 constexpr int kSegRing = 4;        // segments published ahead of the roles that work on them
 
 // How an item uses the two streams.
@@ -157,7 +159,8 @@ __device__ __forceinline__ int tiles_mode(const Segment& g, int group) {
 
 template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k,
-                                                                        const __grid_constant__ CUtensorMap map_v) {
+                                                                        const __grid_constant__ CUtensorMap map_v,
+                                                                        const __grid_constant__ CUtensorMap map_q) {
   using Cfg = TilesCfg<T, FP8, D>;
   using Op = typename Cfg::Op;
   constexpr bool kBf16 = std::is_same<Op, __nv_bfloat16>::value;
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     }
     mbar_init(bar(BAR_Q_FULL), 128);
     mbar_init(bar(BAR_Q_EMPTY), 1);
+    mbar_init(bar(BAR_Q_RAW), 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(BAR_S_FULL + s), 1);
       mbar_init(bar(BAR_P_FULL + s), 128);
@@ -197,6 +201,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
   if (tid == 32) {
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
+    tma_prefetch_desc(&map_q);
   }
   if (warp == 12) {
     tmem_alloc(smem_u32(&tmem_holder), 512);
@@ -352,11 +357,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       raw.next(Cfg::kStageRing);
     };
     int item_parity = 0;
+    uint32_t q_raw_phase = 0;
+    const bool remake = kToF16 || p.negate;                        // queries are not multiplied as they are
     auto q_free = [&]() { return mbar_try(bar(BAR_Q_EMPTY), q_phase); };
     auto start_q = [&](const Segment& g) {  // copies under way
       wait(BAR_Q_EMPTY, q_phase, ST_PRODUCER_EMPTY_WAIT);
       q_phase ^= 1u;
       if (!ok) return;
+      if (p.q_box) {  // rows of no token of the tile get other tokens' queries, or zeros behind the last: nobody reads their results
+        if (lt == 0) {
+          const uint32_t there = bar(remake ? BAR_Q_RAW : BAR_Q_FULL);
+          mbar_expect_tx(there, 2 * Cfg::kTile);
+          for (int i = 0; i < 2 * Cfg::kHalves; ++i) {
+            const int half = i % Cfg::kHalves, stream = i / Cfg::kHalves;
+            tma_load_4d(base + Cfg::kQ + stream * Cfg::kTile + half * Cfg::kHalf, &map_q, there, half * 64, kv_head * p.group,
+                        g.s.t0 + g.tok0 + stream * (p.tok_tile / 2), 0);
+          }
+        }
+        return;
+      }
       const int rows = g.toks * p.group;
       const int64_t first = g.s.t0 + g.tok0;
       constexpr int CH = D / 8;
@@ -376,10 +395,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     };
     auto finish_q = [&]() {                 // copies there, and in the form the products take
       if (!ok) return;
+      if (p.q_box && !remake) {  // thread 0 arrived when it announced the copies' bytes
+        if (lt != 0) mbar_arrive(bar(BAR_Q_FULL));
+        return;
+      }
       constexpr int CH = D / 8;
       const int ch = lt % CH;
-      cp_async_wait<0>();
-      if (kToF16 || p.negate) {  // bf16 rows to f16 in place, and the sign of a negative softmax scale: each thread what it copied
+      if (p.q_box) {
+        wait(BAR_Q_RAW, q_raw_phase, ST_PRODUCER_EMPTY_WAIT);
+        q_raw_phase ^= 1u;
+        if (!ok) return;
+      } else {
+        cp_async_wait<0>();
+      }
+      if (remake) {  // bf16 rows to f16 in place, and the sign of a negative softmax scale: each thread what it copied itself, or what TMA did
         const uint32_t flip = p.negate ? 0x80008000u : 0u;
 #pragma unroll 4
         for (int r = lt / CH; r < kTilesRows; r += 128 / CH) {     // CH neighbouring lanes hold a row

@@ -2,7 +2,7 @@
 #include "attn_tiles_launch.cuh"
 
 namespace llg {
-cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s) {
-  return attn_tiles_dispatch<__half>(p, k, v, fp8, ctas, pdl, s);
+cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, bool fp8, int ctas, bool pdl, cudaStream_t s) {
+  return attn_tiles_dispatch<__half>(p, k, v, q, fp8, ctas, pdl, s);
 }
 }  // namespace llg

@@ -78,10 +78,10 @@ inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_
 bool make_dense_map(CUtensorMap* m, const void* ptr, int64_t row_bytes, int64_t rows, int64_t ld_bytes, int box_bytes,
                     int box_rows, bool streamed);
 
-// Map over a paged cache tensor [pages, heads, slots, head_dim] (strides in bytes: page, head, slot): box = box_rows slots x at most
+// Map over a paged cache tensor [pages, heads, slots, head_dim] (strides in bytes: page, head, slot): box = box_heads heads x box_rows slots x at most
 // 128 bytes of a row, swizzled over the box's width (128 or 64 bytes) or not at all. False when the strides cannot be described.
 bool make_paged_map(CUtensorMap* m, const void* ptr, int head_dim, int elem_bytes, int slots, int heads, int pages, const int64_t stride[3],
-                    int box_rows, bool swizzle);
+                    int box_rows, bool swizzle, int box_heads = 1);
 
 // ---- skinny GEMV -------------------------------------------------------------------------------------------------
 struct SkinnyDev {
@@ -146,8 +146,8 @@ int64_t attn_workspace(const llg_attn_args& a);
 cudaError_t attn_launch(const llg_attn_args& a, unsigned* status, cudaStream_t s);
 cudaError_t attn_rows_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
 cudaError_t attn_rows_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int blocks, int ctas, bool pdl, cudaStream_t s);
-cudaError_t attn_tiles_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
-cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, bool fp8, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_tiles_launch_bf16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, bool fp8, int ctas, bool pdl, cudaStream_t s);
+cudaError_t attn_tiles_launch_f16(const AttnDev& p, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, bool fp8, int ctas, bool pdl, cudaStream_t s);
 // Adds up what the tile kernel's `many_ctas` and the few-row kernel's `few_ctas` CTAs (tiles of few_rows rows) left; 0 for a kernel
 // that did not run, whose descriptor is then only the other's.
 cudaError_t attn_combine_launch(const AttnDev& many, const AttnDev& few, bool f16, int many_ctas, int few_ctas, int few_rows, cudaStream_t s);

@@ -89,6 +89,7 @@ struct AttnDev {
   int scale16;            // 16 scale bytes of a page from a multiple of 16 on lie together, 16-byte aligned
   int tok_tile;           // whole tokens per row tile
   int box;                // rows of a TMA box (16, or a divisor of 32 and of the page size in the tile kernel), 0: no tensor maps
+  int q_box;              // tile kernel: queries by TMA, 128 rows to a box
   float* part_o;          // [slots][rows per tile][head_dim]; tile kernel: [slots][head_dim / 4][256 rows][4]
   float* part_ml;         // [slots][rows per tile][2]: maximum (log2 domain), sum
   int4* split;            // [CTAs][2]: the cut item that goes on at the beginning of a CTA's share, and the one that starts at its
