@@ -75,7 +75,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     same h // (heads / kv_heads) share a kv head, up to 32 of them. scale: 1 / sqrt(head_dim) unless given. causal: query t of
     a sequence's n sees keys up to its own position kv_len - n + t. window > 0: only the last `window` keys up to there.
     A query that sees nothing (an empty sequence, fewer cached tokens than new ones) gives zeros and lse = -inf. Rows of q
-    behind the last sequence are left as they were in `out`. An infinite or NaN key or value reaches every query of its
+    behind the last sequence are left as they were in `out`. Forward only, like every call of this package. An infinite or NaN key or value reaches every query of its
     sequence's call, also through weights of zero."""
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
