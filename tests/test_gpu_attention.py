@@ -297,6 +297,24 @@ def test_a_nan_query_stays_a_nan_and_alone(news, lens, ct):
 
 
 @pytest.mark.parametrize("ct", ["same", "e4m3"])
+def test_queries_of_other_sequences_stay_apart(ct):
+    """Rows of the tile that belong to no token of it may hold anything: the next sequence's NaN, rows behind the last sequence."""
+    ct = E4M3 if ct == "e4m3" else BF
+    news, lens = [70, 3, 45], [300, 40, 2000]
+    table, pages = pages_for(lens, 16, 51)
+    kc, vc, ks, vs = make_cache(pages, 1, 16, 128, ct, 52)
+    g = torch.Generator().manual_seed(53)
+    q = torch.randn(sum(news) + 9, 8, 128, generator=g).to(BF).cuda()
+    starts = torch.tensor([0, 70, 73, 118], dtype=torch.int32, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = L.paged_attention(q, kc, vc, table, ln, q_starts=starts, k_scale=ks, v_scale=vs)
+    bad = q.clone()
+    bad[70:73], bad[118:] = math.nan, math.inf
+    got = L.paged_attention(bad, kc, vc, table, ln, q_starts=starts, k_scale=ks, v_scale=vs)
+    assert torch.equal(got[:70], want[:70]) and torch.equal(got[73:118], want[73:118]) and bool(got[70:73].isnan().all())
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
 @pytest.mark.parametrize("news,lens", [([1, 1], [70, 500]), ([90, 2], [300, 150])])
 def test_keys_and_values_in_one_allocation(news, lens, ct):
     """Strided views of one tensor, scale rows that are not contiguous, and a strided output: the same results."""
