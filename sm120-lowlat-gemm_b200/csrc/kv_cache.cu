@@ -6,9 +6,10 @@
 // Reading. value * 2^e, one rounding to the output type (none for bf16 and fp32: four significant bits fit).
 //
 // Both move bytes. A CTA takes a few tokens: a thread per token finds its page and slot once, then the rows of all heads go
-// through, 16 values (append: of K's row and of V's) or 16 stored bytes (read) per lane, a row on 4 to 32 lanes so that a row's
-// maximum is a shuffle, several rows requested before the first is written. Measured: 8192 tokens of 8 kv heads, bf16 into e4m3, 12.3 us
-// (4.1 TB/s of read and written bytes; conversions and maxima fill 60% of the issue slots); 8 x 8192 tokens back to bf16 80 us (4.8 TB/s).
+// through, 16 values (append: of K's row and of V's) or 8 (read) per lane, a row on 2 to 32 lanes so that a row's maximum is a
+// shuffle, several rows requested before the first is written. Measured: 8192 tokens of 8 kv heads, bf16 into e4m3, 12.3 us
+// (4.1 TB/s of read and written bytes; conversions and maxima fill 60% of the issue slots); 8 x 8192 tokens back to bf16 72 us (5.4 TB/s; 80
+// with 16 values per lane, whose two stores each touched half of every sector).
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -179,7 +180,7 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// LPR lanes per row, 16 stored bytes per lane; tokens [blockIdx.x * per, + per) of sequence blockIdx.y; blockIdx.z: K or V. Rows go
+// LPR lanes per row, 8 values per lane, so that a 16-bit row is written 16 bytes by 16 bytes without gaps; tokens [blockIdx.x * per, + per) of sequence blockIdx.y; blockIdx.z: K or V. Rows go
 // through in the order of the output.
 template <typename T, bool FP8, int LPR>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadDev p, int per) {
@@ -190,7 +191,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   const int seq = blockIdx.y, t0 = blockIdx.x * per, count = min(per, p.max_len - t0);
   const bool is_v = blockIdx.z != 0;
   const int sub = threadIdx.x % LPR;
-  constexpr int kValues = FP8 ? 16 : 8;  // per lane
+  constexpr int kValues = 8;  // per lane
+  using Raw = typename std::conditional<FP8, uint2, uint4>::type;
   if (threadIdx.x < count) {
     const int pos = t0 + threadIdx.x;
     Place w{-1, 0};
@@ -209,20 +211,20 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   const int64_t c_page = is_v ? c.vs_page : c.ks_page, c_head = is_v ? c.vs_head : c.ks_head, c_slot = is_v ? c.vs_slot : c.ks_slot;
   unsigned char* const out = (is_v ? p.v : p.k) + ((int64_t)seq * p.max_len + t0) * c.kv_heads * c.head_dim * (int64_t)sizeof(T);
   const int rows = count * c.kv_heads;
-  constexpr int kRowsPass = kThreads / LPR, kAhead = 4;
+  constexpr int kRowsPass = kThreads / LPR, kAhead = FP8 ? 8 : 4;
   for (int r0 = threadIdx.x / LPR; r0 < rows; r0 += kRowsPass * kAhead) {
-    uint4 raw[kAhead];
+    Raw raw[kAhead];
     uint32_t b[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int r = r0 + k * kRowsPass;
-      raw[k] = make_uint4(0u, 0u, 0u, 0u);
+      raw[k] = Raw{};
       b[k] = 0u;
       if (r < rows) {
         const int i = r / c.kv_heads, head = r - i * c.kv_heads;
         const Place w = where[i];
         if (w.pg >= 0) {
-          raw[k] = *reinterpret_cast<const uint4*>(base + w.pg * s_page + head * s_head + w.slot * s_slot + sub * 16);
+          raw[k] = *reinterpret_cast<const Raw*>(base + w.pg * s_page + head * s_head + w.slot * s_slot + sub * (int)sizeof(Raw));
           if constexpr (FP8) b[k] = scales[w.pg * c_page + head * c_head + w.slot * c_slot];
         }
       }
@@ -234,28 +236,28 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
       unsigned char* const dst = out + ((int64_t)r * c.head_dim + sub * kValues) * (int64_t)sizeof(T);
       if constexpr (FP8) {
         const float up = __uint_as_float(b[k] << 23);
-        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        float f[16];
+        const float2 x[4] = {e4m3x2_to_f32(raw[k].x & 0xffffu), e4m3x2_to_f32(raw[k].x >> 16), e4m3x2_to_f32(raw[k].y & 0xffffu),
+                             e4m3x2_to_f32(raw[k].y >> 16)};
+        float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 x = e4m3x2_to_f32(w[i] & 0xffffu), y = e4m3x2_to_f32(w[i] >> 16);
-          f[4 * i] = x.x * up; f[4 * i + 1] = x.y * up; f[4 * i + 2] = y.x * up; f[4 * i + 3] = y.y * up;
+          f[2 * i] = x[i].x * up;
+          f[2 * i + 1] = x[i].y * up;
         }
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          for (int i = 0; i < 2; ++i) __stcs(reinterpret_cast<float4*>(dst) + i, make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]));
         } else {
-          T o[16];
+          alignas(16) T o[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             if constexpr (std::is_same<T, __half>::value) o[i] = __float2half_rn(f[i]);
             else o[i] = __float2bfloat16_rn(f[i]);
           }
-          reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(o)[0];
-          reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(o)[1];
+          __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(o));
         }
       } else {
-        *reinterpret_cast<uint4*>(dst) = raw[k];
+        __stcs(reinterpret_cast<uint4*>(dst), raw[k]);
       }
     }
   }
@@ -285,8 +287,8 @@ cudaError_t append(const AppendDev& p, cudaStream_t s) {
 
 template <typename T, bool FP8>
 cudaError_t read(const ReadDev& p, cudaStream_t s) {
-  const int lpr = lanes_for(p.c.head_dim / (FP8 ? 16 : 8));
-  const int per = tokens_per_cta((long long)p.c.batch * p.max_len * 2, p.c.kv_heads, lpr, 4);
+  const int lpr = lanes_for(p.c.head_dim / 8);
+  const int per = tokens_per_cta((long long)p.c.batch * p.max_len * 2, p.c.kv_heads, lpr, FP8 ? 8 : 4);
   const dim3 grid((unsigned)((p.max_len + per - 1) / per), (unsigned)p.c.batch, 2), block(kThreads), one(1, 1, 1);
   switch (lpr) {
     case 4: return launch_ex(kv_read_kernel<T, FP8, 4>, grid, block, 0, s, pdl_on(), one, p, per);
