@@ -6,7 +6,7 @@
 // Reading. value * 2^e, one rounding to the output type (none for bf16 and fp32: four significant bits fit).
 //
 // Both move bytes. A CTA takes a few tokens: a thread per token finds its page and slot once, then the rows of all heads go
-// through, 16 values (append: of K's row and of V's) or 8 (read) per lane, a row on 2 to 32 lanes so that a row's maximum is a
+// through, 16 values (append: of K's row and of V's) or 8 (read) per lane, a row on 4 to 32 lanes so that a row's maximum is a
 // shuffle, several rows requested before the first is written. Measured: 8192 tokens of 8 kv heads, bf16 into e4m3, 12.3 us
 // (4.1 TB/s of read and written bytes; conversions and maxima fill 60% of the issue slots); 8 x 8192 tokens back to bf16 72 us (5.4 TB/s; 80
 // with 16 values per lane, whose two stores each touched half of every sector).
