@@ -280,7 +280,8 @@ LLG_API int llg_tc_gemm_static_ws(const llg_tc_args* args, void* stream);
  * [batch + 1] gives the rows of the new tokens in the per-token tensors; NULL: every sequence has tokens / batch of them
  * (tokens must be a multiple of batch). Rows at and behind q_starts[batch] belong to no sequence: they are neither read into
  * the cache nor written. Lengths and offsets are read on the device only, so a captured call follows them from replay to replay.
- * A length beyond table_width * page_size is cut to it. A page table entry in use that names no page (negative, or >= pages)
+ * A length may go beyond table_width * page_size: the tokens behind that end have no place, so they are neither written nor seen,
+ * and every new token keeps the position that the whole length gives it. A page table entry in use that names no page (negative, or >= pages)
  * is not followed: its rows are not written and read as zeros, and llg_device_status() returns 32. Sequences may share pages
  * that a call only reads; the slots that one call writes must be distinct.
  * No counterpart in the reference, which leaves the cache to the serving framework. */

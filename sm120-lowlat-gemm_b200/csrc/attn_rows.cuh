@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
   while (next_segment<KT>(p, share, g)) {
     const int rows = g.toks * p.group;
     const int nb_used = (rows + 7) >> 3;
-    const int pos0 = g.s.len - g.s.n + g.tok0;  // position of the tile's first token
+    const int pos0 = g.s.pos + g.tok0;  // position of the tile's first token
 
     // ---- the warp's ring: tile t holds the warp's groups of 16 keys, from key_of(t) on
     const int nt = g.tile1 - g.tile0;

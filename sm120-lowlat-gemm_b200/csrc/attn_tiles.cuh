@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int step = mode == MODE_KEYS ? 2 : 1;
       const bool live = row < rows;
       const int tok = row / p.group;
-      const int pos = g.s.len - g.s.n + g.tok0 + tok;
+      const int pos = g.s.pos + g.tok0 + tok;
       // rows of no token see everything: they keep no tile from the unmasked path, and nobody reads them
       const int last = !live ? INT_MAX : p.causal ? min(pos, g.s.len - 1) : g.s.len - 1;
       const int first = live && p.window > 0 ? pos - p.window + 1 : 0;

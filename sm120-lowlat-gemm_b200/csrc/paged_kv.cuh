@@ -30,10 +30,13 @@ struct PagedKV {
 };
 
 struct SeqView {
-  int t0, n, len;  // first row of its new tokens in q / k / v, their number, tokens in the cache with them
+  int t0, n;       // first row of its new tokens in q / k / v, their number
+  int pos;         // position of the first one: the length as it is given, less n
+  int len;         // tokens that the cache holds: no more than the page table can name
 };
 
-// Offsets that point outside the call's tensors are cut to them, lengths to what the page table can name.
+// Offsets that point outside the call's tensors are cut to them. Tokens behind the end of the page table are not in the cache, but
+// the new ones before them stand where they would without that end.
 __device__ __forceinline__ SeqView seq_view(const PagedKV& c, int i) {
   SeqView s;
   if (c.starts) {
@@ -43,8 +46,9 @@ __device__ __forceinline__ SeqView seq_view(const PagedKV& c, int i) {
     s.t0 = i * c.q_len;
     s.n = c.q_len;
   }
-  const int64_t most = (int64_t)c.table_width * c.page_size;
-  s.len = (int)min((int64_t)max(c.lens[i], 0), most);
+  const int len = max(c.lens[i], 0);
+  s.pos = len - s.n;
+  s.len = (int)min((int64_t)len, (int64_t)c.table_width * c.page_size);
   return s;
 }
 
@@ -111,8 +115,8 @@ struct KeyRange {
 };
 __device__ __forceinline__ KeyRange key_range(const AttnDev& p, const SeqView& s, int tf, int cnt) {
   KeyRange r;
-  r.hi = p.causal ? min(max(s.len - s.n + tf + cnt, 0), s.len) : s.len;
-  r.lo = p.window > 0 ? max(s.len - s.n + tf + 1 - p.window, 0) : 0;
+  r.hi = p.causal ? min(max(s.pos + tf + cnt, 0), s.len) : s.len;
+  r.lo = p.window > 0 ? max(s.pos + tf + 1 - p.window, 0) : 0;
   r.lo = min(r.lo, r.hi);
   return r;
 }

@@ -10,7 +10,8 @@ float8_e8m0fnu power of two per row beside it: k_scale and v_scale [pages, kv_he
 Where tokens are: page_table [batch, n] int32 names each sequence's pages in order, kv_lens [batch] int32 counts its cached
 tokens with the new ones, which are the last. New tokens of all sequences are stacked: q_starts [batch + 1] int32 says where
 each sequence's begin; without it every sequence has tokens / batch of them. These three live on the device and are read there,
-so one captured call serves every step.
+so one captured call serves every step. A length may grow beyond the n * page_size tokens that a sequence's pages hold: tokens
+behind them are not stored and not seen, and positions stay those of the whole length.
 
 A decode step with `x` [batch, hidden]:
 

@@ -1,0 +1,137 @@
+"""Paged cache and attention where they can go wrong: the cache's end, rows that a query may not see, powers of two far apart,
+weights far below the largest."""
+import math
+
+import pytest
+import torch
+
+import lowlat_gemm as L
+from lowlat_gemm import _native as N, tp as TP
+
+from test_gpu_attention import BF, E4M3, E8M0, HF, make_cache, pages_for, rows_of
+from test_gpu_decode_attention import SHAPE, recorded
+
+pytestmark = pytest.mark.gpu
+
+
+def expected(q, kc, vc, ks, vs, table, lens, starts, *, scale=None, causal=True, window=0, shared=0):
+    """(o, lse, tolerance of o) in float64 by the definition: the new tokens' positions count back from the length as it is given,
+    keys end where the page table ends, and every bound comes from the keys that the query sees."""
+    tokens, heads, dim = q.shape
+    group, cap = heads // kc.shape[1], table.shape[1] * kc.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    half = torch.finfo(q.dtype).eps / 2
+    o = torch.zeros(tokens, heads, dim, dtype=torch.float64, device="cuda")
+    lse = torch.full((tokens, heads), -math.inf, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(o)
+    for i, length in enumerate(lens):
+        t0, t1 = starts[i], starts[i + 1]
+        keys, n = min(length, cap), t1 - t0
+        if n == 0 or keys == 0:
+            continue
+        k, v = (rows_of(c, s, table, i, keys).repeat_interleave(group, 1) for c, s in ((kc, ks), (vc, vs)))
+        e = rows_of(torch.ones_like(vc), vs, table, i, keys)[..., :1].repeat_interleave(group, 1)  # powers of two of V's rows, 1 for 16 bits
+        qq = q[t0:t1].double()
+        s = torch.einsum("thd,jhd->thj", qq, k) * scale
+        pos = length - n + torch.arange(n, device="cuda")[:, None]
+        j = torch.arange(keys, device="cuda")[None]
+        seen = (j <= pos) if causal else torch.ones(n, keys, dtype=torch.bool, device="cuda")
+        if window:
+            seen = seen & (j > pos - window)
+        s = torch.where(seen[:, None], s, -math.inf)
+        top = s.amax(-1, keepdim=True)
+        p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+        total = p.sum(-1, keepdim=True)
+        w = p / torch.where(total == 0, 1.0, total)
+        o[t0:t1] = torch.einsum("thj,jhd->thd", w, v)
+        lse[t0:t1] = (top + torch.log(total)).squeeze(-1)
+        # half a step of the result, half a step of each probability, 2^-24 for each product and sum over keys; a score is a dot
+        # product of dim fp32 products and sums, 2^-24 each of sum |q||k|, and moves a weight by twice its error; exp2 adds 2^-21
+        mass = torch.einsum("thj,jhd->thd", w, v.abs())
+        sizes = torch.einsum("thd,jhd->thj", qq.abs(), k.abs()) * abs(scale)
+        delta = torch.where(seen[:, None], sizes, 0.0).amax(-1, keepdim=True) * (dim + 4) * 2.0 ** -24 + 2.0 ** -21
+        # f16 probabilities, times their row's power of two, are whole multiples of 2^-24, off by half of one, the largest being 2^7 at
+        # the least; rows of a tile may share a power of two `shared` binary orders above their own
+        least = torch.einsum("tj,jhd->thd", seen.double(), (v / e).abs()) * (w * e.permute(2, 1, 0)).amax(-1, keepdim=True) * 2.0 ** (shared - 32)
+        tol[t0:t1] = half * o[t0:t1].abs() + mass * (half + 2 * delta + keys * 2.0 ** -24) + torch.finfo(q.dtype).tiny + (0 if kc.dtype == BF else least)
+    return o, lse, tol
+
+
+def setup(news, lens, heads, kvh, dim, page, qt, ct, *, seed=0, width=None, ragged=True):
+    """(q, cache arguments, scales, starts): lens may go beyond width * page, where no row of the cache lies."""
+    cap = (width or 1 << 30) * page
+    table, pages = pages_for([min(n, cap) for n in lens], page, seed, width=width)
+    kc, vc, ks, vs = make_cache(pages, kvh, page, dim, ct, seed + 1)
+    q = torch.randn(sum(news), heads, dim, generator=torch.Generator().manual_seed(seed + 2)).to(qt).cuda()
+    starts = [sum(news[:i]) for i in range(len(news) + 1)]
+    kw = dict(k_scale=ks, v_scale=vs)
+    if ragged:
+        kw["q_starts"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    return q, (kc, vc, table, torch.tensor(lens, dtype=torch.int32, device="cuda")), kw, starts
+
+
+def compare(q, cache, kw, starts, lens, *, causal=True, window=0, scale=None, shared=0):
+    out, lse = L.paged_attention(q, *cache, causal=causal, window=window, scale=scale, return_lse=True, **kw)
+    want, wl, tol = expected(q, cache[0], cache[1], kw["k_scale"], kw["v_scale"], cache[2], lens, starts, causal=causal, window=window,
+                             scale=scale, shared=shared)
+    most = torch.finfo(q.dtype).max  # a result behind the type's largest value is infinite
+    err = torch.where((out == torch.copysign(torch.full_like(out, math.inf), out)) & (want * out.sign() + tol >= most), 0.0, (out.double() - want).abs())
+    assert bool((err <= tol).all()), f"error {err.max().item():.3e}, {(err / tol).max().item():.2f} of its bound"
+    assert torch.equal(torch.isfinite(lse), torch.isfinite(wl))
+    fin = torch.isfinite(wl)
+    # a score is off by 2^-18 of its size (|lse| and dim bound it here), the logarithm of the sum by 2^-19
+    assert bool(((lse.double() - wl)[fin].abs() <= 2.0 ** -18 * (1 + wl[fin].abs() + q.shape[2])).all())
+    assert N.device_status() == 0
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# lengths beyond the page table
+
+
+@pytest.mark.parametrize("ct", ["same", "e4m3"])
+@pytest.mark.parametrize("news,lens", [([3], [66]), ([1, 1], [65, 64]), ([5, 5, 5], [70, 64, 68]), ([40, 2], [80, 65]), ([300], [120]),
+                                       ([2], [500]), ([90], [700])])
+def test_positions_beyond_the_page_table(news, lens, ct):
+    """Four pages of 16: tokens behind the 64th are not there, and the queries before and behind the end keep their positions."""
+    for qt, dim, heads, kvh in ((BF, 128, 8, 1), (HF, 64, 10, 2)):
+        for kw in ({}, dict(window=9), dict(window=70), dict(causal=False), dict(causal=False, window=9)):
+            for ragged in (True, False) if len(set(news)) == 1 else (True,):
+                q, cache, args, starts = setup(news, lens, heads, kvh, dim, 16, qt, E4M3 if ct == "e4m3" else qt, seed=lens[0], width=4,
+                                               ragged=ragged)
+                compare(q, cache, args, starts, lens, **kw)
+
+
+@pytest.mark.parametrize("ct", [BF, E4M3])
+@pytest.mark.parametrize("new", [3, 40])
+def test_append_and_attention_agree_on_positions(new, ct):
+    """With a window of one a query's result is its own token's value, or zero where the cache had no place for it."""
+    table, pages = pages_for([64], 16, 3)
+    kc, vc, ks, vs = make_cache(pages, 1, 16, 128, ct, 4)
+    kv = torch.randint(8, 16, (new, 2, 128), generator=torch.Generator().manual_seed(5)).to(BF).cuda()  # four bits: e4m3 holds them
+    q = torch.randn(new, 8, 128, generator=torch.Generator().manual_seed(6)).to(BF).cuda()
+    for length in (64, 65, 64 + new - 1, 64 + new, 64 + 2 * new):
+        ln = torch.tensor([length], dtype=torch.int32, device="cuda")
+        L.kv_append(kv[:, :1], kv[:, 1:], kc, vc, table, ln, k_scale=ks, v_scale=vs)
+        out = L.paged_attention(q, kc, vc, table, ln, k_scale=ks, v_scale=vs, window=1)
+        there = (torch.arange(length - new, length, device="cuda") < 64)[:, None, None]
+        want = torch.where(there, kv[:, 1:].double(), 0.0).expand(new, 8, 128)
+        assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want).all()), length  # the result's rounding; the one weight is 1
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF])
+def test_steps_that_cross_the_end_of_the_cache(dtype):
+    """Tokens behind the cache's end are not stored; queries of the step that crosses it and of later ones still see what is there."""
+    batch, new, dev = 2, 3, torch.device("cuda", 0)
+    cache = TP.DecodeCache(1, batch, 8, 2, dev, page_size=4, dtype=dtype)
+    step = TP.DecodeStep("bf16", 1, 1, 0, dev, SHAPE, residual=True, cache=cache)
+    calls = recorded(step)
+    g = torch.Generator().manual_seed(5)
+    for t in range(4):
+        calls.clear()
+        step.run((torch.randn(batch * new, 1024, generator=g) * 0.5).to(BF).to(dev))
+        q = calls[0][1][:, :1024].reshape(batch * new, 8, 128)
+        (kc, vc, table, _), scales = cache.layers[0]
+        want, _, tol = expected(q, kc, vc, scales.get("k_scale"), scales.get("v_scale"), table, [(t + 1) * new] * batch, [0, new, 2 * new])
+        assert bool(((calls[1][0].view_as(q).double() - want).abs() <= tol).all()), t
+    assert N.device_status() == 0
