@@ -65,8 +65,9 @@ def shard_gate_up(w: torch.Tensor, tp: int, rank: int) -> torch.Tensor:
 class DecodeCache:
     """Paged key/value caches of `layers` layers for `batch` sequences on this rank: one page table and one length vector serve
     them all. dtype float8_e4m3fn (quantised rows with a power of two each) or the activations' 16-bit type. Sequences own
-    their pages from the start (max_len tokens each); kv_lens begins at 0, and every DecodeStep.run() with this cache adds its
-    tokens. Lengths live on the device, so a captured run appends on every replay; tokens beyond max_len are not stored."""
+    their pages from the start: max_len tokens each, rounded up to whole pages (the attribute max_len says how many). kv_lens
+    begins at 0, and every DecodeStep.run() with this cache adds its tokens. Lengths live on the device, so a captured run appends
+    on every replay; tokens beyond max_len are not stored and not seen, and lengths and positions count on."""
 
     def __init__(self, layers: int, batch: int, max_len: int, kv_heads: int, device, head_dim: int = 128, page_size: int = 64,
                  dtype: torch.dtype = FP8):
@@ -75,7 +76,7 @@ class DecodeCache:
         if min(layers, batch, max_len, kv_heads, page_size) < 1:
             raise ValueError("layers, batch, max_len, kv_heads and page_size must be at least 1")
         per = -(-max_len // page_size)
-        self.batch, self.kv_heads, self.head_dim, self.dtype = batch, kv_heads, head_dim, dtype
+        self.batch, self.kv_heads, self.head_dim, self.dtype, self.max_len = batch, kv_heads, head_dim, dtype, per * page_size
         self.page_table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
         self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         shape = (batch * per, kv_heads, page_size, head_dim)

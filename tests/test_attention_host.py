@@ -132,3 +132,10 @@ def test_decode_cache_arguments():
     with pytest.raises(ValueError, match="own entry points"):
         TP.DecodeStep("bf16", 1, 1, 0, torch.device("cpu"), TP.LayerShape(hidden=256, qkv=512, inter=256), gemm_fn=lambda *a, **k: None,
                       cache=TP.DecodeCache(1, 1, 8, 1, "cpu"))
+
+
+def test_decode_cache_holds_whole_pages():
+    """max_len is what a sequence's pages hold, not less than was asked for."""
+    for asked, page, held in ((100, 16, 112), (64, 64, 64), (1, 64, 64), (65, 64, 128)):
+        c = TP.DecodeCache(1, 2, asked, 1, "cpu", page_size=page)
+        assert c.max_len == held == c.page_table.shape[1] * c.layers[0][0][0].shape[2]
