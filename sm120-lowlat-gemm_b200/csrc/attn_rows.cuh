@@ -15,11 +15,11 @@
 //     TMA's swizzle free of bank conflicts. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's
 //     type is: a bf16 row of q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less
 //     lose bits). The scores take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the
-//     running maximum is that of s + e, so p 2^e <= 2^8 and keeps f16's 11 bits where it matters.
+//     running maximum is that of s + e, so p 2^e <= 2^15 and keeps f16's 11 bits where it matters.
 // P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
 // Measured: 32 sequences of 0.9k to 8.2k keys, 64 heads over 8, e4m3, 65.7 us (4.4 TB/s); 4 of 50k to 65k, bf16, 50.4 us (5.2 TB/s).
-// The running maximum moves only when a score exceeds it by more than 2^8: p <= 256 then, and the shuffles and the rescaling of
-// O are skipped for almost every tile.
+// m moves only when a score exceeds the largest so far by more than 2^8, so the shuffles and the rescaling of O are skipped for almost
+// every tile; kHead, kMove: where p lies.
 #pragma once
 
 #include <climits>
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
             asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv) : "r"(sb + 32 * u + 16 + krow + 8 * e) : "memory");
             kf[u][e] = pow2_of(bk);
             vf[u][e] = pow2_of(bv);
-            ve[u][e] = __uint_as_float(0x4b000000u + max(bv, 27u)) - 8388735.f;  // e, not below -100: bits of 2^23 + b, less 2^23 + 127
+            ve[u][e] = __uint_as_float(0x4b000000u + max(bv, kLeastV)) - 8388735.f;  // e, not below -88: bits of 2^23 + b, less 2^23 + 127
           }
         }
       uint32_t pf[SUB][NB][2];
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
               const int key = key0 + 16 * u + krow + (e >> 1) * 8;
               if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[u][e] = -INFINITY;
             }
-            more |= x[u][e] + ve[u][e >> 1] > m[nb][e & 1] + 8.f;
+            more |= x[u][e] + ve[u][e >> 1] > m[nb][e & 1] + kMove;
           }
         if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float top = fmaxf(m[nb][e], mx);
+            const float top = fmaxf(m[nb][e], mx - kHead);
             const float keep = m[nb][e] == -INFINITY ? 0.f : exp2_fast(m[nb][e] - top);
             m[nb][e] = top;
             l[nb][e] *= keep;

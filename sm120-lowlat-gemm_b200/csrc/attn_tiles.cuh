@@ -12,7 +12,7 @@
 // head_dim 128) and the exponentials 128 x 128 / 16 = 1024, so the two streams alternate between units that are equally busy.
 // Items of at most 128 rows that several CTAs share (few rows, long cache) give both streams the same queries: A takes the
 // even key tiles, B the odd ones, and each leaves a partial result of its own.
-// The running maximum moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds it by 2^8.
+// m moves (and O is rescaled, from and to tensor memory) only when a row's score exceeds the largest so far by 2^8.
 // Loaders: each of four warps fills a quarter of a 16-bit tile, by TMA in boxes of rows that share a page (page sizes that are a multiple
 // of 8), row by row with cp.async and zeros where a quarter has rows outside the item's keys. e4m3 tiles come the same way, whole,
 // into a staging ring; the loaders widen them into the swizzled tile. Queries: a stream's rows are one box of whole tokens where the
@@ -647,9 +647,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             w = max(w & 0xffu, (w >> 8) & 0xffu);
 #pragma unroll
             for (int d = 1; d < 8; d <<= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, d));
-            return max(w, 27u);
+            return w;
           };
-          const uint32_t top = quarter_top(sc);
+          const uint32_t top = max(quarter_top(sc), is_v ? kLeastV : 27u);
           uint32_t half[2] = {0u, 0u};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           }
           asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + lane * 8), "r"(half[0]), "r"(half[1]) : "memory");
           if (!is_v) {
-            const uint32_t v_top = quarter_top(sv);
+            const uint32_t v_top = max(quarter_top(sv), kLeastV);
             if ((lane & 7) == 0) {
               const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + (lane >> 3);
               asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
@@ -735,11 +735,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t top = max(__reduce_max_sync(0xffffffffu, sc[q]), 27u);
+          const uint32_t top = max(__reduce_max_sync(0xffffffffu, sc[q]), is_v ? kLeastV : 27u);
           const uint32_t d = top - sc[q], half = d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;  // 2^-d as f16
           asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + (32 * q + lane) * 2), "h"((uint16_t)half) : "memory");
           if (!is_v) {
-            const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, other[q]), 27u);
+            const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, other[q]), kLeastV);
             if (lane == 0) {
               const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + q;
               asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       // rows of no token see everything: they keep no tile from the unmasked path, and nobody reads them
       const int last = !live ? INT_MAX : p.causal ? min(pos, g.s.len - 1) : g.s.len - 1;
       const int first = live && p.window > 0 ? pos - p.window + 1 : 0;
-      float m = -INFINITY;                                       // running maximum of the scores in log2 units (+ F)
+      float m = -INFINITY;                                       // reference of the probabilities: scores in log2 units (+ F)
       float c_row = p.scale_log2;
       uint64_t l2 = 0;                                           // two partial row sums
       int done = 0;                                              // key tiles of this stream behind us
@@ -846,9 +846,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         } else {
           top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c_row;
         }
-        const bool move = top > m + 8.f || (m == -INFINITY && top > m);
+        const bool move = top > m + kMove || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
-          const float now = move ? top : m;
+          const float now = move ? top - kHead : m;
           const float keep = m == -INFINITY ? 0.f : exp2_fast(m - now);
           if (done > 0) {  // rescale what has been added up so far
             wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);

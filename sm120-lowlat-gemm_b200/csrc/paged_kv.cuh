@@ -102,6 +102,14 @@ struct AttnDev {
   int* first;             // [CTAs]: the CTA in which the item that goes on started
 };
 
+// Probabilities are 2^(score - m) with m kHead below the largest score that moved it, and m moves when a score exceeds it by 2^15: the
+// largest of a row lies between 2^7 and 2^15. f16 ends at 2^15.99 and, with full accuracy, at 2^-14, so keys down to 2^-21 of the
+// largest keep their bits and keys down to 2^-32 are counted (a largest probability of 1 to 2^8 lost 131k keys 2^-25.3 below one).
+constexpr float kHead = 7.f, kMove = 15.f;
+// Least power of two of a row of V (biased by 127) that the maximum takes account of: row sums, up to 2^(15 + 88) a key, stay in fp32.
+// Smaller rows are multiplied by their power all the same.
+constexpr uint32_t kLeastV = 39;
+
 // CTAs of the few-row kernel that fit an SM: as many as its registers and rings of two to three tiles let in, which hides the chain
 // from a load to the next product better than longer rings (8 rows, decode batch over e4m3: two 74.5 us, three 65.3; 16-bit 51.8, 50.4;
 // 20 rows of 64 values: two of 32 rows 32.9, three of 24 29.4).

@@ -135,3 +135,31 @@ def test_steps_that_cross_the_end_of_the_cache(dtype):
         want, _, tol = expected(q, kc, vc, scales.get("k_scale"), scales.get("v_scale"), table, [(t + 1) * new] * batch, [0, new, 2 * new])
         assert bool(((calls[1][0].view_as(q).double() - want).abs() <= tol).all()), t
     assert N.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# weights far below the largest
+
+
+@pytest.mark.parametrize("strong", [0, 70000, 131071 - 70])
+@pytest.mark.parametrize("ct", [HF, E4M3])
+@pytest.mark.parametrize("new,batch", [(1, 600), (70, 150)])
+def test_a_long_flat_tail_below_one_strong_key(new, batch, ct, strong):
+    """131k keys 2^-25.3 below one, with values of 256: each alone rounds away beside a largest probability of 1, together they are
+    as much as the strong key. As many sequences over the same pages as there are CTAs, so that one of them meets all of the keys."""
+    n, page = 131072, 128
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").repeat(batch, 1)
+    kc, vc = torch.zeros(2, n // page, 1, page, 64, device="cuda").unbind(0)
+    kc[strong // page, 0, strong % page, 0] = 1.0
+    vc[...] = -256.0
+    vc[strong // page, 0, strong % page] = 1.0
+    kw = dict(k_scale=None, v_scale=None)
+    if ct == E4M3:
+        kw = {k: torch.full((n // page, 1, page), 127, dtype=torch.uint8, device="cuda").view(E8M0) for k in kw}
+    q = torch.zeros(batch * new, 1, 64, dtype=HF, device="cuda")
+    q[:, 0, 0] = 25.3 * math.log(2.0)
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = L.paged_attention(q, kc.to(ct), vc.to(ct), table, lens, scale=1.0, **kw).view(batch, new, 1, 64)
+    want, _, tol = expected(q[:new], kc.to(ct), vc.to(ct), kw["k_scale"], kw["v_scale"], table, [n], [0, new], scale=1.0)
+    err = (out.double() - want).abs()
+    assert bool((err <= tol).all()), f"error {err.max().item():.3e}, {(err / tol).max().item():.2f} of its bound"
