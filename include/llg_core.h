@@ -325,11 +325,12 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * sees key j when j <= position (causal) and j > position - window (window > 0); scores are scale * q . k, o = softmax v,
  * lse = log of the sum of exp(scores) (natural, fp32). A query that sees no key gives o = 0 and lse = -inf.
  * head_dim 64 or 128; q and out in the cache's 16-bit type, or either 16-bit type over E4M3; heads / kv_heads <= 32.
- * An E4M3 value is multiplied as F16 whatever q's type is, its row's power of two kept apart where one kv head has few query rows
- * and relative to the largest of 32 neighbouring rows where it has many: rows 2^-15 below that largest then lose bits, rows 2^-24
- * below count as zeros. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
+ * An E4M3 value is multiplied as F16 whatever q's type is, exactly; its row's power of two is applied in fp32, and keys that a query
+ * does not see have no part in its result, whatever their powers are. Rows of 2^-100 or less (bytes up to 27) may count as zeros beside
+ * larger ones. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
  * Weights go into the second product in 16 bits, BF16 over a BF16 cache, else F16: there a weight (times its V row's power of two) keeps
- * its bits down to 2^-21 of the largest and counts down to 2^-32; the row sum has fp32 weights. ws:
+ * its bits down to 2^-21 of the largest and counts down to 2^-32. The row sum has fp32 weights; over E4M3 it counts them down to
+ * 2^(E - min(e, 0) - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12. ws:
  * llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
 typedef struct llg_attn_args {
   llg_paged_kv kv;

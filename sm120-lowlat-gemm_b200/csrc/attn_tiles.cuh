@@ -19,11 +19,15 @@
 // group is a power of two (a ragged windowed batch 73.9 us with 32 cp.async per thread and item instead, 70.8 so);
 // other groups are gathered.
 // e4m3 caches are multiplied in f16 whatever q's type is: one conversion makes two values, exactly. The rows of a quarter tile (32
-// keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values (4 of 11 bits; a row
-// 2^-24 below the quarter's largest becomes 0); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
+// keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values, which is exact down to
+// 2^-15 (4 of 11 bits); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
 // put the rest back where it costs nothing: score * (2^E, q's power) is the factor their multiply-add has anyway, and the
 // probability is 2^(s + F - m) with m the running maximum of s + F, so that P 2^-F V is what the product sums; the row sum takes
 // its quarters times 2^-F.
+// The quarter's largest may be a row that a query does not see, so a tile with rows further apart than that (V: 2^-7, the room that m
+// leaves above) is an own one: its values are widened as they are, and the softmax threads, which find every row's two powers in
+// shared memory, multiply each score by its own and take s + e of the keys that they see. A tile of that kind takes four to five times as long (a chunk
+// of 512 behind 8192 of nothing else 798 us instead of 168).
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
 // Measured, 64 heads over 8, head_dim 128: 2048 tokens behind 14k keys, bf16, 937 us (1.10 PFLOP/s, at the power cap); 512 behind
@@ -55,10 +59,14 @@ struct TilesCfg {
   static constexpr int kRing = kQ + 2 * kTile;
   static constexpr int kStageAt = kRing + kSlots * kTile;
   static constexpr int kScaleAt = kStageAt + kStageRing * kStage;  // [kStageRing][128] f16: a staged row's factor
-  static constexpr int kRefAt = kScaleAt + kStageRing * 256;       // [8 key tiles][8] bytes: E and F of the quarters, biased by 127
+  static constexpr int kRefAt = kScaleAt + kStageRing * 256;       // [8 key tiles][8] bytes: E and F of the quarters, biased by 127; no F: an own tile
   static constexpr int kQFacAt = kRefAt + (FP8 ? 64 : 0);          // [2 items][256] floats: the power of two of a row of q
-  static constexpr int kSmem = kQFacAt + (FP8 ? 2048 : 0) + 1024;  // + alignment slack
+  static constexpr int kOwnAt = kQFacAt + (FP8 ? 2048 : 0);        // [8 key tiles][2][128] bytes: powers of two of an own tile's rows of K, of V
+  static constexpr int kSmem = kOwnAt + (FP8 ? 2048 : 0) + 1024;   // + alignment slack
 };
+
+// How far below a quarter's largest power of two its other rows may lie (see above).
+constexpr uint32_t kSpreadK = 15, kSpreadV = 7;
 
 // Shared-memory descriptor of V: rows of 64 elements (128 bytes, 128-byte swizzle) along K, 8 rows every 1024 bytes, the next
 // 64 columns `half` bytes on (MN-major operand).
@@ -133,6 +141,13 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+
+// An own tile's rows: byte i of sixteen, and the power of two of a row of V that m takes account of (byte 255, no number, reaches P).
+__device__ __forceinline__ uint32_t byte_of(const uint4& v, int i) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  return (w[i >> 2] >> (8 * (i & 3))) & 0xffu;
+}
+__device__ __forceinline__ float v_power(uint32_t b) { return __uint_as_float(0x4b000000u + (b == 255u ? kLeastV : max(b, kLeastV))) - 8388735.f; }
 
 // Ring of mbarrier phases: slot i of n, used round after round.
 struct Ring {
@@ -613,6 +628,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       int j = tile0, entry = INT_MIN;
       const unsigned char *const ks = c.ks + kv_head * c.ks_head, *const vs = c.vs + kv_head * c.vs_head;
       const bool words = p.scale16 && p.box > 0;
+      // Scale bytes are worked on four at a time. Are any of them further below their quarters' largest (`high`) than may be, or beyond
+      // what the softmax's factors can take? Then the tile is an own one. Rows of zeros and others of the smallest power that the cache's
+      // writer knows, 2^-100, do not ask for that: beside larger ones they count as zeros.
+      const uint32_t spread = (is_v ? kSpreadV : kSpreadK) * 0x01010101u, least = (is_v ? kLeastV : 27u) * 0x01010101u;
+      auto far_apart = [&](uint32_t w, uint32_t high, uint32_t by) {
+        w |= __vcmpleu4(w, 27u * 0x01010101u);
+        return __any_sync(0xffffffffu, __vmaxu4(w, __vsubus4(high, by)) != w || __vmaxu4(high, 0xfdfdfdfdu) != 0xfdfdfdfdu);
+      };
+      // by how many powers of two the rows' values go down: an own tile's only where m takes no account of them
+      auto shifts = [&](bool own, uint32_t w, uint32_t top) { return !own ? top - w : is_v ? __vsubus4(least, w) : 0u; };
+      auto down16 = [&](uint32_t d4) {  // 2^-d as f16, d the lowest byte
+        const uint32_t d = d4 & 0xffu;
+        return d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;
+      };
       auto whole = [&](int t) { return words && t * kTilesKT >= key_lo && (t + 1) * kTilesKT <= key_hi; };
       auto look_up = [&](int t) {
         int block, slot;
@@ -649,20 +678,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             for (int d = 1; d < 8; d <<= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, d));
             return w;
           };
-          const uint32_t top = max(quarter_top(sc), is_v ? kLeastV : 27u);
-          uint32_t half[2] = {0u, 0u};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t d = top - ((sc >> (8 * r)) & 0xffu);
-            half[r >> 1] |= (d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u) << (16 * (r & 1));  // 2^-d as f16
-          }
-          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + lane * 8), "r"(half[0]), "r"(half[1]) : "memory");
+          const uint32_t high = quarter_top(sc) * 0x01010101u;
+          const bool own = far_apart(sc, high, spread);
+          const uint32_t top = __vmaxu4(high, least), d4 = shifts(own, sc, top);
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + lane * 8), "r"(down16(d4) | down16(d4 >> 8) << 16),
+                       "r"(down16(d4 >> 16) | down16(d4 >> 24) << 16) : "memory");
           if (!is_v) {
-            const uint32_t v_top = max(quarter_top(sv), kLeastV);
+            const uint32_t v_high = quarter_top(sv) * 0x01010101u, v_top = __vmaxu4(v_high, kLeastV * 0x01010101u);
+            const bool v_own = far_apart(sv, v_high, kSpreadV * 0x01010101u), any_own = own || v_own;
+            if (any_own) {
+              const uint32_t to = base + Cfg::kOwnAt + (tiles_in & 7) * 256 + lane * 4;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(own ? sc : top) : "memory");
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 128), "r"(v_own ? sv : v_top) : "memory");
+            }
             if ((lane & 7) == 0) {
               const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + (lane >> 3);
               asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(any_own ? 0u : v_top) : "memory");
             }
             ++tiles_in;
           }
@@ -733,21 +765,34 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           cp_async_wait<0>();
           fence_async_shared();  // a later TMA writes here
         }
+        uint32_t w = 0u, v = 0u, high = 0u, v_high = 0u;  // a byte of each word per quarter; rows that are not there have none
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t top = max(__reduce_max_sync(0xffffffffu, sc[q]), is_v ? kLeastV : 27u);
-          const uint32_t d = top - sc[q], half = d < 15u ? (15u - d) << 10 : d <= 24u ? 1u << (24u - d) : 0u;  // 2^-d as f16
-          asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + (32 * q + lane) * 2), "h"((uint16_t)half) : "memory");
-          if (!is_v) {
-            const uint32_t v_top = max(__reduce_max_sync(0xffffffffu, other[q]), kLeastV);
-            if (lane == 0) {
-              const uint32_t ref = base + Cfg::kRefAt + (tiles_in & 7) * 8 + q;
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref), "r"(top) : "memory");
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"(ref + 4), "r"(v_top) : "memory");
+          w |= sc[q] << (8 * q);
+          v |= other[q] << (8 * q);
+          high |= __reduce_max_sync(0xffffffffu, sc[q]) << (8 * q);
+          v_high |= __reduce_max_sync(0xffffffffu, other[q]) << (8 * q);
+        }
+        const bool own = far_apart(w, high, spread);
+        const uint32_t top = __vmaxu4(high, least), d4 = shifts(own, w, top);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + Cfg::kScaleAt + raw.slot * 256 + (32 * q + lane) * 2), "h"((uint16_t)down16(d4 >> (8 * q))) : "memory");
+        if (!is_v) {
+          const bool v_own = far_apart(v, v_high, kSpreadV * 0x01010101u), any_own = own || v_own;
+          const uint32_t v_top = __vmaxu4(v_high, kLeastV * 0x01010101u);
+          if (any_own) {  // rows that are not there are zeros: any power will do
+            const uint32_t to = base + Cfg::kOwnAt + (tiles_in & 7) * 256 + lane, k4 = own ? w : top, v4 = v_own ? v : v_top;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + 32 * q), "r"(k4 >> (8 * q)) : "memory");
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + 128 + 32 * q), "r"(v4 >> (8 * q)) : "memory");
             }
           }
+          if (lane == 0)
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base + Cfg::kRefAt + (tiles_in & 7) * 8), "r"(top), "r"(any_own ? 0u : v_top) : "memory");
+          ++tiles_in;
         }
-        if (!is_v) ++tiles_in;
         mbar_arrive(full);
         raw.next(Cfg::kStageRing);
       }
@@ -820,39 +865,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         // does any row of the warp see only a part of the tile?
         const bool edge = __any_sync(0xffffffffu, key0 + kTilesKT - 1 > last || key0 < first);
         const int hi = last - key0, lo = first - key0;           // columns [lo, hi] are seen
-        float x[4][32];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, x[q]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_wait_ld32(x[q]);
-        if (edge) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[q][i] = 32 * q + i <= hi && 32 * q + i >= lo ? x[q][i] : -INFINITY;
-        }
-        float part[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          part[q] = fmaxf(x[q][0], x[q][1]);
-#pragma unroll
-          for (int i = 2; i < 32; i += 2) part[q] = fmaxf(part[q], fmaxf(x[q][i], x[q][i + 1]));
-        }
-        float top;
-        if constexpr (FP8) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) part[q] = fmaf(part[q], cq[q], fq[q]);
-          top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        } else {
-          top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c_row;
-        }
-        const bool move = top > m + kMove || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, move)) {
+        // the reference follows a row's largest score; what has been added up so far is rescaled
+        auto follow = [&](float top) {
+          const bool move = top > m + kMove || (m == -INFINITY && top > m);
+          if (!__any_sync(0xffffffffu, move)) return;
           const float now = move ? top - kHead : m;
           const float keep = m == -INFINITY ? 0.f : exp2_fast(m - now);
-          if (done > 0) {  // rescale what has been added up so far
+          if (done > 0) {
             wait(BAR_PV_DONE + s, pv_phase ^ 1u, ST_EPILOGUE_WAIT);
-            if (!ok) break;
+            if (!ok) return;
             tc_fence_after();
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
@@ -868,28 +889,99 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             l2 = pack_f32x2(a * keep, b * keep);
           }
           m = now;
-        }
-        const float base_m = m == -INFINITY ? 0.f : m;
+        };
+        float x[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint64_t c2 = pack_f32x2(cq[q], cq[q]), neg = pack_f32x2(fq[q] - base_m, fq[q] - base_m);
-          uint64_t quarter = 0;
-          uint32_t w[16];
+        for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, x[q]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a, b;
-            unpack_f32x2(fma_f32x2(pack_f32x2(x[q][2 * i], x[q][2 * i + 1]), c2, neg), a, b);
-            a = exp2_fast(a);
-            b = exp2_fast(b);
-            if constexpr (FP8) quarter = add_f32x2(quarter, pack_f32x2(a, b));
-            else l2 = add_f32x2(l2, pack_f32x2(a, b));
-            w[i] = Mma<Op>::pack(a, b);
+        for (int q = 0; q < 4; ++q) tmem_wait_ld32(x[q]);
+        if (FP8 && __builtin_expect(__any_sync(0xffffffffu, f_bytes == 0u), 0)) {
+          // an own tile, 16 columns at a time: scores in log2 units, masked, go back to where they came from, then become P
+          const uint32_t powers = base + Cfg::kOwnAt + ((my_base + j) & 7) * 256;
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c16 = 0; c16 < 128; c16 += 16) {
+            uint32_t y[16];
+            tmem_ld16(tS + c16, y);
+            tmem_wait_ld16(y);
+            const uint4 kb = lds16(powers + c16), vb = lds16(powers + 128 + c16);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float score = __uint_as_float(y[i]) * c_row * e8m0_value(byte_of(kb, i));
+              const float z = c16 + i <= hi && c16 + i >= lo ? score : -INFINITY;
+              top = fmaxf(top, z + v_power(byte_of(vb, i)));
+              y[i] = __float_as_uint(z);
+            }
+            tmem_st16(tS + c16, y);
+          }
+          tmem_wait_st();
+          follow(top);
+          if (!ok) break;
+          const float base_m = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+          for (int c16 = 0; c16 < 128; c16 += 16) {
+            uint32_t y[16], w[8];
+            tmem_ld16(tS + c16, y);
+            tmem_wait_ld16(y);
+            const uint4 vb = lds16(powers + 128 + c16);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float z[2], pr[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                z[e] = __uint_as_float(y[i + e]);
+                const uint32_t b = byte_of(vb, i + e);
+                pr[e] = b == 255u && z[e] > -INFINITY ? __uint_as_float(0x7fffffffu) : exp2_fast(z[e] + v_power(b) - base_m);
+              }
+              l2 = add_f32x2(l2, pack_f32x2(exp2_fast(z[0] - base_m), exp2_fast(z[1] - base_m)));
+              w[i / 2] = Mma<Op>::pack(pr[0], pr[1]);
+            }
+            tmem_st8(tS + c16 / 2, w);  // over columns that have been read
+          }
+        } else {
+          if (edge) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[q][i] = 32 * q + i <= hi && 32 * q + i >= lo ? x[q][i] : -INFINITY;
+          }
+          float part[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            part[q] = fmaxf(x[q][0], x[q][1]);
+#pragma unroll
+            for (int i = 2; i < 32; i += 2) part[q] = fmaxf(part[q], fmaxf(x[q][i], x[q][i + 1]));
           }
           if constexpr (FP8) {
-            const float down = pow2_of(254u - ((f_bytes >> (8 * q)) & 0xffu));  // 2^-F
-            l2 = fma_f32x2(quarter, pack_f32x2(down, down), l2);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[q] = fmaf(part[q], cq[q], fq[q]);
+            follow(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+          } else {
+            follow(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c_row);
           }
-          tmem_st16(tS + 16 * q, w);  // P lies over the first half of S, which this thread holds in registers
+          if (!ok) break;
+          const float base_m = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint64_t c2 = pack_f32x2(cq[q], cq[q]), neg = pack_f32x2(fq[q] - base_m, fq[q] - base_m);
+            uint64_t quarter = 0;
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, b;
+              unpack_f32x2(fma_f32x2(pack_f32x2(x[q][2 * i], x[q][2 * i + 1]), c2, neg), a, b);
+              a = exp2_fast(a);
+              b = exp2_fast(b);
+              if constexpr (FP8) quarter = add_f32x2(quarter, pack_f32x2(a, b));
+              else l2 = add_f32x2(l2, pack_f32x2(a, b));
+              w[i] = Mma<Op>::pack(a, b);
+            }
+            if constexpr (FP8) {
+              const float down = pow2_of(254u - ((f_bytes >> (8 * q)) & 0xffu));  // 2^-F
+              l2 = fma_f32x2(quarter, pack_f32x2(down, down), l2);
+            }
+            tmem_st16(tS + 16 * q, w);  // P lies over the first half of S, which this thread holds in registers
+          }
         }
         tmem_wait_st();
         tc_fence_before();

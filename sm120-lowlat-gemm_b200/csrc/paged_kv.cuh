@@ -71,6 +71,11 @@ __device__ __forceinline__ int page_of(const PagedKV& c, int seq, int block) {
   return -1;
 }
 
+// 2^(b - 127), NaN for 255.
+__device__ __forceinline__ float e8m0_value(uint32_t b) {
+  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7fffffffu : b << 23);
+}
+
 // ---- attention ---------------------------------------------------------------------------------------------------
 // Rows of a sequence are packed token-major over the query heads that share a key/value head: row = token * group + head in
 // group. An item is (sequence, kv head, tile of whole tokens); it walks the key tiles that any of its rows sees. All items'

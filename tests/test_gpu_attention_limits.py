@@ -138,6 +138,54 @@ def test_steps_that_cross_the_end_of_the_cache(dtype):
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# powers of two of e4m3 rows
+
+
+def cached_row(cache, table, i, j):
+    return int(table[i, j // cache.shape[2]]), j % cache.shape[2]
+
+
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+@pytest.mark.parametrize("new,length,late,window", [(70, 70, 65, 0), (70, 400, 395, 0), (90, 300, 215, 8), (300, 300, 131, 0), (1, 70, 40, 8)])
+def test_rows_that_a_query_may_not_see_do_not_matter(new, length, late, window, which):
+    """One token's rows are 2^30 larger than their neighbours'. Queries before it, or whose window lies behind it, never see it."""
+    for qt, dim, page in ((BF, 128, 16), (HF, 64, 5)):
+        q, cache, kw, starts = setup([new], [length], 8, 2, dim, page, qt, E4M3, seed=late)
+        kc, vc, table, _ = cache
+        pg, slot = cached_row(kc, table, 0, late)
+        for n, s in (("k", kw["k_scale"]), ("v", kw["v_scale"])):
+            if n in which:
+                s.view(torch.uint8)[pg, :, slot] = 151
+        compare(q, cache, kw, starts, [length], window=window, shared=7)
+
+
+@pytest.mark.parametrize("qt", [BF, HF])
+@pytest.mark.parametrize("spread", [0, 7, 8, 15, 16, 24, 40])
+@pytest.mark.parametrize("new", [1, 70, 200])
+def test_row_scales_of_any_spread(new, spread, qt):
+    """Powers of two of neighbouring rows up to 2^spread apart: each query's error goes by what it sees, per element."""
+    for dim, page, slots_last in ((128, 16, False), (64, 24, True)):
+        q, cache, kw, starts = setup([new], [700], 8, 2, dim, page, qt, E4M3, seed=spread)
+        g = torch.Generator().manual_seed(spread)
+        for name in ("k_scale", "v_scale"):
+            s = kw[name].view(torch.uint8)
+            s.copy_(torch.randint(121 - spread, 122, s.shape, generator=g).to(torch.uint8))
+            if slots_last:  # scale bytes that do not lie together
+                kw[name] = s.transpose(1, 2).contiguous().transpose(1, 2).view(E8M0)
+        compare(q, cache, kw, starts, [700], shared=7)
+
+
+def test_rows_of_zeros_beside_others():
+    """A row of zeros has the smallest power of two: its neighbours keep theirs, and its key keeps its weight."""
+    for new in (1, 80):
+        q, cache, kw, starts = setup([new], [300], 8, 1, 128, 16, BF, E4M3, seed=new)
+        for c, s in ((cache[0], kw["k_scale"]), (cache[1], kw["v_scale"])):
+            c.view(torch.uint8)[:, :, ::3] = 0
+            s.view(torch.uint8)[:, :, ::3] = 27
+        compare(q, cache, kw, starts, [300], shared=7)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # weights far below the largest
 
 
