@@ -275,7 +275,7 @@ LLG_API int llg_tc_gemm_static_ws(const llg_tc_args* args, void* stream);
  * and slots and interleaved k / v allocations are views of it. Token j of sequence i is row
  * (page_table[i][j / page_size], head, j % page_size).
  * Element types: BF16 or F16, or E4M3 with one e8m0 byte b per row in k_scale / v_scale [pages, kv_heads, page_size] (any
- * strides, in bytes): a stored value x stands for x * 2^(b - 127).
+ * strides, in bytes): a stored value x stands for x * 2^(b - 127), for NaN where b is 255. llg_kv_append writes 27 to 246.
  * kv_lens[i] counts the tokens of sequence i in the cache, its new tokens included: they are the last ones. q_starts
  * [batch + 1] gives the rows of the new tokens in the per-token tensors; NULL: every sequence has tokens / batch of them
  * (tokens must be a multiple of batch). Rows at and behind q_starts[batch] belong to no sequence: they are neither read into
@@ -329,7 +329,8 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * does not see have no part in its result, whatever their powers are. Rows of 2^-100 or less (bytes up to 27) may count as zeros beside
  * larger ones. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
  * Weights go into the second product in 16 bits, BF16 over a BF16 cache, else F16: there a weight (times its V row's power of two) keeps
- * its bits down to 2^-21 of the largest and counts down to 2^-32. The row sum has fp32 weights; over E4M3 it counts them down to
+ * its bits down to 2^-21 of the largest and counts down to 2^-32 (over E4M3, where a kv head has many query rows, down to 2^-14 and
+ * 2^-25: 32 neighbouring keys share a power of two that may be 2^7 above their own). The row sum has fp32 weights; over E4M3 it counts them down to
  * 2^(E - min(e, 0) - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12. ws:
  * llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
 typedef struct llg_attn_args {

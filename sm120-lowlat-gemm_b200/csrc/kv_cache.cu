@@ -3,7 +3,8 @@
 // Writing. Row x of head_dim values: a = max |x|, e = smallest integer with a * 2^-e <= 448 (clamped to [-100, 119], -100 for a
 // zero row), stored e4m3(x * 2^-e), round to nearest even, saturating, and the byte e + 127. The multiply by a power of two is
 // exact, so the one rounding is the conversion's. An infinity saturates to 448 * 2^119, a NaN stays one. A 16-bit cache is a copy.
-// Reading. value * 2^e, one rounding to the output type (none for bf16 and fp32: four significant bits fit).
+// Reading. value * 2^e (NaN for byte 255), one rounding to the output type (none for bf16 and fp32 from byte 27 on: four significant
+// bits fit).
 //
 // Both move bytes. A CTA takes a few tokens: a thread per token finds its page and slot once, then the rows of all heads go
 // through, 16 values (append: of K's row and of V's) or 8 (read) per lane, a row on 4 to 32 lanes so that a row's maximum is a
@@ -180,8 +181,8 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// LPR lanes per row, 8 values per lane, so that a 16-bit row is written 16 bytes by 16 bytes without gaps; tokens [blockIdx.x * per, + per) of sequence blockIdx.y; blockIdx.z: K or V. Rows go
-// through in the order of the output.
+// LPR lanes per row, 8 values per lane, so that a 16-bit row is written 16 bytes by 16 bytes without gaps; tokens [blockIdx.x * per,
+// + per) of sequence blockIdx.y; blockIdx.z: K or V. Rows go through in the order of the output.
 template <typename T, bool FP8, int LPR>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadDev p, int per) {
   __shared__ Place where[kMaxTokens];
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
       if (r >= rows) break;
       unsigned char* const dst = out + ((int64_t)r * c.head_dim + sub * kValues) * (int64_t)sizeof(T);
       if constexpr (FP8) {
-        const float up = __uint_as_float(b[k] << 23);
+        const float up = e8m0_value(b[k]);
         const float2 x[4] = {e4m3x2_to_f32(raw[k].x & 0xffffu), e4m3x2_to_f32(raw[k].x >> 16), e4m3x2_to_f32(raw[k].y & 0xffffu),
                              e4m3x2_to_f32(raw[k].y >> 16)};
         float f[8];

@@ -211,3 +211,23 @@ def test_a_long_flat_tail_below_one_strong_key(new, batch, ct, strong):
     want, _, tol = expected(q[:new], kc.to(ct), vc.to(ct), kw["k_scale"], kw["v_scale"], table, [n], [0, new], scale=1.0)
     err = (out.double() - want).abs()
     assert bool((err <= tol).all()), f"error {err.max().item():.3e}, {(err / tol).max().item():.2f} of its bound"
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scale bytes that kv_append never writes
+
+
+@pytest.mark.parametrize("ot", [torch.float32, BF])
+def test_read_of_the_smallest_and_largest_scale_bytes(ot):
+    """value * 2^(byte - 127) from byte 0 to 254, NaN for byte 255."""
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    values = torch.arange(256, dtype=torch.uint8, device="cuda").view(E4M3)
+    kc = values.view(1, 1, 1, 256).expand(1, 1, 16, 256).contiguous()
+    byte = torch.tensor([0, 1, 2, 26, 27, 100, 127, 200, 246, 247, 253, 254, 255, 255, 0, 254], dtype=torch.uint8, device="cuda")
+    ks = byte.view(1, 1, 16).view(E8M0)
+    k, v = L.kv_read(kc, kc, table, torch.tensor([16], dtype=torch.int32, device="cuda"), 16, k_scale=ks, v_scale=ks, out_dtype=ot)
+    want = values.double()[None] * torch.exp2(byte.double() - 127)[:, None]
+    want[byte == 255] = math.nan
+    want = want.float().to(ot)  # the product is exact in fp32 up to its largest value
+    for x in (k, v):
+        assert torch.equal(x[0, :, 0].isnan(), want.isnan()) and torch.equal(x[0, :, 0].nan_to_num(), want.nan_to_num())
