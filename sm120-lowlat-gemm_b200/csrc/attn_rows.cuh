@@ -450,20 +450,21 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       const bool inner = key0 >= all_lo && key0 + 16 * SUB - 1 <= all_hi;
       float kf[SUB][2], vf[SUB][2], ve[SUB][2];  // keys krow, krow + 8 of a group: 2^e of K, 2^e and e of V
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
+      for (int u = 0; u < SUB; ++u) {
+        kf[u][0] = kf[u][1] = vf[u][0] = vf[u][1] = 1.f;
+        ve[u][0] = ve[u][1] = 0.f;
+        if constexpr (FP8) {
+          uint32_t bk[2], bv[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          kf[u][e] = vf[u][e] = 1.f;
-          ve[u][e] = 0.f;
-          if constexpr (FP8) {
-            uint32_t bk, bv;
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk) : "r"(sb + 32 * u + krow + 8 * e) : "memory");
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv) : "r"(sb + 32 * u + 16 + krow + 8 * e) : "memory");
-            kf[u][e] = pow2_of(bk);
-            vf[u][e] = pow2_of(bv);
-            ve[u][e] = __uint_as_float(0x4b000000u + max(bv, kLeastV)) - 8388735.f;  // e, not below -88: bits of 2^23 + b, less 2^23 + 127
+          for (int e = 0; e < 2; ++e) {
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk[e]) : "r"(sb + 32 * u + krow + 8 * e) : "memory");
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv[e]) : "r"(sb + 32 * u + 16 + krow + 8 * e) : "memory");
+            ve[u][e] = e8m0_power(bv[e], kLeastV);
           }
+          e8m0_values(bk[0], bk[1], kf[u][0], kf[u][1]);
+          e8m0_values(bv[0], bv[1], vf[u][0], vf[u][1]);
         }
+      }
       uint32_t pf[SUB][NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {

@@ -142,12 +142,11 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// An own tile's rows: byte i of sixteen, and the power of two of a row of V that m takes account of (byte 255, no number, reaches P).
+// Byte i of sixteen.
 __device__ __forceinline__ uint32_t byte_of(const uint4& v, int i) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   return (w[i >> 2] >> (8 * (i & 3))) & 0xffu;
 }
-__device__ __forceinline__ float v_power(uint32_t b) { return __uint_as_float(0x4b000000u + (b == 255u ? kLeastV : max(b, kLeastV))) - 8388735.f; }
 
 // Ring of mbarrier phases: slot i of n, used round after round.
 struct Ring {
@@ -909,7 +908,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             for (int i = 0; i < 16; ++i) {
               const float score = __uint_as_float(y[i]) * c_row * e8m0_value(byte_of(kb, i));
               const float z = c16 + i <= hi && c16 + i >= lo ? score : -INFINITY;
-              top = fmaxf(top, z + v_power(byte_of(vb, i)));
+              top = fmaxf(top, z + e8m0_power(byte_of(vb, i), kLeastV));
               y[i] = __float_as_uint(z);
             }
             tmem_st16(tS + c16, y);
@@ -931,7 +930,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
               for (int e = 0; e < 2; ++e) {
                 z[e] = __uint_as_float(y[i + e]);
                 const uint32_t b = byte_of(vb, i + e);
-                pr[e] = b == 255u && z[e] > -INFINITY ? __uint_as_float(0x7fffffffu) : exp2_fast(z[e] + v_power(b) - base_m);
+                pr[e] = b == 255u && z[e] > -INFINITY ? __uint_as_float(0x7fffffffu) : exp2_fast(z[e] + e8m0_power(b, kLeastV) - base_m);
               }
               l2 = add_f32x2(l2, pack_f32x2(exp2_fast(z[0] - base_m), exp2_fast(z[1] - base_m)));
               w[i / 2] = Mma<Op>::pack(pr[0], pr[1]);

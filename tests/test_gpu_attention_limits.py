@@ -231,3 +231,39 @@ def test_read_of_the_smallest_and_largest_scale_bytes(ot):
     want = want.float().to(ot)  # the product is exact in fp32 up to its largest value
     for x in (k, v):
         assert torch.equal(x[0, :, 0].isnan(), want.isnan()) and torch.equal(x[0, :, 0].nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_scale_byte_that_is_no_number(new, which):
+    """255 is NaN: queries that see the row get NaN (the row sum only where it is a key's), others what they got without it."""
+    length, late = 300, 299 if new == 1 else 290
+    q, cache, kw, starts = setup([new], [length], 8, 2, 128, 16, BF, E4M3, seed=new)
+    want, wl = L.paged_attention(q, *cache, return_lse=True, **kw)
+    pg, slot = cached_row(cache[0], cache[2], 0, late)
+    kw[which + "_scale"].view(torch.uint8)[pg, :, slot] = 255
+    out, lse = L.paged_attention(q, *cache, return_lse=True, **kw)
+    sees = torch.arange(length - new, length, device="cuda") >= late
+    assert bool(out[sees].isnan().all())
+    assert bool(out[~sees].isfinite().all())
+    if which == "k":
+        assert bool(lse[sees].isnan().all())
+    else:
+        assert bool(((lse - wl)[sees].abs() <= 2.0 ** -18 * (1 + wl[sees].abs() + 128)).all())
+    # another reference power of two, but the values of each row are exact either way: a rounding of P and of the result each
+    assert bool(((out.double() - want.double())[~sees].abs() <= 2.0 ** -7 * (want.double().abs() + 4.0)[~sees]).all())
+    assert bool(((lse - wl)[~sees].abs() <= 2.0 ** -18 * (1 + wl[~sees].abs() + 128)).all())
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("k_byte,v_byte", [(0, 127), (127, 227), (127, 0), (0, 0)])
+def test_attention_over_the_smallest_and_largest_scale_bytes(new, k_byte, v_byte):
+    """Every row has the same extreme power of two."""
+    q, cache, kw, starts = setup([new], [300], 8, 2, 128, 16, BF, E4M3, seed=9)
+    kw["k_scale"].view(torch.uint8)[:] = k_byte
+    kw["v_scale"].view(torch.uint8)[:] = v_byte
+    out, lse = L.paged_attention(q, *cache, return_lse=True, **kw)
+    want, wl, tol = expected(q, cache[0], cache[1], kw["k_scale"], kw["v_scale"], cache[2], [300], starts, shared=7)
+    # rows of less than 2^-100 may count as zeros
+    assert bool(((out.double() - want).abs() <= tol + 448 * 2.0 ** -100).all())
+    assert bool(((lse.double() - wl).abs() <= 2.0 ** -18 * (1 + wl.abs() + 128)).all())
