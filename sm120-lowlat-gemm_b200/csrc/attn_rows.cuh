@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[u][e] = s[u][nb][e] * (row_f[nb][e & 1] * kf[u][e >> 1]);
+            x[u][e] = s[u][nb][e] * row_f[nb][e & 1] * kf[u][e >> 1];  // in this order: the factors alone may pass fp32, and 0 stay 0
             if (!inner) {
               const int key = key0 + 16 * u + krow + (e >> 1) * 8;
               if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[u][e] = -INFINITY;

@@ -849,8 +849,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
           f_bytes = ref.y;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            // not 0, which would make NaN of a masked column's -inf (a row of zeros against rows of zeros: 2^-121 * 2^-100)
-            cq[q] = fmaxf(c_row * pow2_of((ref.x >> (8 * q)) & 0xffu), 1.17549435e-38f);
+            // not 0, which would make NaN of a masked column's -inf (a row of zeros against rows of zeros: 2^-121 * 2^-100), nor infinite,
+            // which would of a product of 0
+            cq[q] = fminf(fmaxf(c_row * pow2_of((ref.x >> (8 * q)) & 0xffu), 1.17549435e-38f), 3.40282347e38f);
             fq[q] = __uint_as_float(0x4b000000u + ((ref.y >> (8 * q)) & 0xffu)) - 8388735.f;  // F: bits of 2^23 + byte, less 2^23 + 127
           }
         } else {

@@ -267,3 +267,14 @@ def test_attention_over_the_smallest_and_largest_scale_bytes(new, k_byte, v_byte
     # rows of less than 2^-100 may count as zeros
     assert bool(((out.double() - want).abs() <= tol + 448 * 2.0 ** -100).all())
     assert bool(((lse.double() - wl).abs() <= 2.0 ** -18 * (1 + wl.abs() + 128)).all())
+
+
+def test_large_queries_at_right_angles_to_large_keys():
+    """Factors of a row of q and of a row of K beyond fp32 together: a product of zero stays zero."""
+    for new in (1, 70):
+        q, cache, kw, starts = setup([new], [300], 8, 2, 128, 16, BF, E4M3, seed=3)
+        q.zero_()
+        q[..., 0] = 2.0 ** 100
+        cache[0].view(torch.uint8)[..., 0] = 0
+        kw["k_scale"].view(torch.uint8)[:] = 230
+        compare(q, cache, kw, starts, [300])
