@@ -152,6 +152,14 @@ class DecodeStep:
             if cache.kv_heads != kv // (2 * cache.head_dim * tp) or len(cache.layers) != layers:
                 raise ValueError(f"the cache holds {len(cache.layers)} layers of {cache.kv_heads} kv heads, the step has {layers} of "
                                  f"{kv // (2 * cache.head_dim * tp)}")
+            # what paged_attention and kv_append would refuse in the middle of a step, after lengths have changed
+            heads = shape.hidden // (cache.head_dim * tp)
+            if cache.head_dim not in (64, 128):
+                raise ValueError(f"attention takes heads of 64 or 128, the cache has {cache.head_dim}")
+            if heads % cache.kv_heads or heads // cache.kv_heads > 32:
+                raise ValueError(f"{heads} query heads must be 1 to 32 times the {cache.kv_heads} kv heads")
+            if cache.dtype not in (FP8, self.act_dtype):
+                raise ValueError(f"a {kind} step's cache holds {FP8} or {self.act_dtype}, not {cache.dtype}")
             if api is None:
                 raise ValueError("a cache needs the library's own entry points")
         self.fuse_quant = fuse_quant  # FP8 with `comm`: all-reduce and the next activation quantizer as one kernel
@@ -245,7 +253,6 @@ class DecodeStep:
         if self.cache is not None:
             if x.shape[0] % self.cache.batch:
                 raise ValueError(f"{x.shape[0]} rows are no multiple of the cache's {self.cache.batch} sequences")
-            self.cache.kv_lens.add_(x.shape[0] // self.cache.batch)
         order = self._order()
         nxt_w = {order[i]: self.layers[order[(i + 1) % len(order)][0]].w[order[(i + 1) % len(order)][1]][0]
                  for i in range(len(order))}
@@ -254,6 +261,8 @@ class DecodeStep:
         for li, layer in enumerate(self.layers):
             qkv = self._project(h_in, *layer.w["qkv"], nxt_w[(li, "qkv")])
             if self.cache is not None:
+                if li == 0:  # behind the first projection: an x that it refuses leaves the cache as it was
+                    self.cache.kv_lens.add_(x.shape[0] // self.cache.batch)
                 attn = self._attend(qkv, li)
             else:
                 attn = qkv[:, :a_width]  # stand-in for this rank's attention heads' output

@@ -139,3 +139,15 @@ def test_decode_cache_holds_whole_pages():
     for asked, page, held in ((100, 16, 112), (64, 64, 64), (1, 64, 64), (65, 64, 128)):
         c = TP.DecodeCache(1, 2, asked, 1, "cpu", page_size=page)
         assert c.max_len == held == c.page_table.shape[1] * c.layers[0][0][0].shape[2]
+
+
+@pytest.mark.parametrize("hidden,kv_heads,cache,kind,text", [
+    (10 * 128, 4, {}, "bf16", "10 query heads"), (66 * 64, 2, dict(head_dim=64), "bf16", "66 query heads"),
+    (512, 2, dict(head_dim=32), "bf16", "64 or 128"), (1024, 2, dict(dtype=torch.bfloat16), "f16", "bfloat16"),
+    (1024, 2, dict(dtype=torch.float16), "w8a16_bf16", "float16")])
+def test_a_step_refuses_caches_that_it_cannot_attend_over(hidden, kv_heads, cache, kind, text):
+    """Before any step, so that lengths never run ahead of what is stored."""
+    c = TP.DecodeCache(1, 1, 8, kv_heads, "cpu", **cache)
+    shape = TP.LayerShape(hidden=hidden, qkv=hidden + 2 * kv_heads * c.head_dim, inter=256)
+    with pytest.raises(ValueError, match=text):
+        TP.DecodeStep(kind, 1, 1, 0, torch.device("cpu"), shape, cache=c)

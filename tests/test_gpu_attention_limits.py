@@ -137,6 +137,19 @@ def test_steps_that_cross_the_end_of_the_cache(dtype):
     assert N.device_status() == 0
 
 
+def test_a_refused_step_leaves_the_cache_alone():
+    dev = torch.device("cuda", 0)
+    cache = TP.DecodeCache(1, 2, 64, 2, dev)
+    step = TP.DecodeStep("bf16", 1, 1, 0, dev, SHAPE, cache=cache)
+    for x in (torch.zeros(2, 1000, dtype=BF, device=dev), torch.zeros(2, 1024, dtype=torch.float32, device=dev),
+              torch.zeros(3, 1024, dtype=BF, device=dev)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            step.run(x)
+        assert cache.kv_lens.tolist() == [0, 0]
+    step.run(torch.zeros(2, 1024, dtype=BF, device=dev))
+    assert cache.kv_lens.tolist() == [1, 1]
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # powers of two of e4m3 rows
 
