@@ -346,7 +346,8 @@ typedef struct llg_attn_args {
 
 LLG_API int llg_paged_attention(const llg_attn_args* args, void* stream);
 /* Bytes of scratch llg_paged_attention needs for these arguments on the current device (ws itself is not looked at): two partial
- * results per CTA, whatever the lengths are - up to 39 MB on 148 SMs where a kv head has many query rows, 10 MB where it has few.
+ * results per CTA, whatever the lengths are. On 148 SMs at most 39.5 MB where a kv head has many query rows, 7.5 MB where it has few, and
+ * both, 47 MB, with q_starts, which only the device reads.
  * Negative: LLG_E_*, also for calls of more key tiles (of 64 tokens, table_width * page_size of them per sequence and kv head) than
  * 31 bits count. */
 LLG_API int64_t llg_paged_attention_ws(const llg_attn_args* args);

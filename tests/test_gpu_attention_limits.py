@@ -1,5 +1,6 @@
 """Paged cache and attention where they can go wrong: the cache's end, rows that a query may not see, powers of two far apart,
 weights far below the largest."""
+import ctypes as C
 import math
 
 import pytest
@@ -291,3 +292,32 @@ def test_large_queries_at_right_angles_to_large_keys():
         cache[0].view(torch.uint8)[..., 0] = 0
         kw["k_scale"].view(torch.uint8)[:] = 230
         compare(q, cache, kw, starts, [300])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scratch
+
+
+def test_scratch_stays_within_the_documented_bounds():
+    """Of every row count, head dimension and type: 39.5 MB for many query rows, 7.5 MB for few, 47 MB for both, on 148 SMs."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    most = {}
+    for dtype in (1, 4):
+        for dim in (64, 128):
+            for group in (1, 5, 8, 16, 24, 32):
+                for new, starts in ((1, False), (2, False), (3, False), (4, False), (24, False), (32, False), (300, False), (1, True), (300, True)):
+                    a = N.AttnArgs()
+                    c = a.kv
+                    c.k, c.v, c.k_scale, c.v_scale = 4096, 8192, *((4096, 4096) if dtype == 4 else (None, None))
+                    c.k_stride = c.v_stride = (C.c_int64 * 3)(16 * dim, 16 * dim, dim)
+                    c.page_table, c.table_stride, c.kv_lens, c.q_starts = 4096, 4096, 4096, 4096 if starts else None
+                    c.dtype, c.pages, c.kv_heads, c.page_size, c.head_dim, c.table_width, c.batch = dtype, 64, 1, 16, dim, 4096, 64
+                    c.tokens = 64 * new
+                    a.q, a.out, a.q_dtype, a.heads, a.scale = 4096, 4096, 1, group, 0.1
+                    a.q_stride = a.out_stride = (C.c_int64 * 2)(group * dim, dim)
+                    need = N.lib.llg_paged_attention_ws(C.byref(a))
+                    assert need > 0
+                    kind = "both" if starts else "many" if new * group > 32 else "few" if new * group <= 24 else "either"
+                    most[kind] = max(most.get(kind, 0), need)
+    assert most["few"] <= 7.5e6 * sms / 148 and max(most["many"], most["either"]) <= 39.5e6 * sms / 148 and most["both"] <= 47e6 * sms / 148, most
+    assert most["both"] > 39.5e6 * sms / 148  # the sum is reached
