@@ -129,9 +129,9 @@ constexpr uint32_t kLeastV = 39;
 
 // CTAs of the few-row kernel that fit an SM: as many as its registers and rings of two to three tiles let in, which hides the chain
 // from a load to the next product better than longer rings (8 rows, decode batch over e4m3: two 74.5 us, three 65.3; 16-bit 51.8, 50.4;
-// 20 rows of 64 values: two of 32 rows 32.9, three of 24 29.4).
+// 20 rows of 64 values: two of 32 rows 32.9, three of 24 29.4). Not where registers would spill: 16 rows of 128 e4m3 values three 39.1, two 36.3.
 __host__ __device__ constexpr int rows_ctas_per_sm(bool fp8, int head_dim, int blocks) {
-  return blocks == 4 ? 2 : blocks == 3 ? (head_dim == 64 ? 3 : 2) : blocks == 2 ? (fp8 || head_dim == 64 ? 3 : 2) : fp8 || head_dim == 128 ? 3 : 4;
+  return blocks == 4 ? 2 : blocks == 3 ? (head_dim == 64 ? 3 : 2) : blocks == 2 ? (head_dim == 64 ? 3 : 2) : fp8 || head_dim == 128 ? 3 : 4;
 }
 
 // Keys [lo, hi) that any row of token tile [tf, tf + cnt) sees.
