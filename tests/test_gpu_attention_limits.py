@@ -199,6 +199,23 @@ def test_rows_of_zeros_beside_others():
         compare(q, cache, kw, starts, [300], shared=7)
 
 
+@pytest.mark.parametrize("ct", [BF, E4M3])
+@pytest.mark.parametrize("new", [3, 70])
+def test_a_key_that_is_no_number_reaches_who_sees_it(new, ct):
+    """A NaN among the keys: queries before it, or whose window lies behind it, keep their bits, the others are NaN."""
+    for bad, window in ((298, 0), (300 - new, 2)):
+        q, cache, kw, _ = setup([new], [300], 8, 2, 128, 16, BF, ct, seed=new, ragged=False)
+        want, wl = L.paged_attention(q, *cache, window=window, return_lse=True, **kw)
+        pg, slot = cached_row(cache[0], cache[2], 0, bad)
+        cache[0][pg, 1, slot, 7] = math.nan
+        out, lse = L.paged_attention(q, *cache, window=window, return_lse=True, **kw)
+        pos = torch.arange(300 - new, 300, device="cuda")
+        sees = (pos >= bad) & ((pos < bad + window) if window else True)
+        assert torch.equal(out[:, :4], want[:, :4]) and torch.equal(lse[:, :4], wl[:, :4])  # the other kv head
+        assert torch.equal(out[~sees], want[~sees]) and torch.equal(lse[~sees], wl[~sees])
+        assert bool(out[sees][:, 4:].isnan().all()) and bool(lse[sees][:, 4:].isnan().all())
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # weights far below the largest
 
