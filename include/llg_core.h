@@ -325,8 +325,9 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * sees key j when j <= position (causal) and j > position - window (window > 0); scores are scale * q . k, o = softmax v,
  * lse = log of the sum of exp(scores) (natural, fp32). A query that sees no key gives o = 0 and lse = -inf.
  * head_dim 64 or 128; q and out in the cache's 16-bit type, or either 16-bit type over E4M3; heads / kv_heads <= 32.
- * An E4M3 value is multiplied as F16 whatever q's type is, exactly; its row's power of two is applied in fp32, and keys that a query
- * does not see have no part in its result, whatever their powers are. Rows of 2^-100 or less (bytes up to 27) may count as zeros beside
+ * Keys that a query does not see have no part in its result, whatever their powers of two are, with one exception: an infinite or NaN
+ * value of v may reach every query of its sequence in the call, through a weight of zero (such a key only those that see it).
+ * An E4M3 value is multiplied as F16 whatever q's type is, exactly; its row's power of two is applied in fp32. Rows of 2^-100 or less (bytes up to 27) may count as zeros beside
  * larger ones. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
  * Weights go into the second product in 16 bits, BF16 over a BF16 cache, else F16: there a weight (times its V row's power of two) keeps
  * its bits down to 2^-21 of the largest and counts down to 2^-32 (over E4M3, where a kv head has many query rows, down to 2^-14 and

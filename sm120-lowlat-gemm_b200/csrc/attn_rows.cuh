@@ -157,8 +157,8 @@ __device__ __forceinline__ uint32_t rows_at(int row, int ch) {
 }
 
 template <typename T, bool FP8, int D, int NB>
-__global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas)) attn_rows_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v) {
+__global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
+    attn_rows_kernel(const __grid_constant__ AttnDev p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Cfg = RowsCfg<T, FP8, D, NB>;
   using Op = typename Cfg::Op;
   constexpr bool kToF16 = FP8 && std::is_same<T, __nv_bfloat16>::value;

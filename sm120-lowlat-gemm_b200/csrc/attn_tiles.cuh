@@ -22,16 +22,17 @@
 // keys) keep their powers of two relative to the quarter's largest, 2^E of K and 2^F of V, in the f16 values, which is exact down to
 // 2^-15 (4 of 11 bits); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
 // put the rest back where it costs nothing: score * (2^E, q's power) is the factor their multiply-add has anyway, and the
-// probability is 2^(s + F - m) with m the running maximum of s + F, so that P 2^-F V is what the product sums; the row sum takes
+// probability is 2^(s + F - m) with m following the maximum of s + F, so that P 2^-F V is what the product sums; the row sum takes
 // its quarters times 2^-F.
 // The quarter's largest may be a row that a query does not see, so a tile with rows further apart than that (V: 2^-7, the room that m
 // leaves above) is an own one: its values are widened as they are, and the softmax threads, which find every row's two powers in
-// shared memory, multiply each score by its own and take s + e of the keys that they see. A tile of that kind takes four to five times as long (a chunk
-// of 512 behind 8192 of nothing else 798 us instead of 168).
+// shared memory, multiply each score by its own and take s + e of the keys that they see. A tile of that kind takes four to five times
+// as long (a chunk of 512 behind 8192 of nothing else 798 us instead of 168): its code stays small, since code beside the loop that
+// always runs slows that down (176 and 183 us with the whole tile unrolled).
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
 // Measured, 64 heads over 8, head_dim 128: 2048 tokens behind 14k keys, bf16, 937 us (1.10 PFLOP/s, at the power cap); 512 behind
-// 8192, e4m3, 176 us (0.81 PFLOP/s: the loaders' conversions and their shared-memory traffic).
+// 8192, e4m3, 169 us (0.84 PFLOP/s: the loaders' conversions and their shared-memory traffic).
 // P is rounded to 16 bits (bf16 2^-8, f16 2^-11 relative); statistics and O stay in fp32, l sums the unrounded values.
 #pragma once
 

@@ -53,7 +53,7 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tens
             k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
     """The first max_len tokens of every sequence: (k, v), each [batch, max_len, kv_heads, head_dim], zero behind kv_lens.
     out_dtype: a 16-bit cache's own type (the default there), or bf16 (default), f16 or f32 for an e4m3 cache; bf16 and f32
-    hold value * scale exactly, f16 rounds where its range ends."""
+    hold value * scale exactly (of every row that kv_append wrote), f16 rounds where its range ends."""
     if max_len < 0:
         raise ValueError(f"lowlat_gemm: max_len must not be negative, got {max_len}")
     e4m3 = k_cache.dtype == torch.float8_e4m3fn
@@ -76,8 +76,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     same h // (heads / kv_heads) share a kv head, up to 32 of them. scale: 1 / sqrt(head_dim) unless given. causal: query t of
     a sequence's n sees keys up to its own position kv_len - n + t. window > 0: only the last `window` keys up to there.
     A query that sees nothing (an empty sequence, fewer cached tokens than new ones) gives zeros and lse = -inf. Rows of q
-    behind the last sequence are left as they were in `out`. Forward only, like every call of this package. An infinite or NaN key or value reaches every query of its
-    sequence's call, also through weights of zero."""
+    behind the last sequence are left as they were in `out`. Forward only, like every call of this package.
+
+    Sums, maxima and lse are fp32; the weights are rounded to 16 bits for their product with v: bf16 over a bf16 cache, else f16,
+    where a weight times its v row's power of two counts down to 2^-25 of the largest at the least. e4m3 values are multiplied
+    exactly; a bf16 q over them goes to f16 row by row, where its values 2^-28 below the row's largest lose bits.
+    A key that a query does not see has no part in its result. There is one exception: an infinite or NaN value of v may reach
+    every query of its sequence in the call, through a weight of zero; an infinite or NaN key reaches the queries that see it."""
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
