@@ -311,7 +311,8 @@ typedef struct llg_kv_append_args {
 LLG_API int llg_kv_append(const llg_kv_append_args* args, void* stream);
 
 /* Reads the first max_len tokens of every sequence back: k_out and v_out [batch, max_len, kv_heads, head_dim], contiguous,
- * zero behind kv_lens[i]; at most 65535 sequences. kv.q_starts and kv.tokens are not used. out_dtype: the cache's for BF16 / F16; BF16, F16 or F32 for E4M3. */
+ * zero behind kv_lens[i]; at most 65535 sequences. kv.q_starts and kv.tokens are not used. out_dtype:
+ * the cache's for BF16 / F16; BF16, F16 or F32 for E4M3. */
 typedef struct llg_kv_read_args {
   llg_paged_kv kv;
   void* k_out; void* v_out;
@@ -327,13 +328,14 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * head_dim 64 or 128; q and out in the cache's 16-bit type, or either 16-bit type over E4M3; heads / kv_heads <= 32.
  * Keys that a query does not see have no part in its result, whatever their powers of two are, with one exception: an infinite or NaN
  * value of v may reach every query of its sequence in the call, through a weight of zero (such a key only those that see it).
- * An E4M3 value is multiplied as F16 whatever q's type is, exactly; its row's power of two is applied in fp32. Rows of 2^-100 or less (bytes up to 27) may count as zeros beside
- * larger ones. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
+ * An E4M3 value is multiplied as F16 whatever q's type is, exactly; its row's power of two is applied in fp32. Rows of 2^-100 or less
+ * (bytes up to 27) may count as zeros beside larger ones. A BF16 row of q is brought to F16 by a power of two; its values 2^-28 below its largest lose bits.
  * Weights go into the second product in 16 bits, BF16 over a BF16 cache, else F16: there a weight (times its V row's power of two) keeps
  * its bits down to 2^-21 of the largest and counts down to 2^-32 (over E4M3, where a kv head has many query rows, down to 2^-14 and
  * 2^-25: 32 neighbouring keys share a power of two that may be 2^7 above their own). The row sum has fp32 weights; over E4M3 it counts them down to
- * 2^(E - min(e, 0) - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12. ws:
- * llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is expected in it or kept. */
+ * 2^(E - min(e, 0) - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12.
+ * ws: llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is
+ * expected in it or kept. */
 typedef struct llg_attn_args {
   llg_paged_kv kv;
   const void* q; int64_t q_stride[2];            /* token, head; elements, multiples of 16 bytes */

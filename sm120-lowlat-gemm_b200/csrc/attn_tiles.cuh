@@ -60,7 +60,7 @@ struct TilesCfg {
   static constexpr int kRing = kQ + 2 * kTile;
   static constexpr int kStageAt = kRing + kSlots * kTile;
   static constexpr int kScaleAt = kStageAt + kStageRing * kStage;  // [kStageRing][128] f16: a staged row's factor
-  static constexpr int kRefAt = kScaleAt + kStageRing * 256;       // [8 key tiles][8] bytes: E and F of the quarters, biased by 127; no F: an own tile
+  static constexpr int kRefAt = kScaleAt + kStageRing * 256;       // [8 key tiles][8] bytes: biased E and F of the quarters; F 0: an own tile
   static constexpr int kQFacAt = kRefAt + (FP8 ? 64 : 0);          // [2 items][256] floats: the power of two of a row of q
   static constexpr int kOwnAt = kQFacAt + (FP8 ? 2048 : 0);        // [8 key tiles][2][128] bytes: powers of two of an own tile's rows of K, of V
   static constexpr int kSmem = kOwnAt + (FP8 ? 2048 : 0) + 1024;   // + alignment slack
