@@ -828,6 +828,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
       const int last = !live ? INT_MAX : p.causal ? min(pos, g.s.len - 1) : g.s.len - 1;
       const int first = live && p.window > 0 ? pos - p.window + 1 : 0;
       float m = -INFINITY;                                       // reference of the probabilities: scores in log2 units (+ F)
+      bool huge = false;                                         // kHuge, in a row of the warp
       float c_row = p.scale_log2;
       uint64_t l2 = 0;                                           // two partial row sums
       int done = 0;                                              // key tiles of this stream behind us
@@ -890,6 +891,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             l2 = pack_f32x2(a * keep, b * keep);
           }
           m = now;
+          huge = __any_sync(0xffffffffu, fabsf(m) > kHuge && m > -INFINITY);
         };
         float x[4][32];
 #pragma unroll
@@ -961,6 +963,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             follow(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c_row);
           }
           if (!ok) break;
+          if (__builtin_expect(huge, 0)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint64_t c2 = pack_f32x2(cq[q], cq[q]), f2 = pack_f32x2(fq[q], fq[q]);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[q][i], x[q][i + 1]), c2, f2), x[q][i], x[q][i + 1]);
+              cq[q] = 1.f;
+              fq[q] = 0.f;
+            }
+          }
           const float base_m = m == -INFINITY ? 0.f : m;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {

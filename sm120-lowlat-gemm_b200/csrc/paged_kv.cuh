@@ -126,6 +126,9 @@ constexpr float kHead = 7.f, kMove = 15.f;
 // Least power of two of a row of V (biased by 127) that the maximum takes account of: row sums, up to 2^(15 + 88) a key, stay in fp32.
 // Smaller rows are multiplied by their power all the same.
 constexpr uint32_t kLeastV = 39;
+// Scores of 2^22 and more have a last bit of half a power of two and more: there products are rounded before m, which was, is taken off
+// (a multiply-add would be off by powers of two, and f16 ends from scores of 2^27 on).
+constexpr float kHuge = 4194304.f;
 
 // CTAs of the few-row kernel that fit an SM: as many as its registers and rings of two to three tiles let in, which hides the chain
 // from a load to the next product better than longer rings (8 rows, decode batch over e4m3: two 74.5 us, three 65.3; 16-bit 51.8, 50.4;

@@ -311,6 +311,34 @@ def test_large_queries_at_right_angles_to_large_keys():
         compare(q, cache, kw, starts, [300])
 
 
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("qt,ct,size", [(HF, HF, 8000.0), (BF, BF, 2.0 ** 20), (BF, BF, 2.0 ** 45), (BF, E4M3, 2.0 ** 45), (HF, E4M3, 2.0 ** 15)])
+def test_scores_beyond_what_a_rounding_of_fp32_leaves(new, qt, ct, size):
+    """Scores of 2^25 and far more, where the last bit of a product is worth powers of two: the largest still has all of the weight."""
+    q, cache, kw, _ = setup([new], [300], 8, 2, 128, 16, qt, ct, seed=new, ragged=False)
+    g = torch.Generator().manual_seed(31)
+    q.copy_(size * (1 + 0.25 * torch.rand(q.shape, generator=g)))
+    k = cache[0].view(torch.uint8) if ct == E4M3 else cache[0]
+    j = torch.arange(300, device="cuda")
+    pg, slot = cache[2][0].long()[j // 16], j % 16
+    rows = -(1 + 0.25 * torch.rand(300, 2, 128, generator=g)).cuda()  # all far below
+    rows[17] = 1 + 0.25 * torch.rand(2, 128, generator=g).cuda()
+    if ct == E4M3:
+        k[pg, :, slot] = (256 * rows).to(E4M3).view(torch.uint8)
+        kw["k_scale"].view(torch.uint8)[:] = min(127 + int(math.log2(size)), 190)
+    else:
+        k[pg, :, slot] = (size * rows).to(ct)
+    out, lse = L.paged_attention(q, *cache, return_lse=True, **kw)
+    want = rows_of(cache[1], kw["v_scale"], cache[2], 0, 300)[17].repeat_interleave(4, 0).expand(new, 8, 128)
+    key = rows_of(cache[0], kw["k_scale"], cache[2], 0, 300)[17].repeat_interleave(4, 0)
+    half = torch.finfo(qt).eps / 2
+    # half a step of the result and of the one weight, whose exponential is off by 2^-21
+    assert bool(((out.double() - want).abs() <= (2 * half + 2.0 ** -20) * want.abs() + torch.finfo(qt).tiny).all())
+    score = (q.double() * key).sum(-1) / 128 ** 0.5
+    # 128 products and sums of one sign, the scale, log2 and back: 2^-24 each of the score
+    assert bool(((lse.double() - score).abs() <= 136 * 2.0 ** -24 * score).all())
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # scratch
 
