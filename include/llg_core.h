@@ -333,7 +333,7 @@ LLG_API int llg_kv_read(const llg_kv_read_args* args, void* stream);
  * Weights go into the second product in 16 bits, BF16 over a BF16 cache, else F16: there a weight (times its V row's power of two) keeps
  * its bits down to 2^-21 of the largest and counts down to 2^-32 (over E4M3, where a kv head has many query rows, down to 2^-14 and
  * 2^-25: 32 neighbouring keys share a power of two that may be 2^7 above their own, and rows of zeros take any). The row sum has fp32 weights; over E4M3 it counts them down to
- * 2^(E - min(e, 0) - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12.
+ * 2^(E - e - 133) of the largest, 2^e being the key's own power of V (no less than 2^-88) and 2^E the largest: 2^-33 for E up to 12.
  * ws: llg_paged_attention_ws() bytes of scratch, 16-byte aligned, for the stream's use until the call's kernels have run; nothing is
  * expected in it or kept. */
 typedef struct llg_attn_args {

@@ -14,8 +14,8 @@
 //     transposition, and so are the orders of the keys and of head_dim's blocks among the lanes, which keep the reads of the
 //     TMA's swizzle free of bank conflicts. One cvt makes two f16 of two values, exactly, so both products run in f16 whatever q's
 //     type is: a bf16 row of q is brought to f16 by a power of two (its largest value to 2^14; values 2^-28 below that and less
-//     lose bits). The scores take the powers of two of q's and K's rows in fp32; V's goes to the probability, p 2^e, and the
-//     running maximum is that of s + e, so p 2^e <= 2^15 and keeps f16's 11 bits where it matters.
+//     lose bits). The scores take the powers of two of q's and K's rows in fp32; V's goes to the probability, 2^(s + e - m) with m
+//     following the maximum of s + e, which is at most 2^15 and keeps f16's 11 bits where it matters; l takes it times 2^-e.
 // P is rounded to the operand type of the second product (bf16 2^-8, f16 2^-11 relative); l sums the unrounded fp32 values.
 // Measured: 32 sequences of 0.9k to 8.2k keys, 64 heads over 8, e4m3, 65.7 us (4.4 TB/s); 4 of 50k to 65k, bf16, 50.4 us (5.2 TB/s).
 // m moves only when a score exceeds the largest so far by more than 2^8, so the shuffles and the rescaling of O are skipped for almost
@@ -448,21 +448,31 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
       // ---- softmax
       const int key0 = key_of(t);
       const bool inner = key0 >= all_lo && key0 + 16 * SUB - 1 <= all_hi;
-      float kf[SUB][2], vf[SUB][2], ve[SUB][2];  // keys krow, krow + 8 of a group: 2^e of K, 2^e and e of V
+      float kf[SUB][2], ve[SUB][2], out[SUB][2], left[SUB][2];  // keys krow, krow + 8 of a group: 2^e of K; of V: e, 2^-e, what is left
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        kf[u][0] = kf[u][1] = vf[u][0] = vf[u][1] = 1.f;
-        ve[u][0] = ve[u][1] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          kf[u][e] = out[u][e] = left[u][e] = 1.f;
+          ve[u][e] = 0.f;
+        }
         if constexpr (FP8) {
           uint32_t bk[2], bv[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bk[e]) : "r"(sb + 32 * u + krow + 8 * e) : "memory");
             asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bv[e]) : "r"(sb + 32 * u + 16 + krow + 8 * e) : "memory");
-            ve[u][e] = e8m0_power(bv[e], kLeastV);
           }
           e8m0_values(bk[0], bk[1], kf[u][0], kf[u][1]);
-          e8m0_values(bv[0], bv[1], vf[u][0], vf[u][1]);
+          float vf[2];
+          e8m0_values(bv[0], bv[1], vf[0], vf[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t c = carried(bv[e], kLeastV);
+            ve[u][e] = power_of(c);
+            out[u][e] = power_out(c);
+            left[u][e] = least_of_both(vf[e] * 0x1p88f, 1.f);  // 2^(127 - kLeastV)
+          }
         }
       }
       uint32_t pf[SUB][NB][2];
@@ -475,19 +485,20 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[u][e] = s[u][nb][e] * row_f[nb][e & 1] * kf[u][e >> 1];  // in this order: the factors alone may pass fp32, and 0 stay 0
+            if constexpr (FP8) x[u][e] = s[u][nb][e] * finite_product(row_f[nb][e & 1], kf[u][e >> 1]) + ve[u][e >> 1];
+            else x[u][e] = s[u][nb][e] * row_f[nb][e & 1];
             if (!inner) {
               const int key = key0 + 16 * u + krow + (e >> 1) * 8;
               if (key > last_key[nb][e & 1] || key < first_key[nb][e & 1]) x[u][e] = -INFINITY;
             }
-            more |= x[u][e] + ve[u][e >> 1] > m[nb][e & 1] + kMove;
+            more |= x[u][e] > m[nb][e & 1] + kMove;
           }
         if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) mx = fmaxf(mx, fmaxf(x[u][e] + ve[u][0], x[u][e + 2] + ve[u][1]));
+            for (int u = 0; u < SUB; ++u) mx = fmaxf(mx, fmaxf(x[u][e], x[u][e + 2]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -509,10 +520,11 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsCfg<T, FP8, D, NB>::kCtas))
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             pr[e] = exp2_fast(x[u][e] - base[e & 1]);
-            l[nb][e & 1] += pr[e];
+            if constexpr (FP8) l[nb][e & 1] = fmaf(pr[e], out[u][e >> 1], l[nb][e & 1]);
+            else l[nb][e & 1] += pr[e];
           }
-          pf[u][nb][0] = transpose8x8(Mma<Op>::pack(pr[0] * vf[u][0], pr[1] * vf[u][0]));
-          pf[u][nb][1] = transpose8x8(Mma<Op>::pack(pr[2] * vf[u][1], pr[3] * vf[u][1]));
+          pf[u][nb][0] = transpose8x8(Mma<Op>::pack(pr[0] * left[u][0], pr[1] * left[u][0]));
+          pf[u][nb][1] = transpose8x8(Mma<Op>::pack(pr[2] * left[u][1], pr[3] * left[u][1]));
         }
       }
 

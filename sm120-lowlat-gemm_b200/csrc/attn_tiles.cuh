@@ -23,11 +23,11 @@
 // 2^-15 (4 of 11 bits); rows of bf16 queries are brought to f16 by a power of two each. The softmax threads
 // put the rest back where it costs nothing: score * (2^E, q's power) is the factor their multiply-add has anyway, and the
 // probability is 2^(s + F - m) with m following the maximum of s + F, so that P 2^-F V is what the product sums; the row sum takes
-// its quarters times 2^-F.
+// its quarters (an own tile's: its keys) times 2^-F.
 // The quarter's largest may be a row that a query does not see, so a tile with rows further apart than that (V: 2^-7, the room that m
 // leaves above) is an own one: its values are widened as they are, and the softmax threads, which find every row's two powers in
-// shared memory, multiply each score by its own and take s + e of the keys that they see. A tile of that kind takes four to five times
-// as long (a chunk of 512 behind 8192 of nothing else 798 us instead of 168): its code stays small, since code beside the loop that
+// shared memory, multiply each score by its own and take s + e of the keys that they see. A tile of that kind takes four times as
+// long (a chunk of 512 behind 8192 of nothing else 675 us instead of 169): its code stays small, since code beside the loop that
 // always runs slows that down (176 and 183 us with the whole tile unrolled).
 // (Gathering every tile with cp.async was measured first: the proxy fence between a thread's copies and the tensor core's reads
 // waits for all of the thread's copies in flight, 2600 cycles per 32 KB tile.)
@@ -910,9 +910,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             const uint4 kb = lds16(powers + c16), vb = lds16(powers + 128 + c16);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float score = __uint_as_float(y[i]) * c_row * e8m0_value(byte_of(kb, i));
+              const float score = __uint_as_float(y[i]) * finite_product(c_row, e8m0_value(byte_of(kb, i))) + power_of(carried(byte_of(vb, i), kLeastV));
               const float z = c16 + i <= hi && c16 + i >= lo ? score : -INFINITY;
-              top = fmaxf(top, z + e8m0_power(byte_of(vb, i), kLeastV));
+              top = fmaxf(top, z);
               y[i] = __float_as_uint(z);
             }
             tmem_st16(tS + c16, y);
@@ -929,15 +929,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             const uint4 vb = lds16(powers + 128 + c16);
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              float z[2], pr[2];
+              float pr[2], out[2], pv[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                z[e] = __uint_as_float(y[i + e]);
                 const uint32_t b = byte_of(vb, i + e);
-                pr[e] = b == 255u && z[e] > -INFINITY ? __uint_as_float(0x7fffffffu) : exp2_fast(z[e] + e8m0_power(b, kLeastV) - base_m);
+                pr[e] = exp2_fast(__uint_as_float(y[i + e]) - base_m);
+                out[e] = power_out(carried(b, kLeastV));
+                pv[e] = b == 255u && pr[e] != 0.f ? __uint_as_float(0x7fffffffu) : pr[e];
               }
-              l2 = add_f32x2(l2, pack_f32x2(exp2_fast(z[0] - base_m), exp2_fast(z[1] - base_m)));
-              w[i / 2] = Mma<Op>::pack(pr[0], pr[1]);
+              l2 = fma_f32x2(pack_f32x2(pr[0], pr[1]), pack_f32x2(out[0], out[1]), l2);
+              w[i / 2] = Mma<Op>::pack(pv[0], pv[1]);
             }
             tmem_st8(tS + c16 / 2, w);  // over columns that have been read
           }

@@ -76,6 +76,14 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
   return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7fffffffu : b << 23);
 }
 
+__device__ __forceinline__ float least_of_both(float a, float b) {  // NaN if either is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// A product of two factors, no larger than the largest float (a product of 0 with it stays 0).
+__device__ __forceinline__ float finite_product(float a, float b) { return least_of_both(a * b, 3.40282347e38f); }
+
 // Two of them at a time by one conversion (selects for 0 and 255 cost the few-row kernel 1.5 us of 66).
 __device__ __forceinline__ void e8m0_values(uint32_t b0, uint32_t b1, float& f0, float& f1) {
   uint32_t r;
@@ -83,10 +91,12 @@ __device__ __forceinline__ void e8m0_values(uint32_t b0, uint32_t b1, float& f0,
   f0 = __uint_as_float(r << 16);
   f1 = __uint_as_float(r & 0xffff0000u);
 }
-// The power of two of a row of V that the attention's running maximum takes account of (kLeastV: below); 255, no number, is the values' affair.
-__device__ __forceinline__ float e8m0_power(uint32_t b, uint32_t least) {
-  return __uint_as_float(0x4b000000u + (b == 255u ? least : max(b, least))) - 8388735.f;  // bits of 2^23 + byte, less 2^23 + 127
-}
+// Probabilities carry the power of two of V's row, 2^(score + e - m): its byte as carried (255, no number, is the values' affair), e, and
+// 2^-e, which takes it out of the row sum again. That the sum adds up the very exponentials that the values are multiplied with is
+// what keeps them in step where a large score swallows e.
+__device__ __forceinline__ uint32_t carried(uint32_t b, uint32_t least) { return b == 255u ? least : max(b, least); }
+__device__ __forceinline__ float power_of(uint32_t c) { return __uint_as_float(0x4b000000u + c) - 8388735.f; }  // bits of 2^23 + c, less 2^23 + 127
+__device__ __forceinline__ float power_out(uint32_t c) { return __uint_as_float(c == 254u ? 0x00400000u : (254u - c) << 23); }
 
 // ---- attention ---------------------------------------------------------------------------------------------------
 // Rows of a sequence are packed token-major over the query heads that share a key/value head: row = token * group + head in
@@ -123,8 +133,8 @@ struct AttnDev {
 // largest of a row lies between 2^7 and 2^15. f16 ends at 2^15.99 and, with full accuracy, at 2^-14, so keys down to 2^-21 of the
 // largest keep their bits and keys down to 2^-32 are counted (a largest probability of 1 to 2^8 lost 131k keys 2^-25.3 below one).
 constexpr float kHead = 7.f, kMove = 15.f;
-// Least power of two of a row of V (biased by 127) that the maximum takes account of: row sums, up to 2^(15 + 88) a key, stay in fp32.
-// Smaller rows are multiplied by their power all the same.
+// Least power of two of a row of V (biased by 127) that the probabilities carry: row sums, up to 2^(15 + 88) a key, stay in fp32. What
+// smaller rows have below it stays with their values.
 constexpr uint32_t kLeastV = 39;
 // Scores of 2^22 and more have a last bit of half a power of two and more: there products are rounded before m, which was, is taken off
 // (a multiply-add would be off by powers of two, and f16 ends from scores of 2^27 on).

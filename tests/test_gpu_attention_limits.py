@@ -312,6 +312,52 @@ def test_large_queries_at_right_angles_to_large_keys():
 
 
 @pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("byte,alone", [(87, True), (87, False), (246, True), (246, False)])
+def test_factors_at_both_ends_of_the_range(byte, alone, new):
+    """Queries of 2^115 over keys of 2^-40, queries of 1 over keys as large as a saturated infinity: the one key with a score has all
+    of the weight, and its score is the lse. `alone`: only that key's power of two is extreme."""
+    q, cache, kw, _ = setup([new], [300], 8, 2, 128, 16, BF, E4M3, seed=byte, ragged=False)
+    q.zero_()
+    q[..., 0] = 2.0 ** 115 if byte == 87 else 1.0
+    pg, slot = cached_row(cache[0], cache[2], 0, 17)
+    cache[0].view(torch.uint8)[:] = 0
+    cache[0][pg, :, slot, 0] = 448.0
+    ks = kw["k_scale"].view(torch.uint8)
+    if not alone:
+        ks[:] = byte
+    ks[pg, :, slot] = byte
+    out, lse = L.paged_attention(q, *cache, return_lse=True, **kw)
+    want = rows_of(cache[1], kw["v_scale"], cache[2], 0, 300)[17].repeat_interleave(4, 0).expand(new, 8, 128)
+    # half a step of the result; a largest weight of 1 and a row sum of 1 are exact up to the exponential's 2^-21 and fp32's 2^-24 each
+    assert bool(((out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -20) * want.abs()).all())
+    score = q[0, 0, 0].double() * 448 * 2.0 ** (byte - 127) / 128 ** 0.5
+    assert bool(((lse.double() - score).abs() <= 2.0 ** -18 * score).all())
+
+
+@pytest.mark.parametrize("new", [1, 3, 70])
+@pytest.mark.parametrize("v_byte", [121, 137, 151, 190])
+@pytest.mark.parametrize("k_byte", [135, 151, 200])
+def test_a_row_far_above_the_others_is_the_result_of_who_sees_it(k_byte, v_byte, new):
+    """A key of a huge score whose value has a large power of two, too: neither drowns the other. Queries before it are their own."""
+    length, late = 300, 300 - (new + 1) // 2
+    q, cache, kw, starts = setup([new], [length], 8, 2, 128, 16, BF, E4M3, seed=k_byte, ragged=False)
+    q[..., 0] = 8.0
+    pg, slot = cached_row(cache[0], cache[2], 0, late)
+    cache[0].view(torch.uint8)[pg, :, slot] = 0
+    cache[0][pg, :, slot, 0] = 448.0
+    kw["k_scale"].view(torch.uint8)[pg, :, slot], kw["v_scale"].view(torch.uint8)[pg, :, slot] = k_byte, v_byte
+    out, lse = L.paged_attention(q, *cache, return_lse=True, **kw)
+    want, wl, tol = expected(q, cache[0], cache[1], kw["k_scale"], kw["v_scale"], cache[2], [length], starts, shared=7)
+    sees = torch.arange(length - new, length, device="cuda") >= late
+    v = rows_of(cache[1], kw["v_scale"], cache[2], 0, length)[late].repeat_interleave(4, 0)
+    score = 8.0 * 448 * 2.0 ** (k_byte - 127) / 128 ** 0.5  # 2^16 and more, the others' at most 2^10
+    assert bool(((out.double() - v)[sees].abs() <= (2.0 ** -7 + 2.0 ** -20) * v.abs()).all())  # the result's and the one weight's rounding
+    assert bool(((lse.double() - score)[sees].abs() <= 2.0 ** -18 * score).all())
+    assert bool(((out.double() - want).abs() <= tol)[~sees].all())
+    assert bool(((lse.double() - wl)[~sees].abs() <= 2.0 ** -18 * (1 + wl[~sees].abs() + 128)).all())
+
+
+@pytest.mark.parametrize("new", [1, 70])
 @pytest.mark.parametrize("qt,ct,size", [(HF, HF, 8000.0), (BF, BF, 2.0 ** 20), (BF, BF, 2.0 ** 45), (BF, E4M3, 2.0 ** 45), (HF, E4M3, 2.0 ** 15)])
 def test_scores_beyond_what_a_rounding_of_fp32_leaves(new, qt, ct, size):
     """Scores of 2^25 and far more, where the last bit of a product is worth powers of two: the largest still has all of the weight."""
